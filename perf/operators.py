@@ -40,34 +40,34 @@ def logprobs_case(tokens, vocab, dtype="bf16", targets=1, top_k=0, temperature=1
 def listed():
     return [
         # the gate of one decoded token: 512 experts, hidden 2048, logits kept in 32 bits
-        linear_case(1, 512, 2048, out="f32", name="linear gate, 1 token"),
+        linear_case(1, 512, 2048, out="f32", name="linear gate 1 token"),
         # a decode batch through a dense layer: the weights' bytes are the work
-        linear_case(64, 8192, 2048, activation="silu", bias=True, name="linear up, 64 tokens"),
+        linear_case(64, 8192, 2048, activation="silu", bias=True, name="linear up 64 tokens"),
         # a pruned layer: no size is a multiple of anything, rows start at odd addresses
         linear_case(333, 1001, 1999, dtype="f16", activation="gelu", bias=True, residual=True,
-                    name="linear ragged, 333 tokens"),
+                    name="linear ragged 333 tokens"),
         # a prompt through a dense layer: the products are the work
-        linear_case(8192, 8192, 2048, activation="gelu_tanh", bias=True, name="linear up, 8192 tokens"),
+        linear_case(8192, 8192, 2048, activation="gelu_tanh", bias=True, name="linear up 8192 tokens"),
         # the same layer's way back onto the residual stream
-        linear_case(4096, 2048, 8192, residual=True, name="linear down, 4096 tokens"),
+        linear_case(4096, 2048, 8192, residual=True, name="linear down 4096 tokens"),
         # one decoded token's routing: latency alone
         route_case(1, 512, 10, dtype="bf16", bias=True, groups=8, top_groups=4, group_top=2,
-                   name="route, 1 token"),
+                   name="route 1 token"),
         # a small ragged batch, softmax scores, limited to groups, some experts out of service
         route_case(61, 160, 6, scoring="softmax", groups=8, top_groups=3, group_top=1, renormalize=False, scale=16.0,
-                   masked=0.1, name="route softmax, 61 tokens"),
+                   masked=0.1, name="route softmax 61 tokens"),
         # a prompt's routing with the balance bias and the experts' loads
         route_case(8192, 512, 10, bias=True, groups=8, top_groups=4, group_top=2, scale=2.5, counts=True,
-                   name="route, 8192 tokens"),
+                   name="route 8192 tokens"),
         # one answered token with its alternatives
-        logprobs_case(1, 131072, top_k=20, name="logprobs, 1 token"),
+        logprobs_case(1, 131072, top_k=20, name="logprobs 1 token"),
         # a speculative verification batch, 32-bit logits
-        logprobs_case(64, 131072, dtype="f32", top_k=8, name="logprobs, 64 tokens"),
+        logprobs_case(64, 131072, dtype="f32", top_k=8, name="logprobs 64 tokens"),
         # choices scored under a grammar's mask, odd vocabulary
         logprobs_case(37, 50021, dtype="f16", targets=5, top_k=5, temperature=0.7, masked=0.5,
-                      name="logprobs masked, 37 tokens"),
+                      name="logprobs masked 37 tokens"),
         # a prompt scored: every position's token and five alternatives
-        logprobs_case(2048, 131072, top_k=5, name="logprobs, 2048 tokens"),
+        logprobs_case(2048, 131072, top_k=5, name="logprobs 2048 tokens"),
     ]
 
 
