@@ -32,7 +32,9 @@ from .moe import (  # noqa: F401
     library_path,
     linear_bf16,
     route_bf16,
+    route_scores,
     safetensors_tensor_info,
     swiglu_bf16,
+    token_logprobs,
     topk_bf16,
 )

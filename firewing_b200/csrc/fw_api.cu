@@ -246,6 +246,9 @@ int alloc(fw_moe* h, T** p, size_t count, std::vector<void*>& owned) {
     if (rc_ != FW_OK) return rc_; \
   } while (0)
 
+bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+bool known_dtype(int32_t dtype) { return dtype == FW_DTYPE_BF16 || dtype == FW_DTYPE_F16 || dtype == FW_DTYPE_F32; }
+size_t dtype_bytes(int32_t dtype) { return dtype == FW_DTYPE_F32 ? 4 : 2; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
@@ -1326,6 +1329,88 @@ int fw_route_bf16(const uint16_t* logits, int32_t tokens, int32_t experts, int32
     FW_CUDA(zero_fill(c->err, sizeof(int), st));
     return map_device_error(code);
   }
+  return FW_OK;
+}
+
+int fw_route_scores(const fw_route_config* c, const void* logits, int32_t tokens, const float* bias,
+                    int32_t* indices, float* weights, int32_t* counts, void* stream) {
+  if (!c || (tokens != 0 && (!logits || !indices || !weights))) return fail(FW_EINVAL, "null argument");
+  if (c->experts < 1 || c->experts > 1024 || c->top_k < 1 || c->top_k > 32 || tokens < 0)
+    return fail(FW_EINVAL, "route_scores: experts 1..1024, top_k 1..32, tokens not negative");
+  if (c->groups < 1 || c->groups > 32 || c->experts % c->groups != 0 || c->top_groups < 1 ||
+      c->top_groups > c->groups || (c->group_top != 1 && c->group_top != 2) ||
+      c->top_k > c->top_groups * (c->experts / c->groups))
+    return fail(FW_EINVAL,
+                "route_scores: groups 1..32 dividing experts, top_groups 1..groups, group_top 1 or 2, top_k within "
+                "the groups kept");
+  if (c->scoring != FW_SCORE_SOFTMAX && c->scoring != FW_SCORE_SIGMOID)
+    return fail(FW_EINVAL, "route_scores: unknown scoring");
+  if (!known_dtype(c->dtype)) return fail(FW_EINVAL, "route_scores: unknown dtype");
+  if (!std::isfinite(c->scale)) return fail(FW_EINVAL, "route_scores: scale is not finite");
+  if (c->logit_stride < c->experts) return fail(FW_EINVAL, "route_scores: logit_stride below experts");
+  if (!aligned_to(logits, dtype_bytes(c->dtype)) || !aligned_to(bias, 4) || !aligned_to(indices, 4) ||
+      !aligned_to(weights, 4) || !aligned_to(counts, 4))
+    return fail(FW_EINVAL, "route_scores: a buffer is not aligned to its type");
+  if (tokens == 0 && counts == nullptr) return FW_OK;
+  fw::RouteScoreArgs a = {};
+  a.logits = logits;
+  a.stride = c->logit_stride;
+  a.bias = bias;
+  a.indices = indices;
+  a.weights = weights;
+  a.counts = counts;
+  a.tokens = tokens;
+  a.experts = c->experts;
+  a.top_k = c->top_k;
+  a.dtype = c->dtype;
+  a.scoring = c->scoring;
+  a.groups = c->groups;
+  a.top_groups = c->top_groups;
+  a.group_top = c->group_top;
+  a.renormalize = c->renormalize != 0;
+  a.scale = c->scale;
+  const cudaError_t e = fw::launch_route_scores(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(FW_ECUDA, "route_scores", cudaGetErrorString(e));
+  return FW_OK;
+}
+
+int fw_token_logprobs(const fw_logprob_config* c, const void* logits, int32_t tokens, const int32_t* targets,
+                      float* logprobs, float* entropy, int32_t* top_idx, float* top_logprobs, void* stream) {
+  if (!c || (tokens != 0 && !logits)) return fail(FW_EINVAL, "null argument");
+  if (c->vocab < 1 || tokens < 0 || c->targets < 0 || c->targets > 65536)
+    return fail(FW_EINVAL, "token_logprobs: vocab at least 1, tokens not negative, targets 0..65536");
+  if (c->top_k < 0 || c->top_k > 32 || c->top_k > c->vocab)
+    return fail(FW_EINVAL, "token_logprobs: top_k 0..min(32, vocab)");
+  if (tokens > (1 << 28)) return fail(FW_EINVAL, "token_logprobs: too many tokens");
+  if (!known_dtype(c->dtype)) return fail(FW_EINVAL, "token_logprobs: unknown dtype");
+  if (!(c->temperature >= 1e-6f && c->temperature <= 1e6f))
+    return fail(FW_EINVAL, "token_logprobs: temperature 1e-6..1e6");
+  if (c->logit_stride < c->vocab) return fail(FW_EINVAL, "token_logprobs: logit_stride below vocab");
+  if (tokens != 0 &&
+      ((c->targets > 0 && (!targets || !logprobs)) || (c->top_k > 0 && (!top_idx || !top_logprobs))))
+    return fail(FW_EINVAL, "token_logprobs: targets or alternatives asked for without their buffers");
+  if (tokens != 0 && c->targets == 0 && c->top_k == 0 && entropy == nullptr)
+    return fail(FW_EINVAL, "token_logprobs: nothing asked for");
+  if (!aligned_to(logits, dtype_bytes(c->dtype)) || !aligned_to(targets, 4) || !aligned_to(logprobs, 4) ||
+      !aligned_to(entropy, 4) || !aligned_to(top_idx, 4) || !aligned_to(top_logprobs, 4))
+    return fail(FW_EINVAL, "token_logprobs: a buffer is not aligned to its type");
+  if (tokens == 0) return FW_OK;
+  fw::LogprobArgs a = {};
+  a.logits = logits;
+  a.stride = c->logit_stride;
+  a.targets = targets;
+  a.logprobs = logprobs;
+  a.entropy = entropy;
+  a.top_idx = top_idx;
+  a.top_logprobs = top_logprobs;
+  a.tokens = tokens;
+  a.vocab = c->vocab;
+  a.dtype = c->dtype;
+  a.targets_per_row = c->targets;
+  a.top_k = c->top_k;
+  a.inv_temperature = 1.0f / c->temperature;
+  const cudaError_t e = fw::launch_token_logprobs(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(FW_ECUDA, "token_logprobs", cudaGetErrorString(e));
   return FW_OK;
 }
 

@@ -397,6 +397,40 @@ cudaError_t launch_ep_ids(const EpPeers& p, int E, int32_t* idx_all, uint16_t* s
 cudaError_t launch_ep_scatter(const EpPeers& p, int banks, const int32_t* idx_all, const int* offset, int* fill,
                               int32_t* pair_tk, uint16_t* xg, long long xg_rows, int* err, cudaStream_t st);
 
+// ---- primitives with types, strides and epilogues of their own ----------------
+// Element types (FW_DTYPE_* of fwmoe.h).
+constexpr int kBf16 = 0, kF16 = 1, kF32 = 2;
+constexpr int kScoreSoftmax = 0, kScoreSigmoid = 1;  // FW_SCORE_*
+
+struct RouteScoreArgs {
+  const void* logits;  // [tokens] rows of `experts`, `stride` elements apart
+  long long stride;
+  const float* bias;   // [experts] or null
+  int32_t* indices;    // [tokens][top_k]
+  float* weights;      // [tokens][top_k]
+  int32_t* counts;     // [experts] or null
+  int tokens, experts, top_k, dtype, scoring;
+  int groups, top_groups, group_top, renormalize;
+  float scale;
+  int lanes, group_size, group_inv;  // set by launch_route_scores
+};
+cudaError_t launch_route_scores(RouteScoreArgs a, cudaStream_t st);
+
+struct LogprobArgs {
+  const void* logits;    // [tokens] rows of `vocab`, `stride` elements apart
+  long long stride;
+  const int32_t* targets;  // [tokens][targets_per_row]
+  float* logprobs;         // [tokens][targets_per_row]
+  float* entropy;          // [tokens] or null
+  int32_t* top_idx;        // [tokens][top_k]
+  float* top_logprobs;     // [tokens][top_k]
+  int tokens, vocab, dtype, targets_per_row, top_k;
+  float inv_temperature;
+  int splits, part_len;  // set by launch_token_logprobs, as are:
+  float scale, slack;    // log2(e) / temperature; 16 / scale
+};
+cudaError_t launch_token_logprobs(LogprobArgs a, cudaStream_t st);
+
 // Store a failure message for fw_last_error() (fixed buffer, no allocation);
 // returns `code`.
 int record_error(int code, const char* msg);

@@ -34,6 +34,11 @@ FW_ENAN = -6
 EP_TRANSPORT_P2P = 0
 EP_TRANSPORT_NCCL = 1
 
+# element types and scores of the primitives over torch tensors
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+_SCORES = {"softmax": SCORE_SOFTMAX, "sigmoid": SCORE_SIGMOID}
+
 # paths a forward takes (fw_moe_last_path)
 PATH_DECODE = 1
 PATH_PREFILL = 2
@@ -68,6 +73,17 @@ class _Weights(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p) for name in (
         "router", "gate_up", "down", "shared_gate", "shared_up", "shared_down", "shared_gate_w",
         "logit_bias")]
+
+
+class _RouteConfig(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in (
+        "experts", "top_k", "dtype", "scoring", "groups", "top_groups", "group_top", "renormalize")] + [
+        ("scale", ctypes.c_float), ("logit_stride", ctypes.c_int64)]
+
+
+class _LogprobConfig(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("vocab", "dtype", "targets", "top_k")] + [
+        ("temperature", ctypes.c_float), ("logit_stride", ctypes.c_int64)]
 
 
 _lib = None
@@ -124,6 +140,8 @@ def library() -> ctypes.CDLL:
     L.fw_swiglu_bf16.argtypes = [vp, vp, ctypes.c_int64, vp, vp]
     L.fw_add_bf16.argtypes = [vp, vp, ctypes.c_int64, vp, vp]
     L.fw_route_bf16.argtypes = [vp, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, vp, vp, vp]
+    L.fw_route_scores.argtypes = [ctypes.POINTER(_RouteConfig), vp, ctypes.c_int32, vp, vp, vp, vp, vp]
+    L.fw_token_logprobs.argtypes = [ctypes.POINTER(_LogprobConfig), vp, ctypes.c_int32, vp, vp, vp, vp, vp, vp]
     L.fw_moe_forward_noalloc.argtypes = [ctypes.POINTER(_Config), ctypes.POINTER(_Weights), vp,
                                          ctypes.c_int32, vp, vp, vp, vp]
     L.firewing_cuda_topk_bf16.restype = ctypes.c_bool
@@ -137,6 +155,7 @@ def library() -> ctypes.CDLL:
                  "fw_safetensors_tensor_info", "fw_moe_get_config", "fw_moe_last_union", "fw_moe_last_path", "fw_moe_load_expert",
                  "fw_moe_load_expert_container", "fw_codec_container_check",
                  "fw_linear_bf16", "fw_swiglu_bf16", "fw_add_bf16", "fw_route_bf16", "fw_moe_forward_noalloc",
+                 "fw_route_scores", "fw_token_logprobs",
                  "fw_moe_ep_set_transport", "fw_moe_set_wait_limit", "fw_moe_test_stall"):
         getattr(L, name).restype = ctypes.c_int
     _lib = L
@@ -427,6 +446,126 @@ def swiglu_bf16(gate, up, n: int, out, stream=None) -> None:
 def route_bf16(logits, tokens: int, experts: int, top_k: int, indices, scores, stream=None) -> None:
     _check(library().fw_route_bf16(_ptr(logits), tokens, experts, top_k, _ptr(indices),
                                    _ptr(scores), _stream(stream)))
+
+
+# ---- primitives over torch tensors: shapes, types and strides are the tensors' own ----
+
+_dtype_codes: dict = {}
+
+
+def _codes() -> dict:
+    if not _dtype_codes:
+        import torch
+
+        _dtype_codes.update({torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32,
+                             torch.int32: -1})
+    return _dtype_codes
+
+
+def _rows(t, name: str, codes: tuple, rows: Optional[int] = None, cols: Optional[int] = None,
+          device: Optional[int] = None):
+    """(pointer, dtype code, rows, cols, row stride) of a 2-D CUDA tensor with
+    unit column stride, after checking it."""
+    if not hasattr(t, "data_ptr") or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device")
+    code = _codes().get(t.dtype)
+    if code not in codes:
+        raise ValueError(f"{name}: unsupported element type {t.dtype}")
+    r, c = t.shape
+    if (rows is not None and r != rows) or (cols is not None and c != cols):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({rows}, {cols})")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name} is on another device")
+    s0, s1 = t.stride()
+    if s1 != 1 and c > 1:
+        raise ValueError(f"{name} must have consecutive columns")
+    if r <= 1:
+        s0 = c
+    elif s0 < c:
+        raise ValueError(f"{name} has overlapping rows")
+    return t.data_ptr(), code, r, c, s0
+
+
+def _dense(t, name: str, code: int, shape: tuple, device: int) -> Optional[int]:
+    """Pointer of a contiguous CUDA tensor of exactly this shape (None stays None)."""
+    if t is None:
+        return None
+    if not hasattr(t, "data_ptr") or not t.is_cuda or t.get_device() != device:
+        raise ValueError(f"{name} must be a tensor on the operator's device")
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with shape {shape}")
+    if _codes().get(t.dtype) != code:
+        raise ValueError(f"{name}: unsupported element type {t.dtype}")
+    return t.data_ptr()
+
+
+def _call(device: int, function, *args) -> None:
+    """The C entry point on `device`, which stays current only for the call."""
+    import torch
+
+    if torch.cuda.current_device() == device:
+        _check(function(*args))
+    else:
+        with torch.cuda.device(device):
+            _check(function(*args))
+
+
+def route_scores(logits, indices, weights, scoring: str = "softmax", bias=None, groups: int = 1,
+                 top_groups: int = 1, group_top: int = 1, renormalize: bool = True, scale: float = 1.0,
+                 counts=None, stream=None) -> None:
+    """Route tokens by softmax or sigmoid scores (fw_route_scores).
+
+    logits [T][E] (bf16, f16 or f32, rows may be strided) -> indices [T][K]
+    int32 and weights [T][K] f32.  Selection by score + `bias` ([E] f32)
+    among the `top_groups` of `groups` expert groups with the largest sum of
+    their `group_top` best; weights are the scores, renormalised over the
+    selection and scaled.  `counts` ([E] int32) receives how many tokens
+    selected each expert.  Experts at -inf are out; empty places are -1 with
+    weight 0."""
+    if scoring not in _SCORES:
+        raise ValueError(f"scoring must be one of {tuple(_SCORES)}")
+    p, code, T, E, stride = _rows(logits, "logits", (DTYPE_BF16, DTYPE_F16, DTYPE_F32))
+    dev = logits.get_device()
+    if not hasattr(indices, "dim") or indices.dim() != 2:
+        raise ValueError("indices must be a 2-D tensor")
+    K = indices.shape[1]
+    args = (_dense(bias, "bias", DTYPE_F32, (E,), dev), _dense(indices, "indices", -1, (T, K), dev),
+            _dense(weights, "weights", DTYPE_F32, (T, K), dev), _dense(counts, "counts", -1, (E,), dev))
+    if T == 0 and counts is None:
+        return
+    c = _RouteConfig(E, K, code, _SCORES[scoring], groups, top_groups, group_top, 1 if renormalize else 0, scale,
+                     stride)
+    _call(dev, library().fw_route_scores, ctypes.byref(c), p, T, *args, _stream(stream))
+
+
+def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_idx=None, top_logprobs=None,
+                   temperature: float = 1.0, stream=None) -> None:
+    """Log probabilities of given tokens, entropy and top alternatives
+    (fw_token_logprobs).
+
+    logits [T][V] (bf16, f16 or f32, rows may be strided), under
+    softmax(logits / temperature).  targets [T][C] int32 -> logprobs [T][C]
+    f32 (a negative target: 0); entropy [T] f32; top_idx [T][K] int32 and
+    top_logprobs [T][K] f32, K <= 32, best first.  Leave out what is not
+    wanted."""
+    p, code, T, V, stride = _rows(logits, "logits", (DTYPE_BF16, DTYPE_F16, DTYPE_F32))
+    dev = logits.get_device()
+    if (targets is None) != (logprobs is None) or (top_idx is None) != (top_logprobs is None):
+        raise ValueError("targets and logprobs, top_idx and top_logprobs go together")
+    for t, name in ((targets, "targets"), (top_idx, "top_idx")):
+        if t is not None and (not hasattr(t, "dim") or t.dim() != 2):
+            raise ValueError(f"{name} must be a 2-D tensor")
+    C = 0 if targets is None else targets.shape[1]
+    K = 0 if top_idx is None else top_idx.shape[1]
+    args = (_dense(targets, "targets", -1, (T, C), dev), _dense(logprobs, "logprobs", DTYPE_F32, (T, C), dev),
+            _dense(entropy, "entropy", DTYPE_F32, (T,), dev), _dense(top_idx, "top_idx", -1, (T, K), dev),
+            _dense(top_logprobs, "top_logprobs", DTYPE_F32, (T, K), dev))
+    if T == 0:
+        return
+    c = _LogprobConfig(V, code, C, K, temperature, stride)
+    _call(dev, library().fw_token_logprobs, ctypes.byref(c), p, T, *args, _stream(stream))
 
 
 def topk_bf16(values: np.ndarray, k: int):

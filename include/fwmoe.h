@@ -366,6 +366,87 @@ int fw_add_bf16(const uint16_t* a, const uint16_t* b, int64_t n, uint16_t* out, 
 int fw_route_bf16(const uint16_t* logits, int32_t tokens, int32_t experts, int32_t top_k,
                   int32_t* indices, uint16_t* scores, void* stream);
 
+/* Element types of the primitives below. */
+#define FW_DTYPE_BF16 0
+#define FW_DTYPE_F16 1
+#define FW_DTYPE_F32 2
+
+/* Routing from rows of logits with either kind of score, a balance bias,
+ * groups and the experts' loads, stream-ordered (the reference's route,
+ * src/decoder_layer.rs:278-307, is the case softmax, no bias, one group,
+ * renormalised; fw_route_bf16 computes that one with its bf16 roundings).
+ * For a token with logits z:
+ *   s = softmax(z) (FW_SCORE_SOFTMAX) or 1/(1+exp(-z)) (FW_SCORE_SIGMOID);
+ *   key = s + bias, or the order of z itself when bias is NULL;
+ *   the experts form `groups` equal runs of consecutive ids; a group's score
+ *   is the sum of its `group_top` (1 or 2) largest keys (scores when bias is
+ *   NULL), and the `top_groups` best groups stay;
+ *   the top_k best keys in them are selected, equal ones by lowest index;
+ *   weight = s (without the bias), divided by the selected experts' sum when
+ *   `renormalize`, times `scale`.
+ * The selection is that of exact scores: near ties are decided in 64 bits.
+ *   logits [tokens] rows of `experts`, logit_stride elements apart (>=
+ *     experts); dtype FW_DTYPE_*; bias [experts] f32 or NULL;
+ *   indices [tokens][top_k] int32, weights [tokens][top_k] f32, in order;
+ *   counts [experts] int32 or NULL: tokens that selected each expert,
+ *     overwritten.
+ * An expert whose logit (or bias) is -inf is never selected; where fewer
+ * than top_k remain, the rest of a row is index -1, weight 0, and a row of
+ * nothing but -inf selects none.  A row with a NaN in its logits (or in the
+ * bias of an expert that could be selected, or +inf under softmax) has index
+ * -1 and weight NaN throughout.
+ * 1 <= experts <= 1024; 1 <= top_k <= 32; 1 <= groups <= 32 dividing
+ * experts; 1 <= top_groups <= groups; top_k <= top_groups * experts/groups;
+ * scale finite.  Device pointers of the current device; outputs must not
+ * overlap inputs.  FW_EINVAL otherwise; tokens = 0 only clears counts. */
+#define FW_SCORE_SOFTMAX 0
+#define FW_SCORE_SIGMOID 1
+typedef struct fw_route_config {
+    int32_t experts, top_k;
+    int32_t dtype;      /* of the logits */
+    int32_t scoring;    /* FW_SCORE_* */
+    int32_t groups, top_groups, group_top;
+    int32_t renormalize;
+    float scale;
+    int64_t logit_stride;
+} fw_route_config;
+int fw_route_scores(const fw_route_config* config, const void* logits, int32_t tokens, const float* bias,
+                    int32_t* indices, float* weights, int32_t* counts, void* stream);
+
+/* Log probabilities under softmax(z / temperature) of `targets` given tokens
+ * per row, the rows' entropy and their top_k most likely tokens, from rows
+ * of logits in one pass, stream-ordered, no workspace (no reference
+ * counterpart: its endpoint ends at the logits, src/token_text_endpoint.rs;
+ * the accepted tokens of a verification step are decided from these).
+ *   logits [tokens] rows of `vocab`, logit_stride elements apart (>= vocab),
+ *     dtype FW_DTYPE_*;
+ *   targets [tokens][targets] int32 and logprobs [tokens][targets] f32, may
+ *     be NULL when targets is 0: a negative target asks for none and gets 0,
+ *     one of vocab or more gets NaN;
+ *   entropy [tokens] f32 in nats, may be NULL;
+ *   top_idx [tokens][top_k] int32, top_logprobs [tokens][top_k] f32, may be
+ *     NULL when top_k is 0: descending, equal logits by lowest index.
+ * A token whose logit is -inf has probability 0: log probability -inf,
+ * nothing to the entropy, never an alternative (the rest of a row's
+ * alternatives is -1 with -inf).  A row of nothing but -inf has -inf, entropy
+ * 0 and no alternatives; a row with a NaN or +inf has NaN throughout and
+ * alternatives -1.
+ * vocab >= 1; 0 <= targets <= 65536; 0 <= top_k <= min(32, vocab);
+ * temperature positive, at least 1e-6 and at most 1e6.  Device pointers of
+ * the current device, logits aligned to their type; outputs must not overlap
+ * inputs.  FW_EINVAL otherwise. */
+typedef struct fw_logprob_config {
+    int32_t vocab;
+    int32_t dtype;      /* of the logits */
+    int32_t targets;    /* per row */
+    int32_t top_k;
+    float temperature;
+    int64_t logit_stride;
+} fw_logprob_config;
+int fw_token_logprobs(const fw_logprob_config* config, const void* logits, int32_t tokens,
+                      const int32_t* targets, float* logprobs, float* entropy, int32_t* top_idx,
+                      float* top_logprobs, void* stream);
+
 /* Drop-in for the reference's only C ABI on the path,
  * `bool firewing_torch_topk_bf16(const uint16_t*, size_t, size_t, size_t*)`
  * (native/topk_shim.cpp:18-44, bound at src/decoder_layer.rs:19-39): HOST
