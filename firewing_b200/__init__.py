@@ -31,6 +31,8 @@ from .moe import (  # noqa: F401
     library,
     library_path,
     linear_bf16,
+    linear_epilogue,
+    primitive_status,
     route_bf16,
     route_scores,
     safetensors_tensor_info,

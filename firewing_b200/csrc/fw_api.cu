@@ -1332,6 +1332,59 @@ int fw_route_bf16(const uint16_t* logits, int32_t tokens, int32_t experts, int32
   return FW_OK;
 }
 
+int fw_linear_epilogue(const fw_linear_config* c, const void* w, const void* x, int32_t tokens, const void* bias,
+                       const void* residual, void* y, void* stream) {
+  if (!c || !w || (tokens != 0 && (!x || !y))) return fail(FW_EINVAL, "null argument");
+  constexpr int32_t kMost = 1 << 24;
+  if (c->rows < 1 || c->rows > kMost || c->cols < 1 || c->cols > kMost || tokens < 0 || tokens > kMost ||
+      static_cast<int64_t>(c->rows) * tokens > (1ll << 38))
+    return fail(FW_EINVAL, "linear_epilogue: rows and cols 1..2^24, tokens 0..2^24, rows * tokens at most 2^38");
+  if ((c->dtype != FW_DTYPE_BF16 && c->dtype != FW_DTYPE_F16) ||
+      (c->out_dtype != c->dtype && c->out_dtype != FW_DTYPE_F32) || (bias && !known_dtype(c->bias_dtype)) ||
+      (residual && !known_dtype(c->residual_dtype)))
+    return fail(FW_EINVAL, "linear_epilogue: x and w bf16 or f16, y of their type or f32");
+  if (c->activation < FW_ACT_NONE || c->activation > FW_ACT_SIGMOID)
+    return fail(FW_EINVAL, "linear_epilogue: unknown activation");
+  constexpr int64_t kFar = 1ll << 37;
+  if (c->w_stride < c->cols || c->x_stride < c->cols || c->y_stride < c->rows ||
+      (residual && c->residual_stride < c->rows) || c->w_stride > kFar || c->x_stride > kFar || c->y_stride > kFar ||
+      (residual && c->residual_stride > kFar))
+    return fail(FW_EINVAL, "linear_epilogue: a stride is below its row's length or above 2^37");
+  if (!aligned_to(w, 2) || !aligned_to(x, 2) || !aligned_to(y, dtype_bytes(c->out_dtype)) ||
+      (bias && !aligned_to(bias, dtype_bytes(c->bias_dtype))) ||
+      (residual && !aligned_to(residual, dtype_bytes(c->residual_dtype))))
+    return fail(FW_EINVAL, "linear_epilogue: a buffer is not aligned to its type");
+  if (residual == y && residual && (c->residual_dtype != c->out_dtype || c->residual_stride != c->y_stride))
+    return fail(FW_EINVAL, "linear_epilogue: residual and y share memory with another type or stride");
+  if (tokens == 0) return FW_OK;
+  fw::LinearArgs a = {};
+  a.bias = bias;
+  a.residual = residual;
+  a.y = y;
+  a.res_stride = c->residual_stride;
+  a.y_stride = c->y_stride;
+  a.tokens = tokens;
+  a.rows = c->rows;
+  a.cols = c->cols;
+  a.dtype = c->dtype;
+  a.out_dtype = c->out_dtype;
+  a.bias_dtype = c->bias_dtype;
+  a.res_dtype = c->residual_dtype;
+  a.act = c->activation;
+  const cudaError_t e =
+      fw::launch_linear_epilogue(a, static_cast<const uint16_t*>(w), c->w_stride, static_cast<const uint16_t*>(x),
+                                 c->x_stride, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(FW_ECUDA, "linear_epilogue", cudaGetErrorString(e));
+  return FW_OK;
+}
+
+int fw_primitive_status(void* stream) {
+  int code = 0;
+  const cudaError_t e = fw::take_linear_status(&code, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(FW_ECUDA, "primitive_status", cudaGetErrorString(e));
+  return map_device_error(code);
+}
+
 int fw_route_scores(const fw_route_config* c, const void* logits, int32_t tokens, const float* bias,
                     int32_t* indices, float* weights, int32_t* counts, void* stream) {
   if (!c || (tokens != 0 && (!logits || !indices || !weights))) return fail(FW_EINVAL, "null argument");

@@ -416,6 +416,29 @@ struct RouteScoreArgs {
 };
 cudaError_t launch_route_scores(RouteScoreArgs a, cudaStream_t st);
 
+constexpr int kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4, kActSigmoid = 5;  // FW_ACT_*
+
+struct LinearArgs {
+  const void* bias;      // [rows] or null
+  const void* residual;  // [tokens] rows, res_stride apart, or null
+  void* y;               // [tokens] rows, y_stride apart
+  long long res_stride, y_stride;
+  int tokens, rows, cols, dtype, out_dtype, bias_dtype, res_dtype, act;
+  // set by launch_linear_epilogue
+  const uint16_t *p, *q;         // M-side and N-side operand
+  long long p_stride, q_stride;
+  int p_rows, q_rows;
+  int swap;                      // the M side is w
+  int vec;                       // bias, residual and y can be read and written 16 bytes at a time
+  int bn, tiles_p, tiles_q, kblocks, stages, ring_bytes, tmem_cols;
+  int chunk;                     // stages per accumulation (f32 outputs)
+  int splits;                    // CTAs of a cluster that share a tile's columns; warps per row
+};
+cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_stride, const uint16_t* x,
+                                   long long x_stride, cudaStream_t st);
+// Device status of the linear kernels (a DeviceError), cleared; waits for st.
+cudaError_t take_linear_status(int* code, cudaStream_t st);
+
 struct LogprobArgs {
   const void* logits;    // [tokens] rows of `vocab`, `stride` elements apart
   long long stride;

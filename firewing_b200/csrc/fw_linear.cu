@@ -1,0 +1,911 @@
+// fw_linear.cu -- y = act(x w^T + bias) + residual (fw_linear_epilogue).
+//
+// x [T][K], w [N][K], bf16 or f16; sums in f32; bias, activation and residual
+// in f32 on the accumulator; one rounding to y's type.
+//
+// k_linear_mma: the product on the tensor cores.  One operand is the M side
+//   (P, 128 rows per tile), the other the N side (Q, bn rows per tile, a
+//   multiple of 16 up to 256); both are K-major, staged 64 columns at a time
+//   in the 128-byte swizzled layout.
+//     warp 0      producer: TMA loads of both tiles into a ring
+//     warp 1      tcgen05.mma kind::f16 into one of two TMEM accumulators
+//     warps 2-9   epilogue, two sets of four (set s takes the 32-column
+//                 groups s, s + 2, ...)
+//     warps 10-17 only where TMA cannot read an operand (a row stride or base
+//                 that is no multiple of 16 bytes): loaders that realign
+//                 16-byte chunks in registers and write the same layout
+//   Few tokens: w is the M side and the K range is split over the CTAs of a
+//   cluster, which exchange their partial tiles through distributed shared
+//   memory and add them in rank order (no workspace, repeatable sums).
+// k_linear_rows: one to a few tokens on the CUDA cores, a warp (or several)
+//   per weight row: the weights' bytes are the work, and there is no
+//   pipeline to fill.
+//
+// Every wait is bounded (2 s of globaltimer); on expiry the CTA records a
+// time-out, lets its copies and MMAs drain (bounded), frees its TMEM and
+// exits; fw_primitive_status reports it.
+#include <algorithm>
+#include <cstdint>
+#include <mutex>
+
+#include <cudaTypedefs.h>
+#include <cuda_fp16.h>
+
+#include "fw_common.cuh"
+#include "fw_kernels.h"
+
+namespace fw {
+namespace {
+
+constexpr int kBM = 128;                  // M-side rows per tile
+constexpr int kBK = 64;                   // columns per stage (one 128-byte swizzle atom)
+constexpr int kABytes = kBM * kBK * 2;    // 16 KB
+constexpr int kMaxStages = 8;
+constexpr int kEpiWarps = 8;
+constexpr int kLoadWarps = 8;
+constexpr int kMmaThreads = 32 * (2 + kEpiWarps);
+constexpr int kLoaderThreads = kMmaThreads + 32 * kLoadWarps;
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr unsigned kAll = 0xffffffffu;
+
+__device__ int g_status;  // first time-out of this library's linear kernels on the device
+
+// ---- tcgen05 / TMA ----------------------------------------------------------------
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// K-major operand, 128-byte swizzle, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3fffu) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// kind::f16, both operands bf16 or both f16, K-major, f32 accumulator, M x N.
+__device__ __forceinline__ uint32_t idesc_f16(int m, int n, bool bf16) {
+  const uint32_t type = bf16 ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// 32 consecutive f32 columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t saddr, uint32_t rank) {
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(remote)
+               : "memory");
+  return v;
+}
+
+// ---- epilogue arithmetic -------------------------------------------------------------
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The activations in f32.  Those built on exp use x * sigmoid forms, which
+// have no cancellation: their relative error stays near 2^-21 everywhere,
+// far under the rounding of y.  __fdividef(x, y) is 0 for y > 2^126, where
+// the true value is below 2^-118 * |x|.
+template <int ACT>
+__device__ __forceinline__ float activate(float x) {
+  if (ACT == kActRelu) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+    return r;
+  }
+  if (ACT == kActGelu) return __fmul_rn(__fmul_rn(0.5f, x), erfcf(__fmul_rn(x, -0.70710678118654752f)));
+  if (ACT == kActGeluTanh) {
+    // 0.5 x (1 + tanh u) = x / (1 + exp(-2u)), u = sqrt(2/pi) (x + 0.044715 x^3)
+    const float u2 = __fmul_rn(__fmul_rn(x, 1.5957691216057308f), __fmaf_rn(__fmul_rn(x, x), 0.044715f, 1.0f));
+    return __fdividef(x, __fadd_rn(1.0f, ex2(__fmul_rn(u2, -kLog2e))));
+  }
+  if (ACT == kActSilu) return __fdividef(x, __fadd_rn(1.0f, ex2(__fmul_rn(x, -kLog2e))));
+  if (ACT == kActSigmoid) return __fdividef(1.0f, __fadd_rn(1.0f, ex2(__fmul_rn(x, -kLog2e))));
+  return x;
+}
+template <int N>
+__device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
+  switch (act) {
+    case kActRelu:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = activate<kActRelu>(v[j]);
+      break;
+    case kActGelu:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = activate<kActGelu>(v[j]);
+      break;
+    case kActGeluTanh:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = activate<kActGeluTanh>(v[j]);
+      break;
+    case kActSilu:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = activate<kActSilu>(v[j]);
+      break;
+    case kActSigmoid:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = activate<kActSigmoid>(v[j]);
+      break;
+    default: break;
+  }
+}
+
+__device__ __forceinline__ float load_f32(const void* p, long long i, int dtype) {
+  if (dtype == kF32) return static_cast<const float*>(p)[i];
+  const uint16_t v = static_cast<const uint16_t*>(p)[i];
+  return dtype == kBf16 ? bf16_to_f32(v) : __half2float(__ushort_as_half(v));
+}
+__device__ __forceinline__ void store_f32(void* p, long long i, int dtype, float v) {
+  if (dtype == kF32) static_cast<float*>(p)[i] = v;
+  else if (dtype == kBf16) static_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
+  else static_cast<uint16_t*>(p)[i] = __half_as_ushort(__float2half_rn(v));
+}
+// Two values rounded to a 16-bit type, the first in the low half.
+__device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi) {
+  uint32_t r;
+  if (dtype == kBf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void unpack2(int dtype, uint32_t w, float* lo, float* hi) {
+  if (dtype == kBf16) {
+    *lo = lo_bf16(w);
+    *hi = hi_bf16(w);
+  } else {
+    *lo = __half2float(__ushort_as_half(static_cast<uint16_t>(w)));
+    *hi = __half2float(__ushort_as_half(static_cast<uint16_t>(w >> 16)));
+  }
+}
+// N (4 or a multiple of 8) consecutive values as f32, 8 or 16 bytes at a
+// time: p + i aligned to that.
+template <int N>
+__device__ __forceinline__ void load_vec(const void* p, long long i, int dtype, float (&v)[N]) {
+  if (dtype == kF32) {
+    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+      const float4 f = s[j];
+      v[4 * j] = f.x, v[4 * j + 1] = f.y, v[4 * j + 2] = f.z, v[4 * j + 3] = f.w;
+    }
+  } else if (N == 4) {
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    unpack2(dtype, u.x, &v[0], &v[1]);
+    unpack2(dtype, u.y, &v[2], &v[3]);
+  } else {
+    const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < N / 8; ++j) {
+      const uint4 u = s[j];
+      unpack2(dtype, u.x, &v[8 * j], &v[8 * j + 1]);
+      unpack2(dtype, u.y, &v[8 * j + 2], &v[8 * j + 3]);
+      unpack2(dtype, u.z, &v[8 * j + 4], &v[8 * j + 5]);
+      unpack2(dtype, u.w, &v[8 * j + 6], &v[8 * j + 7]);
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_vec(void* p, long long i, int dtype, const float (&v)[N]) {
+  if (dtype == kF32) {
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) d[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  } else if (N == 4) {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) =
+        make_uint2(pack2(dtype, v[0], v[1]), pack2(dtype, v[2], v[3]));
+  } else {
+    uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < N / 8; ++j)
+      d[j] = make_uint4(pack2(dtype, v[8 * j], v[8 * j + 1]), pack2(dtype, v[8 * j + 2], v[8 * j + 3]),
+                        pack2(dtype, v[8 * j + 4], v[8 * j + 5]), pack2(dtype, v[8 * j + 6], v[8 * j + 7]));
+  }
+}
+
+// N consecutive outputs of token t from row r on (bias, activation,
+// residual, rounding).
+template <int N>
+__device__ __forceinline__ void finish_run(const LinearArgs& a, int t, int r, float (&v)[N]) {
+  if (a.vec && r + N <= a.rows) {
+    float b[N];
+    if (a.bias != nullptr) {
+      load_vec<N>(a.bias, r, a.bias_dtype, b);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], b[j]);
+    }
+    activate_all(a.act, v);
+    if (a.residual != nullptr) {
+      load_vec<N>(a.residual, static_cast<long long>(t) * a.res_stride + r, a.res_dtype, b);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], b[j]);
+    }
+    store_vec<N>(a.y, static_cast<long long>(t) * a.y_stride + r, a.out_dtype, v);
+    return;
+  }
+  const int n = min(N, a.rows - r);
+  if (a.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) v[j] = __fadd_rn(v[j], load_f32(a.bias, r + j, a.bias_dtype));
+  }
+  activate_all(a.act, v);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (j >= n) break;
+    if (a.residual != nullptr)
+      v[j] = __fadd_rn(v[j], load_f32(a.residual, static_cast<long long>(t) * a.res_stride + r + j, a.res_dtype));
+    store_f32(a.y, static_cast<long long>(t) * a.y_stride + r + j, a.out_dtype, v[j]);
+  }
+}
+// 32 tokens from t on of row r (lanes of a warp hold consecutive rows).
+__device__ __forceinline__ void finish_column(const LinearArgs& a, int t, int n, int r, float (&v)[32]) {
+  const float b = a.bias != nullptr ? load_f32(a.bias, r, a.bias_dtype) : 0.0f;
+  if (a.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], b);
+  }
+  activate_all(a.act, v);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    if (j >= n) break;
+    if (a.residual != nullptr)
+      v[j] = __fadd_rn(v[j], load_f32(a.residual, static_cast<long long>(t + j) * a.res_stride + r, a.res_dtype));
+    store_f32(a.y, static_cast<long long>(t + j) * a.y_stride + r, a.out_dtype, v[j]);
+  }
+}
+
+// ---- operands that TMA cannot read ----------------------------------------------------
+
+// The n (0..8) 16-bit elements at p, the others 0, from the one or two
+// aligned 16-byte words that hold them (no other word is read).
+__device__ __forceinline__ uint4 load_chunk(const uint16_t* p, int n) {
+  if (n <= 0) return make_uint4(0, 0, 0, 0);
+  const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+  const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) - off);
+  const uint4 a = __ldg(s);
+  uint4 b = make_uint4(0, 0, 0, 0);
+  if (off + 2 * n > 16) b = __ldg(s + 1);
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (off & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (off & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  const uint32_t sh = (off & 2) * 8;
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[i] = __funnelshift_r(w[i], w[i + 1], sh);
+    const int left = n - 2 * i;  // elements of this word that exist
+    if (left <= 0) o[i] = 0u;
+    else if (left == 1) o[i] &= 0xffffu;
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// ---- the tensor-core kernel -------------------------------------------------------------
+
+struct __align__(16) LinearTail {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint64_t drained;
+  uint32_t tmem_base;
+  int abort;
+};
+
+__device__ __forceinline__ void give_up(LinearTail* t) {
+  atomicCAS(&g_status, 0, kErrTimeout);
+  *reinterpret_cast<volatile int*>(&t->abort) = 1;
+}
+__device__ __forceinline__ bool gave_up(LinearTail* t) { return *reinterpret_cast<volatile int*>(&t->abort) != 0; }
+
+struct Tile {
+  int p0, q0;
+};
+// Tiles in groups of kGroup along P, so that those running together share
+// rows of both operands in L2.
+__device__ __forceinline__ Tile tile_of(const LinearArgs& a, int u) {
+  constexpr int kGroup = 16;
+  const int per = kGroup * a.tiles_q;
+  const int g = u / per, rest = u - g * per;
+  const int size = min(kGroup, a.tiles_p - g * kGroup);
+  Tile t;
+  t.q0 = rest / size * a.bn;
+  t.p0 = (g * kGroup + rest % size) * kBM;
+  return t;
+}
+
+// CHUNKED: the accumulation is cut every `chunk` stages and carried on in
+// registers (bn <= 128), for f32 outputs.
+template <bool LOADERS, bool CHUNKED>
+__global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
+    k_linear_mma(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                 const __grid_constant__ LinearArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  unsigned char* ring = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  const int slot = kABytes + a.bn * kBK * 2;
+  LinearTail* tail = reinterpret_cast<LinearTail*>(ring + a.ring_bytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stages = a.stages;
+  const int acc_cols = (a.bn + 31) & ~31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&tail->full[i], LOADERS ? 32 * kLoadWarps : 1);
+      mbar_init(&tail->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tail->acc_full[i], 1);
+      mbar_init(&tail->acc_empty[i], kEpiWarps);
+    }
+    mbar_init(&tail->drained, 1);
+    tail->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tail->tmem_base)),
+                 "r"(a.tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tail->tmem_base;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // This CTA's share of the columns, and its tiles.
+  const int rank = a.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int kb0 = static_cast<int>(static_cast<long long>(a.kblocks) * rank / a.splits);
+  const int kb1 = static_cast<int>(static_cast<long long>(a.kblocks) * (rank + 1) / a.splits);
+  const int total = a.tiles_p * a.tiles_q;
+  const int u0 = static_cast<int>(blockIdx.x) / a.splits;
+  const int step = static_cast<int>(gridDim.x) / a.splits;
+  const int chunk = CHUNKED ? a.chunk : kb1 - kb0;
+
+  if (warp == 0) {
+    if (!LOADERS && lane == 0) {
+      // ---------------- producer ----------------
+      int it = 0;
+      bool ok = true;
+      for (int u = u0; ok && u < total; u += step) {
+        const Tile w = tile_of(a, u);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % stages;
+          if (!mbar_wait_bounded(&tail->empty[st], ((it / stages) & 1) ^ 1u, kWaitNs)) {
+            give_up(tail);
+            ok = false;
+            break;
+          }
+          if (gave_up(tail)) {
+            ok = false;
+            break;
+          }
+          unsigned char* s = ring + static_cast<size_t>(st) * slot;
+          mbar_arrive_expect_tx(&tail->full[st], static_cast<uint32_t>(slot));
+          tma_load_2d(s, &map_p, kb * kBK, w.p0, &tail->full[st]);
+          tma_load_2d(s + kABytes, &map_q, kb * kBK, w.q0, &tail->full[st]);
+        }
+      }
+      // Copies already issued land before the CTA can exit.
+      for (int j = it > stages ? it - stages : 0; j < it; ++j)
+        if (!mbar_wait_bounded(&tail->full[j % stages], (j / stages) & 1, kWaitNs)) give_up(tail);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA ----------------
+    if (lane == 0) {
+      int it = 0, ai = 0;
+      bool ok = true;
+      const uint32_t idesc = idesc_f16(kBM, a.bn, a.dtype == kBf16);
+      for (int u = u0; ok && u < total; u += step) {
+        for (int k = kb0; ok && k < kb1; k += chunk, ++ai) {
+          const int buf = ai & 1;
+          if (gave_up(tail) || !mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u, kWaitNs)) {
+            give_up(tail);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d = tmem + buf * acc_cols;
+          const int end = min(kb1, k + chunk);
+          for (int kb = k; kb < end; ++kb, ++it) {
+            const int st = it % stages;
+            if (!mbar_wait_bounded(&tail->full[st], (it / stages) & 1, kWaitNs)) {
+              give_up(tail);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(ring + static_cast<size_t>(st) * slot), sb = sa + kABytes;
+#pragma unroll
+            for (int i = 0; i < kBK / 16; ++i)
+              umma_f16(d, sw128_desc(sa + i * 32), sw128_desc(sb + i * 32), idesc, (kb > k || i > 0) ? 1u : 0u);
+            umma_commit(&tail->empty[st]);
+          }
+          if (ok) umma_commit(&tail->acc_full[buf]);
+        }
+      }
+      // Every MMA issued has completed once `drained` flips.
+      umma_commit(&tail->drained);
+      if (!mbar_wait_bounded(&tail->drained, 0, kWaitNs)) give_up(tail);
+    }
+  } else if (warp < 2 + kEpiWarps) {
+    // ---------------- epilogue ----------------
+    const int set = (warp - 2) >> 2;
+    const int q = warp & 3;  // TMEM lane quarter this warp may read
+    const int row = q * 32 + lane;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    float* parts = reinterpret_cast<float*>(ring);  // [bn][128] of a split tile
+    int ai = 0;
+    for (int u = u0; u < total; u += step) {
+      const Tile w = tile_of(a, u);
+      const int valid = min(a.bn, a.q_rows - w.q0);
+      auto finish = [&](int c0, float(&v)[32]) {
+        if (a.splits > 1) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j < valid) parts[(c0 + j) * kBM + row] = v[j];
+        } else if (w.p0 + row < a.p_rows && c0 < valid) {
+          if (a.swap) finish_column(a, w.q0 + c0, min(32, valid - c0), w.p0 + row, v);
+          else if (a.bn - c0 >= 32) finish_run<32>(a, w.p0 + row, w.q0 + c0, v);
+          else {  // the last 16 columns of a tile that is no multiple of 32
+            float h[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) h[j] = v[j];
+            finish_run<16>(a, w.p0 + row, w.q0 + c0, h);
+          }
+        }
+      };
+      if (!CHUNKED) {
+        const int buf = ai & 1;
+        const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, kWaitNs);
+        if (!__all_sync(kAll, got)) {
+          if (lane == 0) give_up(tail);
+          break;
+        }
+        tc_fence_after();
+        for (int c0 = 32 * set; c0 < a.bn; c0 += 64) {
+          float v[32];
+          tmem_ld32(lane_base + buf * acc_cols + c0, v);
+          finish(c0, v);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tail->acc_empty[buf]);
+        ++ai;
+      } else {
+        float acc[2][32];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[g][j] = 0.0f;
+        bool ok = true;
+        for (int k = kb0; k < kb1; k += chunk, ++ai) {
+          const int buf = ai & 1;
+          const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, kWaitNs);
+          if (!__all_sync(kAll, got)) {
+            if (lane == 0) give_up(tail);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int c0 = 32 * set + 64 * g;
+            if (c0 < a.bn) {
+              float v[32];
+              tmem_ld32(lane_base + buf * acc_cols + c0, v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) acc[g][j] = __fadd_rn(acc[g][j], v[j]);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tail->acc_empty[buf]);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int c0 = 32 * set + 64 * g;
+          if (c0 < a.bn) finish(c0, acc[g]);
+        }
+      }
+    }
+  } else if (LOADERS) {
+    // ---------------- loaders ----------------
+    const int ltid = threadIdx.x - kMmaThreads;
+    const int chunks = (kBM + a.bn) * 8;  // 16-byte chunks of a stage
+    int it = 0;
+    bool ok = true;
+    for (int u = u0; ok && u < total; u += step) {
+      const Tile w = tile_of(a, u);
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int st = it % stages;
+        const bool got = mbar_wait_bounded(&tail->empty[st], ((it / stages) & 1) ^ 1u, kWaitNs) && !gave_up(tail);
+        if (!__all_sync(kAll, got)) {
+          if (lane == 0) give_up(tail);
+          ok = false;
+          break;
+        }
+        unsigned char* s = ring + static_cast<size_t>(st) * slot;
+        for (int base = ltid; base < chunks; base += 4 * 32 * kLoadWarps) {
+          uint4 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int id = base + i * 32 * kLoadWarps;
+            const int r = id >> 3, k = kb * kBK + (id & 7) * 8;
+            const bool side_p = r < kBM;
+            const int grow = side_p ? w.p0 + r : w.q0 + r - kBM;
+            const bool there = id < chunks && grow < (side_p ? a.p_rows : a.q_rows);
+            const uint16_t* src = side_p ? a.p : a.q;
+            const long long stride = side_p ? a.p_stride : a.q_stride;
+            v[i] = load_chunk(src + (there ? grow * stride + k : 0), there ? min(8, a.cols - k) : 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int id = base + i * 32 * kLoadWarps;
+            const int r = id >> 3, c = id & 7;
+            // row r of P at slot, row r - 128 of Q at slot + 16 KB: r * 128 either way
+            if (id < chunks) *reinterpret_cast<uint4*>(s + r * 128 + ((c ^ (r & 7)) << 4)) = v[i];
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&tail->full[st]);
+      }
+    }
+  }
+
+  if (a.splits > 1) {
+    // Partial tiles lie in the CTAs' rings; CTA r adds up columns r,
+    // r + splits, ... in rank order.  (Every thread comes here, whatever
+    // happened before.)
+    __syncwarp();
+    cluster_sync_all();
+    if (warp >= 2 && warp < 2 + kEpiWarps && !gave_up(tail)) {
+      const Tile w = tile_of(a, u0);
+      const int valid = min(a.bn, a.q_rows - w.q0);
+      const uint32_t parts = smem_u32(ring);
+      for (int c = rank + (warp - 2) * a.splits; c < valid; c += kEpiWarps * a.splits) {
+        const uint32_t at = parts + (c * kBM + 4 * lane) * 4;
+        float4 sum = ld_cluster_f4(at, 0);
+        for (int r = 1; r < a.splits; ++r) {
+          const float4 o = ld_cluster_f4(at, r);
+          sum.x = __fadd_rn(sum.x, o.x);
+          sum.y = __fadd_rn(sum.y, o.y);
+          sum.z = __fadd_rn(sum.z, o.z);
+          sum.w = __fadd_rn(sum.w, o.w);
+        }
+        float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (w.p0 + 4 * lane < a.p_rows) finish_run<4>(a, w.q0 + c, w.p0 + 4 * lane, v);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // the partial tiles stay until they have been read
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+}
+
+// ---- one to four tokens -------------------------------------------------------------------
+
+constexpr int kRowWarps = 8;
+constexpr int kRowTokens = 4;
+
+// acc[t] += sum of 8 products of a weight chunk with each token's chunk.
+template <bool BF16, int NT>
+__device__ __forceinline__ void dot8(const uint4 w, const uint4 (&x)[NT], float (&acc)[NT]) {
+  const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float w0, w1;
+    unpack2(BF16 ? kBf16 : kF16, ww[i], &w0, &w1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint32_t xx = i == 0 ? x[t].x : i == 1 ? x[t].y : i == 2 ? x[t].z : x[t].w;
+      float x0, x1;
+      unpack2(BF16 ? kBf16 : kF16, xx, &x0, &x1);
+      acc[t] = __fmaf_rn(w0, x0, acc[t]);
+      acc[t] = __fmaf_rn(w1, x1, acc[t]);
+    }
+  }
+}
+
+// One weight row per group of `per_row` warps (1, 2, 4 or 8 of the CTA's 8);
+// a lane takes the 8-column chunks lane, lane + 32 * per_row, ..., four in
+// flight.  ALIGNED: every row of both operands starts on 16 bytes.
+template <bool BF16, int NT, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kRowWarps) k_linear_rows(const __grid_constant__ LinearArgs a) {
+  __shared__ float part[kRowWarps][NT];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_row = a.splits;
+  const int r = (blockIdx.x * kRowWarps + warp) / per_row;
+  const int sub = warp % per_row;
+  pdl_wait();
+  pdl_launch_dependents();
+  float acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t] = 0.0f;
+  if (r < a.rows) {
+    const uint16_t* w = a.p + r * a.p_stride;
+    const int chunks = (a.cols + 7) / 8, step = 32 * per_row;
+    for (int c0 = sub * 32 + lane; c0 < chunks; c0 += 4 * step) {
+      uint4 wv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + i * step, n = min(8, a.cols - 8 * c);
+        if (ALIGNED && n == 8) wv[i] = ldg_stream(w + 8 * c);
+        else wv[i] = load_chunk(w + (n > 0 ? 8 * c : 0), n);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + i * step, n = min(8, a.cols - 8 * c);
+        uint4 xv[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const uint16_t* x = a.q + t * a.q_stride;
+          if (ALIGNED && n == 8) xv[t] = *reinterpret_cast<const uint4*>(x + 8 * c);
+          else xv[t] = load_chunk(x + (n > 0 ? 8 * c : 0), n);
+        }
+        dot8<BF16, NT>(wv[i], xv, acc);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) acc[t] = __fadd_rn(acc[t], __shfl_xor_sync(kAll, acc[t], o));
+  }
+  if (per_row > 1) {
+    if (lane == 0) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) part[warp][t] = acc[t];
+    }
+    __syncthreads();
+    if (sub != 0) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      for (int s = 1; s < per_row; ++s) acc[t] = __fadd_rn(acc[t], part[warp + s][t]);
+  }
+  if (r >= a.rows) return;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    if (lane == t) {
+      float v[1] = {acc[t]};
+      if (a.bias != nullptr) v[0] = __fadd_rn(v[0], load_f32(a.bias, r, a.bias_dtype));
+      activate_all(a.act, v);
+      if (a.residual != nullptr)
+        v[0] = __fadd_rn(v[0], load_f32(a.residual, static_cast<long long>(t) * a.res_stride + r, a.res_dtype));
+      store_f32(a.y, static_cast<long long>(t) * a.y_stride + r, a.out_dtype, v[0]);
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static std::once_flag once;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// [rows] rows of `cols` 16-bit elements, `stride` apart: boxes of 64 columns
+// x box_rows rows, 128-byte swizzle, zeros outside.
+bool operand_map(CUtensorMap* m, const void* base, int cols, int rows, long long stride, int box_rows, int dtype) {
+  const auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+  const cuuint32_t box[2] = {kBK, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t es[2] = {1, 1};
+  return fn(m, dtype == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+            const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool tma_can_read(const void* base, int rows, long long stride) {
+  return reinterpret_cast<uintptr_t>(base) % 16 == 0 && (rows == 1 || stride % 8 == 0) && stride < (1ll << 38);
+}
+
+template <typename Kern, typename... Args>
+cudaError_t launch(Kern kern, int grid, int threads, size_t smem, int cluster, cudaStream_t st,
+                   const Args&... args) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+template <bool BF16, int NT>
+cudaError_t launch_rows(const LinearArgs& a, bool aligned, cudaStream_t st) {
+  const int grid = static_cast<int>((static_cast<long long>(a.rows) * a.splits + kRowWarps - 1) / kRowWarps);
+  return aligned ? launch(k_linear_rows<BF16, NT, true>, grid, 32 * kRowWarps, 0, 1, st, a)
+                 : launch(k_linear_rows<BF16, NT, false>, grid, 32 * kRowWarps, 0, 1, st, a);
+}
+template <bool BF16>
+cudaError_t launch_rows(const LinearArgs& a, bool aligned, cudaStream_t st) {
+  switch (a.tokens) {
+    case 1: return launch_rows<BF16, 1>(a, aligned, st);
+    case 2: return launch_rows<BF16, 2>(a, aligned, st);
+    case 3: return launch_rows<BF16, 3>(a, aligned, st);
+    default: return launch_rows<BF16, 4>(a, aligned, st);
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_stride, const uint16_t* x,
+                                   long long x_stride, cudaStream_t st) {
+  DeviceAttrs dev;
+  cudaError_t e = current_device_attrs(&dev);
+  if (e != cudaSuccess) return e;
+  const auto aligned = [](const void* p, long long stride, int dtype) {
+    const long long size = dtype == kF32 ? 4 : 2;
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0);
+  };
+  a.vec = aligned(a.y, a.y_stride, a.out_dtype) && aligned(a.bias, 0, a.bias_dtype) &&
+          aligned(a.residual, a.res_stride, a.res_dtype);
+
+  if (a.tokens <= kRowTokens) {
+    a.p = w;
+    a.p_stride = w_stride;
+    a.q = x;
+    a.q_stride = x_stride;
+    // Warps per row: up to 8, while the GPU has fewer than 16 warps per SM
+    // and a warp keeps a chunk per lane.
+    int per = 1;
+    while (per < kRowWarps && static_cast<long long>(a.rows) * per < 16ll * dev.sms && a.cols >= 512 * per) per *= 2;
+    a.splits = per;
+    const bool al = aligned(w, a.rows == 1 ? 0 : w_stride, kBf16) && aligned(x, a.tokens == 1 ? 0 : x_stride, kBf16);
+    return a.dtype == kBf16 ? launch_rows<true>(a, al, st) : launch_rows<false>(a, al, st);
+  }
+
+  // Few tokens: w on the M side, all tokens in one N tile, K split over a
+  // cluster until the GPU is full.  Otherwise tokens on the M side.
+  a.swap = a.tokens <= 128;
+  const uint16_t* p = a.swap ? w : x;
+  const uint16_t* q = a.swap ? x : w;
+  a.p = p;
+  a.q = q;
+  a.p_rows = a.swap ? a.rows : a.tokens;
+  a.q_rows = a.swap ? a.tokens : a.rows;
+  a.p_stride = a.swap ? w_stride : x_stride;
+  a.q_stride = a.swap ? x_stride : w_stride;
+  const bool chunked = a.out_dtype == kF32;
+  a.bn = std::min(chunked ? 128 : 256, (a.q_rows + 15) & ~15);
+  a.tiles_p = (a.p_rows + kBM - 1) / kBM;
+  if (!a.swap) {
+    // A tile width that leaves the fewest waves' worth of columns idle
+    long long best = -1;
+    for (int bn : {256, 128, 64}) {
+      if (bn > a.bn && bn != 64) continue;
+      const long long tiles = static_cast<long long>(a.tiles_p) * ((a.q_rows + bn - 1) / bn);
+      const long long cost = (tiles + dev.sms - 1) / dev.sms * (bn + 32);  // 32: what a tile costs beside its columns
+      if (best < 0 || cost < best) {
+        best = cost;
+        a.bn = std::min(bn, (a.q_rows + 15) & ~15);
+      }
+    }
+  }
+  a.tiles_q = (a.q_rows + a.bn - 1) / a.bn;
+  a.kblocks = (a.cols + kBK - 1) / kBK;
+  a.chunk = 4;
+  const long long tiles = static_cast<long long>(a.tiles_p) * a.tiles_q;
+  a.splits = 1;
+  if (a.swap)
+    while (a.splits < 8 && tiles * a.splits * 2 <= dev.sms && a.kblocks >= 4 * a.splits) a.splits *= 2;
+  const int slot = kABytes + a.bn * kBK * 2;
+  a.stages = std::min(kMaxStages, (200 * 1024) / slot);
+  a.ring_bytes = std::max(a.stages * slot, a.splits > 1 ? a.bn * kBM * 4 : 0);
+  int cols = 32;
+  while (cols < 2 * ((a.bn + 31) & ~31)) cols *= 2;
+  a.tmem_cols = cols;
+  const size_t smem = 1024 + a.ring_bytes + sizeof(LinearTail);
+  const int grid = a.splits > 1 ? static_cast<int>(tiles) * a.splits
+                                : static_cast<int>(std::min<long long>(tiles, dev.sms));
+
+  CUtensorMap mp = {}, mq = {};
+  const long long ps = a.p_rows == 1 ? (a.cols + 7) / 8 * 8 : a.p_stride;
+  const long long qs = a.q_rows == 1 ? (a.cols + 7) / 8 * 8 : a.q_stride;
+  if (tma_can_read(p, a.p_rows, a.p_stride) && tma_can_read(q, a.q_rows, a.q_stride)) {
+    if (!operand_map(&mp, p, a.cols, a.p_rows, ps, kBM, a.dtype) ||
+        !operand_map(&mq, q, a.cols, a.q_rows, qs, a.bn, a.dtype))
+      return cudaErrorInvalidValue;
+    return chunked ? launch(k_linear_mma<false, true>, grid, kMmaThreads, smem, a.splits, st, mp, mq, a)
+                   : launch(k_linear_mma<false, false>, grid, kMmaThreads, smem, a.splits, st, mp, mq, a);
+  }
+  return chunked ? launch(k_linear_mma<true, true>, grid, kLoaderThreads, smem, a.splits, st, mp, mq, a)
+                 : launch(k_linear_mma<true, false>, grid, kLoaderThreads, smem, a.splits, st, mp, mq, a);
+}
+
+cudaError_t take_linear_status(int* code, cudaStream_t st) {
+  cudaError_t e = cudaMemcpyFromSymbolAsync(code, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e != cudaSuccess || (e = cudaStreamSynchronize(st)) != cudaSuccess || *code == 0) return e;
+  const int none = 0;
+  if ((e = cudaMemcpyToSymbolAsync(g_status, &none, sizeof(int), 0, cudaMemcpyHostToDevice, st)) != cudaSuccess)
+    return e;
+  return cudaStreamSynchronize(st);
+}
+
+}  // namespace fw

@@ -37,6 +37,7 @@ EP_TRANSPORT_NCCL = 1
 # element types and scores of the primitives over torch tensors
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+_ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}  # FW_ACT_*
 _SCORES = {"softmax": SCORE_SOFTMAX, "sigmoid": SCORE_SIGMOID}
 
 # paths a forward takes (fw_moe_last_path)
@@ -79,6 +80,12 @@ class _RouteConfig(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int32) for name in (
         "experts", "top_k", "dtype", "scoring", "groups", "top_groups", "group_top", "renormalize")] + [
         ("scale", ctypes.c_float), ("logit_stride", ctypes.c_int64)]
+
+
+class _LinearConfig(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in (
+        "rows", "cols", "dtype", "out_dtype", "bias_dtype", "residual_dtype", "activation")] + [
+        (name, ctypes.c_int64) for name in ("w_stride", "x_stride", "residual_stride", "y_stride")]
 
 
 class _LogprobConfig(ctypes.Structure):
@@ -141,6 +148,8 @@ def library() -> ctypes.CDLL:
     L.fw_add_bf16.argtypes = [vp, vp, ctypes.c_int64, vp, vp]
     L.fw_route_bf16.argtypes = [vp, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, vp, vp, vp]
     L.fw_route_scores.argtypes = [ctypes.POINTER(_RouteConfig), vp, ctypes.c_int32, vp, vp, vp, vp, vp]
+    L.fw_linear_epilogue.argtypes = [ctypes.POINTER(_LinearConfig), vp, vp, ctypes.c_int32, vp, vp, vp, vp]
+    L.fw_primitive_status.argtypes = [vp]
     L.fw_token_logprobs.argtypes = [ctypes.POINTER(_LogprobConfig), vp, ctypes.c_int32, vp, vp, vp, vp, vp, vp]
     L.fw_moe_forward_noalloc.argtypes = [ctypes.POINTER(_Config), ctypes.POINTER(_Weights), vp,
                                          ctypes.c_int32, vp, vp, vp, vp]
@@ -155,7 +164,7 @@ def library() -> ctypes.CDLL:
                  "fw_safetensors_tensor_info", "fw_moe_get_config", "fw_moe_last_union", "fw_moe_last_path", "fw_moe_load_expert",
                  "fw_moe_load_expert_container", "fw_codec_container_check",
                  "fw_linear_bf16", "fw_swiglu_bf16", "fw_add_bf16", "fw_route_bf16", "fw_moe_forward_noalloc",
-                 "fw_route_scores", "fw_token_logprobs",
+                 "fw_route_scores", "fw_token_logprobs", "fw_linear_epilogue", "fw_primitive_status",
                  "fw_moe_ep_set_transport", "fw_moe_set_wait_limit", "fw_moe_test_stall"):
         getattr(L, name).restype = ctypes.c_int
     _lib = L
@@ -510,6 +519,41 @@ def _call(device: int, function, *args) -> None:
     else:
         with torch.cuda.device(device):
             _check(function(*args))
+
+
+def linear_epilogue(w, x, y, bias=None, activation: str = "none", residual=None, stream=None) -> None:
+    """y = act(x w^T + bias) + residual (fw_linear_epilogue).
+
+    w [N][K] and x [T][K] of one 16-bit type, y [T][N] of that type or f32,
+    bias [N], residual [T][N] (which may be y); all but bias may have strided
+    rows.  activation: none, relu, gelu, gelu_tanh, silu, sigmoid."""
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {tuple(_ACTIVATIONS)}")
+    pw, code, N, K, ws = _rows(w, "w", (DTYPE_BF16, DTYPE_F16))
+    dev = w.get_device()
+    px, _, T, _, xs = _rows(x, "x", (code,), None, K, dev)
+    py, out, _, _, ys = _rows(y, "y", (code, DTYPE_F32), T, N, dev)
+    pb = pr = None
+    bcode = rcode = code
+    rs = N
+    if bias is not None:
+        bcode = _codes().get(bias.dtype, -1)
+        if bcode < 0:
+            raise ValueError(f"bias: unsupported element type {bias.dtype}")
+        pb = _dense(bias, "bias", bcode, (N,), dev)
+    if residual is not None:
+        pr, rcode, _, _, rs = _rows(residual, "residual", (DTYPE_BF16, DTYPE_F16, DTYPE_F32), T, N, dev)
+    if T == 0:
+        return
+    c = _LinearConfig(N, K, code, out, bcode, rcode, act, ws, xs, rs, ys)
+    _call(dev, library().fw_linear_epilogue, ctypes.byref(c), pw, px, T, pb, pr, py, _stream(stream))
+
+
+def primitive_status(stream=None) -> None:
+    """Wait for `stream` and raise FwError if a linear_epilogue kernel on the
+    current device gave up a bounded wait."""
+    _check(library().fw_primitive_status(_stream(stream)))
 
 
 def route_scores(logits, indices, weights, scoring: str = "softmax", bias=None, groups: int = 1,

@@ -447,6 +447,44 @@ int fw_token_logprobs(const fw_logprob_config* config, const void* logits, int32
                       const int32_t* targets, float* logprobs, float* entropy, int32_t* top_idx,
                       float* top_logprobs, void* stream);
 
+/* y = act(x w^T + bias) + residual for the dense products around the block,
+ * stream-ordered, no workspace (linear_bf16, src/expert.rs:554-560, with an
+ * epilogue; sums in the tensor cores' order instead of the reference's, which
+ * fw_linear_bf16 keeps).
+ *   x [tokens][cols], w [rows][cols] of one 16-bit type (dtype:
+ *     FW_DTYPE_BF16 or FW_DTYPE_F16); y [tokens][rows] of that type or f32
+ *     (out_dtype); bias [rows] or NULL, residual [tokens][rows] or NULL, each
+ *     of any FW_DTYPE_*; strides in elements between rows, at least the
+ *     row's length;
+ *   products are summed in f32, bias, activation and residual are applied in
+ *   f32, and the result is rounded once.
+ * Any sizes, strides and element alignment: operands whose rows start on 16
+ * bytes are read by TMA, others are realigned on the way.  residual may be y
+ * itself (same pointer, stride and type); y overlaps nothing else.
+ * 1 <= rows, cols <= 2^24, 0 <= tokens <= 2^24, rows * tokens <= 2^38.
+ * Device pointers of the current device.  FW_EINVAL otherwise.
+ *   FW_ACT_GELU is x/2 (1 + erf(x / sqrt 2)), FW_ACT_GELU_TANH its tanh form,
+ *   FW_ACT_SILU x / (1 + exp(-x)). */
+#define FW_ACT_NONE 0
+#define FW_ACT_RELU 1
+#define FW_ACT_GELU 2
+#define FW_ACT_GELU_TANH 3
+#define FW_ACT_SILU 4
+#define FW_ACT_SIGMOID 5
+typedef struct fw_linear_config {
+    int32_t rows, cols;
+    int32_t dtype, out_dtype, bias_dtype, residual_dtype; /* FW_DTYPE_* */
+    int32_t activation;                                   /* FW_ACT_* */
+    int64_t w_stride, x_stride, residual_stride, y_stride;
+} fw_linear_config;
+int fw_linear_epilogue(const fw_linear_config* config, const void* w, const void* x, int32_t tokens,
+                       const void* bias, const void* residual, void* y, void* stream);
+
+/* Wait for `stream`, then report and clear the device-side status of
+ * fw_linear_epilogue on the current device: FW_ETIMEOUT when one of its
+ * kernels gave up a bounded wait (its y is then incomplete). */
+int fw_primitive_status(void* stream);
+
 /* Drop-in for the reference's only C ABI on the path,
  * `bool firewing_torch_topk_bf16(const uint16_t*, size_t, size_t, size_t*)`
  * (native/topk_shim.cpp:18-44, bound at src/decoder_layer.rs:19-39): HOST

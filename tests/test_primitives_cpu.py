@@ -74,3 +74,41 @@ def test_the_bindings_take_tensors_of_one_gpu():
         fw.token_logprobs(z[0], entropy=torch.zeros(2))
     with pytest.raises(ValueError, match="scoring"):
         fw.route_scores(z, i, torch.zeros(2, 2), scoring="tanh")
+
+
+def linear(**kw):
+    c = dict(rows=64, cols=32, dtype=0, out_dtype=0, bias_dtype=2, residual_dtype=0, activation=0, w_stride=32,
+             x_stride=32, residual_stride=64, y_stride=64)
+    c.update({k: v for k, v in kw.items() if k in c})
+    p = dict(w=FAKE, x=FAKE, tokens=1, bias=FAKE, residual=FAKE + 4096, y=FAKE)
+    p.update({k: v for k, v in kw.items() if k in p})
+    return fw.library().fw_linear_epilogue(ctypes.byref(moe._LinearConfig(**c)), *[p[k] for k in (
+        "w", "x", "tokens", "bias", "residual", "y")], None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(rows=0), dict(cols=0), dict(rows=(1 << 24) + 1, residual_stride=1 << 25, y_stride=1 << 25),
+    dict(cols=(1 << 24) + 1, w_stride=1 << 25, x_stride=1 << 25), dict(tokens=-1), dict(tokens=(1 << 24) + 1),
+    dict(rows=1 << 20, tokens=1 << 20, residual_stride=1 << 20, y_stride=1 << 20), dict(dtype=2), dict(dtype=3),
+    dict(out_dtype=1), dict(dtype=1), dict(bias_dtype=3), dict(residual_dtype=-1), dict(activation=-1),
+    dict(activation=6), dict(w_stride=31), dict(x_stride=31), dict(residual_stride=63), dict(y_stride=63),
+    dict(w_stride=1 << 38), dict(x_stride=1 << 38), dict(y_stride=1 << 38), dict(residual_stride=1 << 38),
+    dict(w=None), dict(x=None), dict(y=None), dict(w=FAKE + 1), dict(x=FAKE + 1), dict(y=FAKE + 1),
+    dict(out_dtype=2, y=FAKE + 2), dict(bias=FAKE + 2), dict(residual=FAKE + 1),
+    dict(residual=FAKE, residual_dtype=2), dict(residual=FAKE, residual_stride=65)])
+def test_linear_epilogue_refusals(bad):
+    assert linear(**bad) == fw.FW_EINVAL
+    assert fw.library().fw_last_error()
+
+
+def test_linear_epilogue_without_tokens_is_a_success():
+    assert linear(tokens=0) == fw.FW_OK
+
+
+def test_the_linear_binding_takes_tensors_of_one_gpu():
+    torch = pytest.importorskip("torch")
+    w, x, y = (torch.zeros(4, 4, dtype=torch.bfloat16) for _ in range(3))
+    with pytest.raises(ValueError, match="CUDA"):
+        fw.linear_epilogue(w, x, y)
+    with pytest.raises(ValueError, match="activation"):
+        fw.linear_epilogue(w, x, y, activation="tanh")
