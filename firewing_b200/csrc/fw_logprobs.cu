@@ -12,16 +12,16 @@
 // The reference: each warp takes the maximum of its first batch and changes
 // it only when a later value is over it by kSlack powers of two, which f32
 // sums stand without loss, so that the loop carries no maximum.
-// The alternatives: K values at least are >= `floor`, taken from the first
-// batch (the r-th largest of each warp's lane maxima, r = ceil(K / warps),
-// and the lowest of these over the warps).  Values under it cost one comparison
-// per lane and batch; the few others go to a list in shared memory.  A list
-// that overflows (a row of equal values, an ascending row) is made anew in a
-// second pass that cuts it back to K whenever it fills.
+// The alternatives: K values at least are >= `floor` (publish_floor), taken from
+// the first batch and raised after 1, 2, 4, ... of them.  Values under it cost
+// one comparison per lane and batch; the few others go to a list in shared
+// memory.  A list that overflows (a row of equal values, an ascending row) is
+// made anew in a second pass that cuts it back to K whenever it fills.
 //
 // Few rows: a row is split over the CTAs of a cluster, whose first CTA joins
 // the parts through distributed shared memory: no workspace, and sums in an
 // order that depends on the shape and the row's 16-byte alignment alone.
+#include <algorithm>
 #include <cstdint>
 
 #include <cooperative_groups.h>
@@ -39,10 +39,13 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kUnroll = 4;             // 16-byte loads in flight per thread
-constexpr int kList = 1024;            // candidates a CTA holds in the fast pass
+constexpr int kSeg = 128;              // candidates a warp holds in the fast pass
+constexpr int kList = kWarps * kSeg;   // and a CTA
+constexpr int kShare = kList / 8;      // keys a part of a split row may hand on
+constexpr int kRankMost = 384;         // candidates ranked by counting
 constexpr int kSlackLog2 = 16;         // how far over its reference (log2) a term may be
 constexpr int kMaxTop = 32;
-constexpr int kMaxSplits = 8;          // portable cluster size
+constexpr int kMaxSplits = 8;          // portable cluster size; kShare each fit `merged`
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -1.0e4f;     // floor of y: 2^y is 0, and 0 * y stays 0 for y = -inf
@@ -76,6 +79,15 @@ __device__ __forceinline__ uint64_t list_key(float v, int e) {
   return (static_cast<uint64_t>(ordered(__fadd_rn(v, 0.0f))) << 32) | static_cast<uint32_t>(~e);
 }
 
+// Halfwise maximum of a batch of 16-bit values (a NaN loses).
+template <typename R>
+__device__ __forceinline__ uint32_t highest2(const uint4 (&v)[kUnroll]) {
+  uint32_t h = R::kDead;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) h = R::max2(h, R::max2(R::max2(v[u].x, v[u].y), R::max2(v[u].z, v[u].w)));
+  return h;
+}
+
 template <int DT>
 struct Row;  // N values in 16 bytes
 template <>
@@ -85,6 +97,27 @@ struct Row<kBf16> {
   __device__ static __forceinline__ void unpack(uint4 v, float* x) {
     x[0] = lo_bf16(v.x), x[1] = hi_bf16(v.x), x[2] = lo_bf16(v.y), x[3] = hi_bf16(v.y);
     x[4] = lo_bf16(v.z), x[5] = hi_bf16(v.z), x[6] = lo_bf16(v.w), x[7] = hi_bf16(v.w);
+  }
+  __device__ static __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ static __forceinline__ float highest(const uint4 (&v)[kUnroll]) {
+    const uint32_t h = highest2<Row>(v);
+    return fmaxf(lo_bf16(h), hi_bf16(h));
+  }
+  // v, or the type's lowest value above it
+  __device__ static __forceinline__ float at_least(float v) { return bf16_to_f32(f32_to_bf16(fmaxf(v, -3.38e38f))); }
+  using Least = uint32_t;
+  __device__ static __forceinline__ Least spread(float v) { return (__float_as_uint(v) >> 16) * 0x10001u; }
+  __device__ static __forceinline__ uint32_t raise2(uint32_t w, uint32_t low) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(low));
+    return r;
+  }
+  __device__ static __forceinline__ void unpack_raised(uint4 v, Least low, float* x) {
+    unpack(make_uint4(raise2(v.x, low), raise2(v.y, low), raise2(v.z, low), raise2(v.w, low)), x);
   }
   __device__ static __forceinline__ float one(const void* p, long long i) {
     return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
@@ -102,6 +135,27 @@ struct Row<kF16> {
       x[2 * i + 1] = __half2float(__ushort_as_half(static_cast<uint16_t>(w[i] >> 16)));
     }
   }
+  __device__ static __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ static __forceinline__ float highest(const uint4 (&v)[kUnroll]) {
+    const uint32_t h = highest2<Row>(v);
+    return fmaxf(__half2float(__ushort_as_half(static_cast<uint16_t>(h))),
+                 __half2float(__ushort_as_half(static_cast<uint16_t>(h >> 16))));
+  }
+  __device__ static __forceinline__ float at_least(float v) { return __half2float(__float2half_rn(fmaxf(v, -65504.0f))); }
+  using Least = uint32_t;
+  __device__ static __forceinline__ Least spread(float v) { return __half_as_ushort(__float2half_rn(v)) * 0x10001u; }
+  __device__ static __forceinline__ uint32_t raise2(uint32_t w, uint32_t low) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(low));
+    return r;
+  }
+  __device__ static __forceinline__ void unpack_raised(uint4 v, Least low, float* x) {
+    unpack(make_uint4(raise2(v.x, low), raise2(v.y, low), raise2(v.z, low), raise2(v.w, low)), x);
+  }
   __device__ static __forceinline__ float one(const void* p, long long i) {
     return __half2float(__ushort_as_half(static_cast<const uint16_t*>(p)[i]));
   }
@@ -113,6 +167,25 @@ struct Row<kF32> {
   __device__ static __forceinline__ void unpack(uint4 v, float* x) {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y);
     x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+  }
+  __device__ static __forceinline__ float highest(const uint4 (&v)[kUnroll]) {
+    float h = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float x[N];
+      unpack(v[u], x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) h = fmaxf(h, x[i]);
+    }
+    return h;
+  }
+  __device__ static __forceinline__ float at_least(float v) { return fmaxf(v, -3.4e38f); }
+  using Least = float;
+  __device__ static __forceinline__ Least spread(float v) { return v; }
+  __device__ static __forceinline__ void unpack_raised(uint4 v, Least low, float* x) {
+    unpack(v, x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = max_nan(x[i], low);
   }
   __device__ static __forceinline__ float one(const void* p, long long i) { return static_cast<const float*>(p)[i]; }
 };
@@ -140,17 +213,23 @@ __device__ __forceinline__ Part join(const Part& a, const Part& b, float c) {
 }
 
 struct __align__(16) LogprobSmem {
-  uint64_t list[kList];
+  uint64_t list[kWarps][kSeg];     // each warp's candidates; all of it: the careful pass's list
+  uint64_t shortlist[kList];       // those of the CTA that reach the floor
+  uint64_t merged[kList];          // first CTA of a cluster: those of every part
   uint64_t best[kMaxTop];
+  uint4 lane_raw[kWarps][kUnroll];  // one lane's batch, looked at by its warp
   Part part[kWarps];
   Part whole;
   float floor[kWarps];
-  int count;
+  float part_floor;
+  int count;         // of list, in the careful pass
+  int short_count, merged_count;
+  int base;          // where this part's keys go in the first CTA's `merged`
   int found;
 };
 
 // The K largest keys of list[0..n) into best, descending; returns how many.
-// Called by one whole warp.
+// Called by one whole warp: K rounds of a maximum over the list.
 __device__ __forceinline__ int best_of(const uint64_t* list, int n, int K, uint64_t* best, int lane) {
   uint64_t last = ~0ull;
   for (int k = 0; k < K; ++k) {
@@ -169,48 +248,141 @@ __device__ __forceinline__ int best_of(const uint64_t* list, int n, int K, uint6
   return K;
 }
 
-// The careful pass: the candidates of row part [v0, v1) over again, the list
-// cut back to its K best whenever the next round might not fit.  All threads.
+// The K largest of list[0..n) into sm->best, by the whole CTA between
+// barriers of the caller; sets sm->found.  A short list is ranked at once, a
+// thread counting the keys above its own (all reads broadcasts); a long one
+// takes one warp K rounds.
+__device__ __forceinline__ void pick_best(LogprobSmem* sm, const uint64_t* list, int n, int K) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (n <= kRankMost) {
+    for (int base = warp * 32; base < n; base += kThreads) {
+      const int i = base + lane;
+      const uint64_t key = i < n ? list[i] : 0ull;
+      int above = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) above += list[j] > key ? 1 : 0;
+      if (i < n && above < K) sm->best[above] = key;
+    }
+    if (threadIdx.x == 0) sm->found = min(n, K);
+  } else if (warp == 0) {
+    const int found = best_of(list, n, K, sm->best, lane);
+    if (lane == 0) sm->found = found;
+  }
+}
+
+// This warp's share of a floor: the r-th largest of its lane maxima.  With
+// r = ceil(K / warps), K values at least reach the lowest share of `warps`
+// warps.  A share only grows, so one that is read late is still a floor.
+__device__ __forceinline__ void publish_floor(LogprobSmem* sm, float high, int r, int warp, int lane) {
+  uint32_t o = ordered(high), v = 0u;
+  for (int i = 0; i < r; ++i) {
+    v = __reduce_max_sync(kAll, o);
+    if (lane == __ffs(__ballot_sync(kAll, o == v)) - 1) o = 0u;
+  }
+  if (lane == 0) *reinterpret_cast<volatile float*>(&sm->floor[warp]) = from_ordered(v);
+}
+__device__ __forceinline__ float read_floor(const LogprobSmem* sm, int warps) {
+  float floor = INFINITY;
+  for (int i = 0; i < warps; ++i) floor = fminf(floor, *reinterpret_cast<const volatile float*>(&sm->floor[i]));
+  return floor;
+}
+
+// The careful pass, for row parts with a warp whose candidates overflowed its
+// list: the part [v0, v1) over again with one list, cut back to its K best
+// whenever the next round might not fit.  The K best end up in sm->best
+// (sm->found of them).  All threads.
 template <int DT>
 __device__ __noinline__ void collect_again(const LogprobArgs& a, long long row, int v0, int v1, LogprobSmem* sm) {
+  constexpr int kEach = 8;  // elements of a thread per step
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* list = &sm->list[0][0];
   __syncthreads();
-  if (threadIdx.x == 0) sm->count = kList;  // the list holds this many of the candidates
-  uint64_t floor = 0ull;
-  for (int base = v0; base < v1; base += kThreads) {
+  if (threadIdx.x == 0) sm->count = 0;
+  uint64_t last = 0ull;  // key of the K-th best at the last cut
+  float floor = -INFINITY;
+  auto cut_if_over = [&](int most) {
     __syncthreads();
     const int held = sm->count;
     __syncthreads();  // everyone has read the count that decides
-    if (held > kList - kThreads) {
-      if (warp == 0) {
-        const int n = best_of(sm->list, held, a.top_k, sm->best, lane);
-        __syncwarp();
-        if (lane < n) sm->list[lane] = sm->best[lane];
-        if (lane == 0) {
-          sm->count = n;
-          sm->found = n;
-        }
+    if (held <= most) return;
+    if (warp == 0) {
+      const int n = best_of(list, held, a.top_k, sm->best, lane);
+      __syncwarp();
+      if (lane < n) list[lane] = sm->best[lane];
+      if (lane == 0) {
+        sm->count = n;
+        sm->found = n;
       }
-      __syncthreads();
-      if (sm->found == a.top_k) floor = sm->best[a.top_k - 1];
     }
-    const int e = base + threadIdx.x;
-    if (e < v1) {
-      const float x = Row<DT>::one(a.logits, row + e);
-      const uint64_t key = list_key(x, e);
-      if (x > -INFINITY && key > floor) {
-        // The list may hold this element from the fast pass already.
-        bool there = false;
-        for (int i = 0; i < a.top_k; ++i) there |= sm->best[i] == key;
-        if (!there) sm->list[atomicAdd(&sm->count, 1)] = key;
-      }
+    __syncthreads();
+    if (sm->found == a.top_k) {
+      last = sm->best[a.top_k - 1];
+      floor = fmaxf(floor, from_ordered(static_cast<uint32_t>(last >> 32)));
+    }
+  };
+  for (int base = v0; base < v1; base += kEach * kThreads) {
+    float x[kEach];
+    float high = -INFINITY;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int e = base + i * kThreads + threadIdx.x;
+      x[i] = e < v1 ? Row<DT>::one(a.logits, row + e) : -INFINITY;
+      high = fmaxf(high, x[i]);
+      any |= x[i] > -INFINITY && list_key(x[i], e) > last;
+    }
+    // A step that ends the row may have lanes without values: no floor from it.
+    const bool whole = base + kEach * kThreads <= v1;
+    if (whole) publish_floor(sm, high, (a.top_k + kWarps - 1) / kWarps, warp, lane);
+    if (!__syncthreads_or(any)) continue;
+    if (whole) floor = fmaxf(floor, read_floor(sm, kWarps));
+#pragma unroll 1
+    for (int i = 0; i < kEach; ++i) {
+      cut_if_over(kList - kThreads);
+      const int e = base + i * kThreads + threadIdx.x;
+      float v = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) v = k == i ? x[k] : v;
+      const uint64_t key = list_key(v, e);
+      if (v > -INFINITY && v >= floor && key > last) list[atomicAdd(&sm->count, 1)] = key;
     }
   }
   __syncthreads();
+  if (threadIdx.x == 0) sm->found = 0;
+  cut_if_over(0);
+  __syncthreads();
+}
+
+// Two f32 values per 64-bit register, one instruction for both.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 pack(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack(F2 p, float* a, float* b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(p.v));
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) k_token_logprobs(LogprobArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_constant__ LogprobArgs a) {
   using R = Row<DT>;
   __shared__ LogprobSmem sm;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
@@ -226,43 +398,87 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs(LogprobArgs a) {
   // [head scalars][vectors][tail scalars]: vectors start on 16 bytes
   const unsigned char* p = static_cast<const unsigned char*>(a.logits) + (row + v0) * (16 / R::N);
   const int head = min(n, static_cast<int>((16u - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / (16 / R::N));
-    const int nvec = (n - head) / R::N;
+  const int nvec = (n - head) / R::N;
   const int first = v0 + head;             // element of vector 0
   const int tail = first + nvec * R::N;    // elements [tail, v1)
   const uint4* vec = reinterpret_cast<const uint4*>(p + static_cast<size_t>(head) * (16 / R::N));
 
-  if (tid == 0) sm.count = 0;
-  Part acc = {-INFINITY, 0.0f, 0.0f};
-  float m = 0.0f, limit = -INFINITY;  // reference, and the value from which it has to change
-  float floor = INFINITY;             // candidates are >= floor
+  // A given token's logit is fetched while the row is read.
+  int target = -1;
+  float target_x = 0.0f;
+  if (part == 0 && tid < a.targets_per_row) {
+    target = a.targets[static_cast<long long>(t) * a.targets_per_row + tid];
+    if (target >= 0 && target < a.vocab) target_x = R::one(a.logits, row + target);
+  }
 
-  auto add = [&](float x) {
-    const float y = max_nan(__fmul_rn(__fsub_rn(x, m), c), kLowest);
-    const float e = ex2(y);
-    acc.s = __fadd_rn(acc.s, e);
-    acc.w = __fmaf_rn(e, y, acc.w);
+  if (tid == 0) sm.short_count = sm.merged_count = 0;
+  // The warp's reference M; a value from `limit` on changes it.  With mc =
+  // fl(M c) the terms are y = fma(z, c, -mc), which is (z - M) c + off for
+  // one small `off` common to the warp: taken out again at the end.  Values
+  // are raised to `least`, far enough below M for 2^y to be 0, so that a
+  // masked -inf adds 0 * y = 0.  Where the type has no such number (M near
+  // its lowest value, or a high temperature), or M c overflows, `plain` terms
+  // are computed as max((z - M) c, kLowest).
+  float m = -INFINITY, limit = -INFINITY, mc = 0.0f, least = 0.0f;
+  bool plain = false;
+  F2 s2 = pack(0.0f, 0.0f), w2 = pack(0.0f, 0.0f);  // the lane's sums, even and odd elements
+  float seen = -INFINITY;                            // the lane's maximum so far
+  float floor = INFINITY;                            // candidates are >= floor
+
+  // (S, W) against the exact reference M.
+  auto settle = [&]() {
+    if (plain || m == -INFINITY) return;
+    const float off = __fmaf_rn(m, c, -mc);
+    const F2 f = pack(ex2(-off), ex2(-off));
+    w2 = mul2(fma2(pack(-off, -off), s2, w2), f);
+    s2 = mul2(s2, f);
   };
-  // The warp's reference covers `high` (the warp's values' maximum).
+  // The warp's reference covers `high` (lane maxima).
   auto cover = [&](float high) {
-    if (__any_sync(kAll, high > limit)) {
-      const float to = warp_max(high);
-      if (acc.m > -INFINITY) {
-        const float d = max_nan(__fmul_rn(__fsub_rn(acc.m, to), c), kLowest);
-        const float f = ex2(d);
-        acc.w = __fmul_rn(__fmaf_rn(d, acc.s, acc.w), f);
-        acc.s = __fmul_rn(acc.s, f);
-      }
-      acc.m = m = to;
-      limit = __fadd_rn(to, a.slack);
+    if (!__any_sync(kAll, high > limit)) return;
+    const float to = warp_max(high);
+    if (m > -INFINITY) {
+      settle();
+      const float d = max_nan(__fmul_rn(__fsub_rn(m, to), c), kLowest);
+      const F2 f = pack(ex2(d), ex2(d));
+      w2 = mul2(fma2(pack(d, d), s2, w2), f);
+      s2 = mul2(s2, f);
+    }
+    m = to;
+    limit = __fadd_rn(to, a.slack);
+    mc = __fmul_rn(m, c);
+    least = R::at_least(__fsub_rn(m, a.depth));
+    plain = !(fabsf(mc) < 1e30f && __fmul_rn(__fsub_rn(least, m), c) < -1000.0f);
+    if (!plain) {  // the sums go on against the rounded reference
+      const float off = __fmaf_rn(m, c, -mc);
+      const F2 f = pack(ex2(off), ex2(off));
+      w2 = mul2(fma2(pack(off, off), s2, w2), f);
+      s2 = mul2(s2, f);
     }
   };
+  auto add = [&](float x0, float x1) {  // raised to `least` already
+    float y0, y1;
+    const F2 y = fma2(pack(x0, x1), pack(c, c), pack(-mc, -mc));
+    unpack(y, &y0, &y1);
+    const F2 e = pack(ex2(y0), ex2(y1));
+    s2 = add2(s2, e);
+    w2 = fma2(e, y, w2);
+  };
+  auto add_plain = [&](float x) {
+    // (no reference yet: every value is -inf, or NaN)
+    const float y = max_nan(__fmul_rn(__fsub_rn(x, m == -INFINITY ? 0.0f : m), c), kLowest);
+    const float e = ex2(y);
+    s2 = add2(s2, pack(e, 0.0f));
+    w2 = fma2(pack(e, 0.0f), pack(y, 0.0f), w2);
+  };
+  int held = 0;  // candidates of this warp, listed up to kSeg
   auto offer = [&](float x, int e) {
-    if (x >= floor && x > -INFINITY) {
-      const int at = atomicAdd(&sm.count, 1);
-      if (at < kList) sm.list[at] = list_key(x, e);
-    }
+    const bool in = x >= floor && x > -INFINITY;
+    const unsigned who = __ballot_sync(kAll, in);
+    const int at = held + __popc(who & ((1u << lane) - 1u));
+    if (in && at < kSeg) sm.list[warp][at] = list_key(x, e);
+    held += __popc(who);
   };
-  __syncthreads();
 
   // Head and tail: at most 2 (N - 1) elements, one per lane of warp 0.
   float ragged = -INFINITY;
@@ -272,111 +488,183 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs(LogprobArgs a) {
     else if (lane - head < v1 - tail) ragged_e = tail + lane - head;
     if (lane < head + (v1 - tail)) ragged = R::one(a.logits, row + ragged_e);
     cover(ragged);
-    if (lane < head + (v1 - tail)) add(ragged);
+    if (lane < head + (v1 - tail)) {
+      if (plain || m == -INFINITY) add_plain(ragged);
+      else add(max_nan(ragged, least), least);
+    }
   }
 
-  for (int j0 = 0; j0 < nvec; j0 += kThreads * kUnroll) {
+  const int full = min(kWarps, nvec / 32);  // warps whose lanes all have values
+  const uint4 dead = make_uint4(R::kDead, R::kDead, R::kDead, R::kDead);
+  uint4 next[kUnroll];
+  auto fetch = [&](int j0) {
+    if (j0 + kThreads * kUnroll <= nvec) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) next[u] = ldg_stream(vec + j0 + u * kThreads + tid);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int j = j0 + u * kThreads + tid;
+        next[u] = j < nvec ? ldg_stream(vec + j) : dead;
+      }
+    }
+  };
+  fetch(0);
+  const int share = full > 0 ? (K + full - 1) / full : 0;
+  int raise_at = 1;
+  for (int j0 = 0, batch = 1; j0 < nvec; j0 += kThreads * kUnroll, ++batch) {
     uint4 raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int j = j0 + u * kThreads + tid;
-      raw[u] = j < nvec ? ldg_stream(vec + j) : make_uint4(R::kDead, R::kDead, R::kDead, R::kDead);
-    }
-    float high = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float x[R::N];
-      R::unpack(raw[u], x);
-#pragma unroll
-      for (int i = 0; i < R::N; ++i) high = fmaxf(high, x[i]);
-    }
+    for (int u = 0; u < kUnroll; ++u) raw[u] = next[u];
+    fetch(j0 + kThreads * kUnroll);
+    const float high = R::highest(raw);
     cover(high);
     if (K > 0) {
-      if (j0 == 0) {
-        // r-th largest lane maximum of each warp whose lanes all have values
-        const int full = min(kWarps, nvec / 32);
-        if (full > 0) {
-          uint32_t o = ordered(high), r = 0u;
-          for (int i = 0; i < (K + full - 1) / full; ++i) {
-            r = __reduce_max_sync(kAll, o);
-            if (lane == __ffs(__ballot_sync(kAll, o == r)) - 1) o = 0u;
-          }
-          if (lane == 0) sm.floor[warp] = from_ordered(r);
-        }
-        __syncthreads();
-        floor = full > 0 ? sm.floor[0] : -INFINITY;
-        for (int i = 1; i < full; ++i) floor = fminf(floor, sm.floor[i]);
+      seen = fmaxf(seen, high);
+      // Raised after 1, 2, 4, ... batches, so that each stretch of the row
+      // leaves about as many candidates as the first batch.  Only the first
+      // time do the warps wait for one another's shares.
+      if (batch == raise_at) {
+        publish_floor(&sm, seen, share, warp, lane);
+        if (batch == 1) __syncthreads();
+        else __syncwarp();
+        floor = full > 0 ? read_floor(&sm, full) : -INFINITY;
+        raise_at *= 2;
       }
-      if (high >= floor) {
+      // A lane that has a candidate shows its batch to the warp, an element
+      // for each lane.
+      for (unsigned who = __ballot_sync(kAll, high >= floor); who != 0u; who &= who - 1u) {
+        const int src = __ffs(who) - 1;
+        __syncwarp();
+        if (lane == src) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          float x[R::N];
-          R::unpack(raw[u], x);
-#pragma unroll
-          for (int i = 0; i < R::N; ++i) offer(x[i], first + (j0 + u * kThreads + tid) * R::N + i);
+          for (int u = 0; u < kUnroll; ++u) sm.lane_raw[warp][u] = raw[u];
         }
+        __syncwarp();
+        const float x = lane < kUnroll * R::N ? R::one(sm.lane_raw[warp], lane) : -INFINITY;
+        offer(x, first + (j0 + lane / R::N * kThreads + warp * 32 + src) * R::N + lane % R::N);
       }
     }
+    if (!plain && m > -INFINITY) {
+      const typename R::Least low = R::spread(least);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float x[R::N];
-      R::unpack(raw[u], x);
+      for (int u = 0; u < kUnroll; ++u) {
+        float x[R::N];
+        R::unpack_raised(raw[u], low, x);
 #pragma unroll
-      for (int i = 0; i < R::N; ++i) add(x[i]);
+        for (int i = 0; i < R::N; i += 2) add(x[i], x[i + 1]);
+      }
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < kUnroll; ++u) {
+        uint4 v = raw[0];
+#pragma unroll
+        for (int k = 1; k < kUnroll; ++k) v = k == u ? raw[k] : v;
+        float x[R::N];
+        R::unpack(v, x);
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) add_plain(x[i]);
+      }
     }
   }
-  if (K > 0 && warp == 0 && lane < head + (v1 - tail)) {
+  if (K > 0 && warp == 0) {
     if (nvec == 0) floor = -INFINITY;
     offer(ragged, ragged_e);
+    seen = fmaxf(seen, ragged);
   }
+  settle();
 
-  // Join the warps.
-  acc.s = warp_sum(acc.s);
-  acc.w = warp_sum(acc.w);
+  // Join the lanes, then the warps.
+  float s_even, s_odd, w_even, w_odd;
+  unpack(s2, &s_even, &s_odd);
+  unpack(w2, &w_even, &w_odd);
+  Part acc;
+  acc.m = m;
+  acc.s = warp_sum(__fadd_rn(s_even, s_odd));
+  acc.w = warp_sum(__fadd_rn(w_even, w_odd));
   if (lane == 0) sm.part[warp] = acc;
-  __syncthreads();
-  if (K > 0 && sm.count > kList) collect_again<DT>(a, row, v0, v1, &sm);
-  if (warp == 0) {
-    if (K > 0) {
-      const int found = best_of(sm.list, min(sm.count, kList), K, sm.best, lane);
-      if (lane == 0) sm.found = found;
+  if (K > 0) publish_floor(&sm, seen, share, warp, lane);
+  const bool over = __syncthreads_or(held > kSeg);
+  const Part none = {-INFINITY, 0.0f, 0.0f};
+  // parts[0..n) joined in a fixed order by one warp (n <= 8)
+  auto join_all = [&](Part p) {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      Part q;
+      q.m = __shfl_xor_sync(kAll, p.m, o);
+      q.s = __shfl_xor_sync(kAll, p.s, o);
+      q.w = __shfl_xor_sync(kAll, p.w, o);
+      p = (lane & o) != 0 ? join(q, p, c) : join(p, q, c);
     }
-    if (lane == 0) {
-      Part whole = sm.part[0];
-      for (int i = 1; i < kWarps; ++i) whole = join(whole, sm.part[i], c);
-      sm.whole = whole;
-    }
-    __syncwarp();
+    return p;
+  };
+  if (warp == kWarps - 1) {
+    const Part whole = join_all(lane < kWarps ? sm.part[lane] : none);
+    if (lane == 0) sm.whole = whole;
   }
-
-  // Join the parts of the row in its first CTA.
-  if (a.splits > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    if (part == 0 && warp == 0) {
-      if (lane == 0) {
-        Part whole = sm.whole;
-        for (int r = 1; r < a.splits; ++r) whole = join(whole, cluster.map_shared_rank(&sm, r)->whole, c);
-        sm.whole = whole;
-      }
-      if (K > 0) {
-        int total = 0;
-        for (int r = 0; r < a.splits; ++r) {
-          const LogprobSmem* other = cluster.map_shared_rank(&sm, r);
-          const int found = other->found;
-          if (lane < found) sm.list[total + lane] = other->best[lane];
-          total += found;
-        }
-        __syncwarp();
-        const int found = best_of(sm.list, total, K, sm.best, lane);
-        __syncwarp();
-        if (lane == 0) sm.found = found;
-      }
+  cg::cluster_group cluster = cg::this_cluster();
+  const bool split = a.splits > 1;
+  if (K > 0) {
+    if (over) {
+      collect_again<DT>(a, row, v0, v1, &sm);
+      const int found = sm.found;
+      floor = found == K ? from_ordered(static_cast<uint32_t>(sm.best[K - 1] >> 32)) : -INFINITY;
+      held = warp == 0 ? found : 0;
+      if (warp == 0 && lane < found) sm.list[0][lane] = sm.best[lane];
       __syncwarp();
+    } else {
+      floor = full > 0 ? read_floor(&sm, full) : -INFINITY;
     }
-    cluster.sync();  // the others' shared memory stays until it has been read
-    if (part != 0) return;
   }
+  if (split) {
+    if (tid == 0) sm.part_floor = floor;
+    cluster.sync();
+    if (K > 0)  // K values of the row reach the best part's floor
+      floor = warp_max(lane < a.splits ? cluster.map_shared_rank(&sm, lane)->part_floor : -INFINITY);
+    if (part == 0 && warp == kWarps - 1) {
+      const Part whole = join_all(lane < a.splits ? cluster.map_shared_rank(&sm, lane)->whole : none);
+      __syncwarp();
+      if (lane == 0) sm.whole = whole;
+    }
+  }
+  if (K > 0) {
+    // This part's candidates that reach the floor.
+    const uint64_t least_key = static_cast<uint64_t>(ordered(__fadd_rn(floor, 0.0f))) << 32;
+    for (int i = lane; i - lane < held; i += 32) {
+      const uint64_t key = i < held ? sm.list[warp][i] : 0ull;
+      const bool in = key != 0ull && key >= least_key;
+      const unsigned who = __ballot_sync(kAll, in);
+      if (who == 0u) continue;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&sm.short_count, __popc(who));
+      at = __shfl_sync(kAll, at, 0) + __popc(who & ((1u << lane) - 1u));
+      if (in) sm.shortlist[at] = key;
+    }
+    __syncthreads();
+    int n = sm.short_count;
+    const uint64_t* keys = sm.shortlist;
+    if (split) {
+      // All parts' keys to the first CTA, no more than kShare from each.
+      if (n > kShare) {
+        pick_best(&sm, keys, n, K);
+        __syncthreads();
+        keys = sm.best;
+        n = sm.found;
+      }
+      LogprobSmem* to = cluster.map_shared_rank(&sm, 0);
+      if (tid == 0) sm.base = n > 0 ? atomicAdd(&to->merged_count, n) : 0;
+      __syncthreads();
+      if (tid < n) to->merged[sm.base + tid] = keys[tid];
+      cluster.sync();
+      keys = sm.merged;
+      n = sm.merged_count;
+    }
+    if (part != 0) return;
+    pick_best(&sm, keys, n, K);
+  } else if (split) {
+    cluster.sync();  // the others' sums stay until they have been read
+  }
+  if (part != 0) return;
   __syncthreads();
 
   const Part whole = sm.whole;
@@ -393,10 +681,13 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs(LogprobArgs a) {
   };
   for (int i = tid; i < a.targets_per_row; i += kThreads) {
     const long long o = static_cast<long long>(t) * a.targets_per_row + i;
-    const int e = a.targets[o];
-    a.logprobs[o] = e < 0 ? 0.0f : e >= a.vocab ? nan : logprob(R::one(a.logits, row + e));
+    if (i != tid) {
+      target = a.targets[o];
+      if (target >= 0 && target < a.vocab) target_x = R::one(a.logits, row + target);
+    }
+    a.logprobs[o] = target < 0 ? 0.0f : target >= a.vocab ? nan : logprob(target_x);
   }
-  if (a.entropy != nullptr && tid == 0)
+  if (a.entropy != nullptr && tid == kThreads - 1)
     a.entropy[t] = bad ? nan : empty ? 0.0f : __fmul_rn(__fsub_rn(log_s, __fdiv_rn(whole.w, whole.s)), kLn2);
   if (tid < K) {
     const long long o = static_cast<long long>(t) * K + tid;
@@ -415,11 +706,10 @@ cudaError_t launch_token_logprobs(LogprobArgs a, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   a.scale = kLog2e * a.inv_temperature;
   a.slack = static_cast<float>(kSlackLog2) / a.scale;
-  // Two CTAs per SM at least, while a part has 4096 values.
-  int splits = 1;
-  while (splits < kMaxSplits && static_cast<long long>(a.tokens) * splits < 2 * dev.sms &&
-         a.vocab / (2 * splits) >= 4096)
-    splits *= 2;
+  a.depth = 20000.0f / a.scale;
+  // Few rows: as many parts as the GPU has room for at once (three CTAs per
+  // SM), of 4096 values at least.
+  const int splits = std::max(1, std::min({kMaxSplits, 3 * dev.sms / a.tokens, a.vocab / 4096}));
   a.splits = splits;
   a.part_len = ((a.vocab + splits - 1) / splits + 7) & ~7;
   cudaLaunchConfig_t cfg = {};

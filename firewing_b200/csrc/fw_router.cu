@@ -15,6 +15,7 @@
 // than the bound allows is decided again in 64 bits by the same warp.
 //
 // One warp per token; lane l holds the experts l, l + 32, ...
+#include <algorithm>
 #include <cstdint>
 
 #include <cuda_fp16.h>
@@ -31,10 +32,10 @@ constexpr unsigned kAll = 0xffffffffu;
 
 // Bounds of the f32 scores' errors.  z * log2(e) is off by 2^-23.4 |z log2 e|,
 // ex2.approx by 2^-22 relative; for the sigmoid both reach s scaled by
-// s (1 - s), with 1 + t, and the quotient adding 2^-23: under 2^-21.8 in
-// all.  For the softmax the sum of at most 32 terms per lane and 5 tree
+// s (1 - s) (at most 1/4, and 0.224 / |z|), 1 + t adds 2^-24 and the quotient
+// 2^-22: under 2^-21.3 in all.  For the softmax the sum of at most 32 terms per lane and 5 tree
 // steps adds 37 * 2^-24 relative: under 2^-18.3 of s.
-constexpr float kSigmoidError = 0x1p-20f;          // absolute
+constexpr float kSigmoidError = 0x1p-21f;          // absolute
 constexpr float kSoftmaxError = 0x1p-18f;          // relative to the row's largest score
 constexpr float kAddError = 0x1p-23f;              // one f32 addition, relative to its result
 
@@ -57,6 +58,13 @@ __device__ __forceinline__ float load_logit(const void* p, long long i, int dtyp
   if (dtype == kF32) return static_cast<const float*>(p)[i];
   const uint16_t v = static_cast<const uint16_t*>(p)[i];
   return dtype == kBf16 ? bf16_to_f32(v) : __half2float(__ushort_as_half(v));
+}
+
+template <int DT>
+__device__ __forceinline__ float logit_of(const void* p, long long i) {
+  if (DT == kF32) return static_cast<const float*>(p)[i];
+  const uint16_t v = static_cast<const uint16_t*>(p)[i];
+  return DT == kBf16 ? bf16_to_f32(v) : __half2float(__ushort_as_half(v));
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -112,47 +120,51 @@ __device__ __forceinline__ unsigned choose_groups(const F* keys, const RouteScor
   return __ballot_sync(kAll, chosen && l == 0);
 }
 
-// The selection in 64 bits, for the rows that f32 does not decide: lane k
-// returns the k-th selected expert, -1 where there is none.
-__device__ __noinline__ int select_in_64_bits(const RouteScoreArgs& a, long long row, int lanes, double* keys,
-                                              int lane) {
-  const double none = -INFINITY;
+// Score (and bias) of a logit in 64 bits; top and sum are the softmax's.
+__device__ __forceinline__ double key_in_64_bits(const RouteScoreArgs& a, double z, int e, double top, double sum) {
+  double key = a.scoring == kScoreSoftmax ? exp(z - top) / sum : 1.0 / (1.0 + exp(-z));
+  if (a.bias != nullptr) key += static_cast<double>(a.bias[e]);
+  return z == -INFINITY ? -INFINITY : key;
+}
+__device__ __noinline__ double softmax_sum_in_64_bits(const void* logits, int dtype, long long row, int E, double top,
+                                                      int lane) {
+  double sum = 0.0;
+  for (int e = lane; e < E; e += 32) sum += exp(static_cast<double>(load_logit(logits, row + e, dtype)) - top);
+  return warp_sum(sum);
+}
+// The groups chosen by 64-bit scores, for a row whose f32 scores leave the
+// border open; the row's keys stay in `keys`.
+__device__ __noinline__ unsigned groups_in_64_bits(const RouteScoreArgs& a, long long row, double top, double sum,
+                                                   int lanes, double* keys, int lane) {
+  __syncwarp();
+  for (int e = lane; e < a.experts; e += 32) {
+    const int g = (e * a.group_inv) >> 20;
+    keys[e + g * lanes] = key_in_64_bits(a, load_logit(a.logits, row + e, a.dtype), e, top, sum);
+  }
+  __syncwarp();
+  double gap, high;
+  const unsigned chosen = choose_groups<double>(keys, a, lanes, lane, &gap, &high);
+  __syncwarp();
+  return chosen;
+}
+// Repeated maxima of 64-bit keys, for a row with more near ties than are
+// ranked: lane k returns the k-th selected expert, -1 where there is none.
+__device__ __noinline__ int select_in_64_bits(const RouteScoreArgs& a, long long row, double top, double sum,
+                                              unsigned chosen, int lanes, double* keys, int lane) {
   const int E = a.experts;
-  double top = none, sum = 0.0;
-  if (a.scoring == kScoreSoftmax) {
-    for (int e = lane; e < E; e += 32) top = fmax(top, static_cast<double>(load_logit(a.logits, row + e, a.dtype)));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(kAll, top, o));
-    for (int e = lane; e < E; e += 32) sum += exp(static_cast<double>(load_logit(a.logits, row + e, a.dtype)) - top);
-    sum = warp_sum(sum);
-  }
   __syncwarp();
-  for (int e = lane; e < E; e += 32) {
-    const double z = load_logit(a.logits, row + e, a.dtype);
-    double key = a.scoring == kScoreSoftmax ? exp(z - top) / sum : 1.0 / (1.0 + exp(-z));
-    if (a.bias != nullptr) key += static_cast<double>(a.bias[e]);
-    if (z == none) key = none;
-    const int g = e / a.group_size;
-    keys[e + g * lanes] = key;
-  }
+  for (int e = lane; e < E; e += 32)
+    keys[e] = key_in_64_bits(a, load_logit(a.logits, row + e, a.dtype), e, top, sum);
   __syncwarp();
-  unsigned chosen = kAll;
-  if (a.groups > 1) {
-    double gap, high;
-    chosen = choose_groups<double>(keys, a, lanes, lane, &gap, &high);
-  }
   int mine = -1;
   double last = INFINITY;
   int last_e = -1;
   for (int k = 0; k < a.top_k; ++k) {
-    double best = none;
+    double best = -INFINITY;
     int best_e = E;
     for (int e = lane; e < E; e += 32) {
-      const int g = e / a.group_size;
-      if (a.groups > 1 && !((chosen >> (g * lanes)) & 1u)) continue;
-      const double key = keys[e + g * lanes];
-      if (key == none) continue;
-      const double v = a.bias != nullptr ? key : static_cast<double>(load_logit(a.logits, row + e, a.dtype));
+      const double v = keys[e];
+      if (v == -INFINITY || !((chosen >> ((((e * a.group_inv) >> 20) * lanes) & 31)) & 1u)) continue;
       if ((v < last || (v == last && e > last_e)) && (v > best || best_e == E)) {
         best = v;
         best_e = e;
@@ -175,191 +187,343 @@ __device__ __noinline__ int select_in_64_bits(const RouteScoreArgs& a, long long
   __syncwarp();
   return mine;
 }
+// The `n` candidates (ids in id[0..n)) ranked by 64-bit keys: lane k returns
+// the k-th.
+__device__ __noinline__ int rank_in_64_bits(const RouteScoreArgs& a, long long row, double top, double sum, int n,
+                                            double* keys, const int* id, int lane) {
+  const int eu = lane < n ? id[lane] : 0, ev = lane + 32 < n ? id[lane + 32] : 0;
+  const double u = key_in_64_bits(a, load_logit(a.logits, row + eu, a.dtype), eu, top, sum);
+  const double v = key_in_64_bits(a, load_logit(a.logits, row + ev, a.dtype), ev, top, sum);
+  keys[lane] = u;
+  keys[lane + 32] = v;
+  __syncwarp();
+  int ru = 0, rv = 0;
+  for (int j = 0; j < n; ++j) {
+    const double o = keys[j];
+    const int e = id[j];
+    ru += (o > u || (o == u && e < eu)) ? 1 : 0;
+    rv += (o > v || (o == v && e < ev)) ? 1 : 0;
+  }
+  __syncwarp();
+  int* order = reinterpret_cast<int*>(keys);
+  if (lane < n) order[ru] = eu;
+  if (lane + 32 < n) order[rv] = ev;
+  __syncwarp();
+  const int mine = lane < n ? order[lane] : -1;
+  __syncwarp();
+  return mine;
+}
 
-// NE experts per lane (E <= 32 * NE).
+// Lane maxima sorted over the warp, descending: lane k returns the k-th.
+__device__ __forceinline__ uint32_t sort_lanes(uint32_t v, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1) {
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const uint32_t o = __shfl_xor_sync(kAll, v, j);
+      const bool keep_max = ((lane & k) == 0) == ((lane & j) == 0);
+      v = keep_max ? max(v, o) : min(v, o);
+    }
+  }
+  return v;
+}
+
+// The first `rounds` experts in the order of `order` (0: dead) by repeated
+// maxima: lane k gets the k-th one's key and id (id -1 when there is none).
+// For the rows whose candidates do not fit the ranking.
 template <int NE>
-__global__ void __launch_bounds__(32 * kRouteWarps) k_route_scores(RouteScoreArgs a) {
+__device__ __noinline__ void select_by_rounds(const uint32_t* order_in, int rounds, int lane, uint32_t* key, int* id) {
+  uint32_t last = 0xffffffffu;
+  int last_e = 0x7fffffff;
+  *key = 0u;
+  *id = -1;
+  for (int k = 0; k < rounds; ++k) {
+    uint32_t b = 0u;
+    int be = 0x7fffffff;
+    for (int i = 0; i < NE; ++i) {
+      const int e = i * 32 + lane;
+      const uint32_t v = order_in[i];
+      if ((v < last || (v == last && e > last_e)) && v > b) {
+        b = v;
+        be = e;
+      }
+    }
+    const uint32_t m = __reduce_max_sync(kAll, b);
+    if (m == 0u) break;
+    const int e = static_cast<int>(__reduce_min_sync(kAll, b == m ? static_cast<unsigned>(be) : 0x7fffffffu));
+    if (lane == k) {
+      *key = m;
+      *id = e;
+    }
+    last = m;
+    last_e = e;
+  }
+}
+
+// Shared memory of one warp: f32 or f64 keys of a row (group g shifted by
+// g * lanes <= 32), or the candidates being ranked.
+constexpr int kRanked = 64;
+constexpr int kRankedDoubles = kRanked + kRanked / 2;  // keys and ids
+__host__ __device__ inline int warp_doubles(int experts) {
+  return experts + 32 > kRankedDoubles ? experts + 32 : kRankedDoubles;
+}
+
+// NE experts per lane (E <= 32 * NE), logits of type DT.  A warp takes the
+// rows warp, warp + warps, ...; the next row's logits are on their way while
+// one is routed.
+template <int NE, int DT>
+__global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? 4 : 2) k_route_scores(const __grid_constant__ RouteScoreArgs a) {
   extern __shared__ __align__(16) unsigned char route_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int t = blockIdx.x * kRouteWarps + warp;
-  if (t >= a.tokens) return;
   const int E = a.experts, K = a.top_k;
-  const long long row = static_cast<long long>(t) * a.stride;
-  // 64-bit keys of one row per warp; the f32 keys use the same memory
-  double* keys64 = reinterpret_cast<double*>(route_smem) + static_cast<size_t>(warp) * (E + 32);
+  double* keys64 = reinterpret_cast<double*>(route_smem) + static_cast<size_t>(warp) * warp_doubles(E);
   float* keys = reinterpret_cast<float*>(keys64);
+  uint64_t* ranked = reinterpret_cast<uint64_t*>(keys64);
+  int* loads = reinterpret_cast<int*>(reinterpret_cast<double*>(route_smem) + kRouteWarps * warp_doubles(E));
   const bool softmax = a.scoring == kScoreSoftmax;
   const bool biased = a.bias != nullptr;
   const bool grouped = a.groups > 1;
   const int lanes = a.lanes;
+  const int first = blockIdx.x * kRouteWarps + warp, step = gridDim.x * kRouteWarps;
+  if (a.counts != nullptr) {
+    for (int e = threadIdx.x; e < E; e += blockDim.x) loads[e] = 0;
+    __syncthreads();
+  }
+  pdl_wait();
+  pdl_launch_dependents();
 
-  float z[NE];
-  bool bad = false;
-  float top = -INFINITY;
+  float next[NE], bias[NE];
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int e = i * 32 + lane;
-    z[i] = e < E ? load_logit(a.logits, row + e, a.dtype) : -INFINITY;
+    next[i] = e < E && first < a.tokens ? logit_of<DT>(a.logits, first * a.stride + e) : -INFINITY;
+    bias[i] = biased && e < E ? a.bias[e] : 0.0f;
   }
-#pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    bad |= z[i] != z[i];
-    z[i] = __fadd_rn(z[i], 0.0f);  // -0 and +0 are one value
-    top = fmaxf(top, z[i]);
-  }
-  top = warp_max(top);
-  bad |= softmax && top == INFINITY;
 
-  // Scores and keys.
-  uint32_t order[NE];
-  float sum = 0.0f;
-  float error = kSigmoidError;
-  if (softmax && (biased || grouped || !a.renormalize)) {
-    const float ref = top == -INFINITY ? 0.0f : top;
+  for (int t = first; t < a.tokens; t += step) {
+    const long long row = t * a.stride;
+    float z[NE];
+    bool bad = false;
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) sum = __fadd_rn(sum, ex2(__fmul_rn(__fsub_rn(z[i], ref), kLog2e)));
-    sum = warp_sum(sum);
-    error = __fdividef(kSoftmaxError, sum);
-  }
-#pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const int e = i * 32 + lane;
-    float key = z[i];
-    if (biased || grouped) {
-      float s;
-      if (softmax) s = __fdividef(ex2(__fmul_rn(__fsub_rn(z[i], top), kLog2e)), sum);
-      else s = __fdividef(1.0f, __fadd_rn(1.0f, ex2(__fmul_rn(-z[i], kLog2e))));
-      if (biased && e < E) {
-        key = __fadd_rn(__fadd_rn(s, a.bias[e]), 0.0f);
-        bad |= key != key && z[i] > -INFINITY && !(softmax && top == -INFINITY);
-      }
-      if (z[i] == -INFINITY) key = -INFINITY;
-      if (grouped && e < E) {
-        const int g = (e * a.group_inv) >> 20;
-        keys[e + g * lanes] = biased || z[i] == -INFINITY ? key : s;
-      }
+    for (int i = 0; i < NE; ++i) {
+      bad |= next[i] != next[i];
+      z[i] = __fadd_rn(next[i], 0.0f);  // -0 and +0 are one value
+      top = fmaxf(top, z[i]);
     }
-    order[i] = key == -INFINITY ? 0u : ordered(key);
-  }
-  bad = __any_sync(kAll, bad);
+    const bool more = t + step < a.tokens;
+    const long long next_row = (t + static_cast<long long>(step)) * a.stride;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int e = i * 32 + lane;
+      next[i] = e < E && more ? logit_of<DT>(a.logits, next_row + e) : -INFINITY;
+    }
+    top = warp_max(top);
+    bad |= softmax && top == INFINITY;
 
-  int mine = -1;  // lane k: the k-th selected expert
-  if (!bad) {
-    bool again = false;  // f32 does not decide this row
-    if (grouped) {
+    // Scores and keys.
+    uint32_t order[NE];
+    float sum = 0.0f;
+    float error = kSigmoidError;
+    if (softmax && (biased || grouped || !a.renormalize)) {
+      const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) sum = __fadd_rn(sum, ex2(__fmul_rn(__fsub_rn(z[i], ref), kLog2e)));
+      sum = warp_sum(sum);
+      error = __fdividef(kSoftmaxError, sum);
+    }
+    __syncwarp();  // the previous row is done with the shared memory
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int e = i * 32 + lane;
+      float key = z[i];
+      if (biased || grouped) {
+        float s;
+        if (softmax) s = __fdividef(ex2(__fmul_rn(__fsub_rn(z[i], top), kLog2e)), sum);
+        else s = __fdividef(1.0f, __fadd_rn(1.0f, ex2(__fmul_rn(-z[i], kLog2e))));
+        if (biased) {
+          key = __fadd_rn(__fadd_rn(s, bias[i]), 0.0f);
+          bad |= key != key && z[i] > -INFINITY;
+        }
+        if (z[i] == -INFINITY) key = -INFINITY;
+        if (grouped && e < E) {
+          const int g = (e * a.group_inv) >> 20;
+          keys[e + g * lanes] = biased || z[i] == -INFINITY ? key : s;
+        }
+      }
+      order[i] = key == -INFINITY ? 0u : ordered(key);
+    }
+    bad = __any_sync(kAll, bad);
+
+    int mine = -1;  // lane k: the k-th selected expert
+    if (!bad && top > -INFINITY) {
+      unsigned allowed = kAll;  // bit i: this lane's expert i is in a chosen group
+      unsigned chosen = kAll;
+      double top64 = top, sum64 = 0.0;  // the softmax in 64 bits, where it is needed
+      if (grouped) {
+        __syncwarp();
+        float gap, high;
+        chosen = choose_groups<float>(keys, a, lanes, lane, &gap, &high);
+        if (!(gap > 2.0f * (a.group_top * error + 3.0f * kAddError * high))) {
+          if (softmax) sum64 = softmax_sum_in_64_bits(a.logits, DT, row, E, top64, lane);
+          chosen = groups_in_64_bits(a, row, top64, sum64, lanes, keys64, lane);
+        }
+        allowed = 0u;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+          const int g = ((i * 32 + lane) * a.group_inv) >> 20;
+          allowed |= ((chosen >> ((g * lanes) & 31)) & 1u) << i;  // (an e >= E is dead anyway)
+        }
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+          if (!((allowed >> i) & 1u)) order[i] = 0u;
+      }
+      uint32_t lane_best = 0u;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) lane_best = max(lane_best, order[i]);
+      // The candidates from `floor` on, listed in shared memory; returns how
+      // many there are (listed up to kRanked).
+      auto collect = [&](uint32_t floor, auto put) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+          const bool in = order[i] >= floor;
+          const unsigned who = __ballot_sync(kAll, in);
+          if (who != 0u) {
+            const int at = n + __popc(who & ((1u << lane) - 1u));
+            if (in && at < kRanked) put(at, i);
+            n += __popc(who);
+          }
+        }
+        __syncwarp();
+        return n;
+      };
+      // K lanes at least reach the K-th largest lane maximum.
+      const uint32_t floor = max(1u, __shfl_sync(kAll, sort_lanes(lane_best, lane), K - 1));
       __syncwarp();
-      float gap, high;
-      const unsigned chosen = choose_groups<float>(keys, a, lanes, lane, &gap, &high);
-      again = !(gap > 2.0f * (a.group_top * error + 3.0f * kAddError * high));
-#pragma unroll
-      for (int i = 0; i < NE; ++i) {
-        const int g = ((i * 32 + lane) * a.group_inv) >> 20;
-        if (!((chosen >> ((g * lanes) & 31)) & 1u)) order[i] = 0u;  // (an e >= E is dead already)
-      }
-    }
-    // The lane's two best experts after (key, e) = (lo, lo_e).
-    uint32_t b1, b2;
-    int e1, e2;
-    auto scan = [&](uint32_t lo, int lo_e) {
-      b1 = b2 = 0u;
-      e1 = e2 = 0x7fffffff;
-#pragma unroll
-      for (int i = 0; i < NE; ++i) {
-        const int e = i * 32 + lane;
-        const uint32_t k = order[i];
-        const bool after = k < lo || (k == lo && e > lo_e);
-        if (after && k > b1) {
-          b2 = b1;
-          e2 = e1;
-          b1 = k;
-          e1 = e;
-        } else if (after && k > b2) {
-          b2 = k;
-          e2 = e;
-        }
-      }
-    };
-    scan(0xffffffffu, 0x7fffffff);
-    bool two = true;
-    uint32_t key = 0u;
-    // One more than K where the border to the rest has to be looked at.
-    const int rounds = biased ? K + 1 : K;
-    uint32_t next = 0u;  // the key after the K-th
-    for (int k = 0; k < rounds; ++k) {
-      const uint32_t m = __reduce_max_sync(kAll, b1);
-      if (m == 0u) break;
-      const int e = static_cast<int>(__reduce_min_sync(kAll, b1 == m ? static_cast<unsigned>(e1) : 0x7fffffffu));
-      if (k == K) {
-        next = m;
-        if (lane == K) mine = e;  // K = 32 has no such lane: its border counts as near when its key is
-        break;
-      }
-      if (lane == k) {
-        key = m;
-        mine = e;
-      }
-      if (lane == (e & 31)) {
-        if (two) {
-          b1 = b2;
-          e1 = e2;
-          two = false;
+      int n = collect(floor, [&](int at, int i) {
+        ranked[at] = (static_cast<uint64_t>(order[i]) << 32) | static_cast<uint32_t>(~(i * 32 + lane));
+      });
+      uint32_t key = 0u, after = 0u;  // lane k: the k-th key, and the one behind it
+      int after_e = -1;
+      if (n <= kRanked) {
+        // Rank each candidate by the number of those before it.
+        const uint64_t u = lane < n ? ranked[lane] : 0ull, v = lane + 32 < n ? ranked[lane + 32] : 0ull;
+        int ru = 0, rv = 0;
+        if (n <= 32) {
+          for (int j = 0; j < n; ++j) ru += ranked[j] > u ? 1 : 0;
         } else {
-          scan(m, e);
-          two = true;
+          for (int j = 0; j < n; ++j) {
+            const uint64_t o = ranked[j];
+            ru += o > u ? 1 : 0;
+            rv += o > v ? 1 : 0;
+          }
+        }
+        __syncwarp();
+        if (lane < n) ranked[ru] = u;
+        if (lane + 32 < n) ranked[rv] = v;
+        __syncwarp();
+        if (lane < n) {
+          key = static_cast<uint32_t>(ranked[lane] >> 32);
+          mine = static_cast<int>(~static_cast<uint32_t>(ranked[lane]));
+        }
+        if (lane + 1 < n) {
+          after = static_cast<uint32_t>(ranked[lane + 1] >> 32);
+          after_e = static_cast<int>(~static_cast<uint32_t>(ranked[lane + 1]));
+        }
+        __syncwarp();
+      } else {
+        uint32_t copy[NE];
+#pragma unroll
+        for (int i = 0; i < NE; ++i) copy[i] = order[i];
+        select_by_rounds<NE>(copy, min(K + 1, 32), lane, &key, &mine);
+        after = __shfl_down_sync(kAll, key, 1);
+        after_e = __shfl_down_sync(kAll, mine, 1);
+        if (lane == 31) {  // K = 32: the key behind has no lane and counts as near
+          after = K == 32 ? key : 0u;
+          after_e = -1;
         }
       }
-    }
-    if (biased) {
-      // Neighbours in the order have to be further apart than their errors,
-      // unless they are the same logit and bias.
-      if (lane == K) key = next;
-      uint32_t after = __shfl_down_sync(kAll, key, 1);
-      const int after_e = __shfl_down_sync(kAll, mine, 1);
-      if (lane == 31) after = K == 32 ? next : 0u;
-      bool near = false;
-      if (lane < K && key != 0u && after != 0u) {
-        const float u = from_ordered(key), v = from_ordered(after);
-        near = !(__fsub_rn(u, v) > 2.0f * (error + kAddError * fmaxf(fabsf(u), fabsf(v))));
-        if (near && key == after && lane < 31)
-          near = load_logit(a.logits, row + mine, a.dtype) != load_logit(a.logits, row + after_e, a.dtype) ||
-                 a.bias[mine] != a.bias[after_e];
+      if (biased) {
+        // The best key that is no candidate stands behind the last one.
+        if (n <= kRanked && n <= K) {
+          uint32_t below = 0u;
+#pragma unroll
+          for (int i = 0; i < NE; ++i) below = max(below, order[i] < floor ? order[i] : 0u);
+          below = __reduce_max_sync(kAll, below);
+          if (lane == n - 1) after = below;
+        }
+        // Neighbours in the order have to be further apart than their errors,
+        // unless they are the same logit and bias.
+        bool near = false;
+        if (lane < K && key != 0u && after != 0u) {
+          const float u = from_ordered(key), v = from_ordered(after);
+          near = !(__fsub_rn(u, v) > 2.0f * (error + kAddError * fmaxf(fabsf(u), fabsf(v))));
+          if (near && key == after && after_e >= 0)
+            near = logit_of<DT>(a.logits, row + mine) != logit_of<DT>(a.logits, row + after_e) ||
+                   a.bias[mine] != a.bias[after_e];
+        }
+        if (__any_sync(kAll, near)) {
+          if (softmax && sum64 == 0.0) sum64 = softmax_sum_in_64_bits(a.logits, DT, row, E, top64, lane);
+          // Every expert that may be among the K best: down to the K-th key
+          // less both errors.
+          const uint32_t kth = __shfl_sync(kAll, key, K - 1);
+          uint32_t low = 1u;
+          if (kth != 0u) {
+            const float f = from_ordered(kth);
+            const float l = __fsub_rn(f, 2.5f * (error + kAddError * fabsf(f)));
+            if (l > -INFINITY) low = ordered(l);
+          }
+          __syncwarp();
+          int* id = reinterpret_cast<int*>(keys64 + kRanked);
+          n = collect(low, [&](int at, int i) { id[at] = i * 32 + lane; });
+          mine = n <= kRanked ? rank_in_64_bits(a, row, top64, sum64, n, keys64, id, lane)
+                              : select_in_64_bits(a, row, top64, sum64, chosen, lanes, keys64, lane);
+        }
       }
-      again |= __any_sync(kAll, near);
       if (lane >= K) mine = -1;
     }
-    if (again) {
-      __syncwarp();
-      mine = select_in_64_bits(a, row, lanes, keys64, lane);
+
+    // Weights of the selected experts: lane k has the k-th.
+    float w = 0.0f;
+    const bool live = mine >= 0;
+    const float zs = live ? logit_of<DT>(a.logits, row + mine) : -INFINITY;
+    // e^-ref scales numerator and denominator alike, so that scores which
+    // all underflow still have their ratios.
+    if (softmax) {
+      const float ref = a.renormalize ? warp_max(zs) : top;
+      if (live) w = expf(__fsub_rn(zs, ref));
+      if (!a.renormalize) w = __fdiv_rn(w, sum);
+    } else {
+      const float ref = a.renormalize ? fminf(warp_max(zs), 0.0f) : 0.0f;
+      if (live) w = __fdiv_rn(expf(__fsub_rn(fminf(zs, 0.0f), ref)), __fadd_rn(1.0f, expf(-fabsf(zs))));
+    }
+    if (a.renormalize) {
+      const float total = warp_sum(w);
+      w = total > 0.0f ? __fdiv_rn(w, total) : 0.0f;
+    }
+    w = live ? __fmul_rn(w, a.scale) : 0.0f;
+    if (bad) w = __uint_as_float(0x7fc00000u);
+    if (lane < K) {
+      const long long o = static_cast<long long>(t) * K + lane;
+      a.indices[o] = mine;
+      a.weights[o] = w;
+      if (a.counts != nullptr && live) atomicAdd(loads + mine, 1);
     }
   }
+  if (a.counts != nullptr) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += blockDim.x)
+      if (loads[e] != 0) atomicAdd(a.counts + e, loads[e]);
+  }
+}
 
-  // Weights of the selected experts: lane k has the k-th.
-  float w = 0.0f;
-  const bool live = mine >= 0;
-  const float zs = live ? load_logit(a.logits, row + mine, a.dtype) : -INFINITY;
-  // e^-ref scales numerator and denominator alike, so that scores which
-  // all underflow still have their ratios.
-  if (softmax) {
-    const float ref = a.renormalize ? warp_max(zs) : top;
-    if (live) w = expf(__fsub_rn(zs, ref));
-    if (!a.renormalize) w = __fdiv_rn(w, sum);
-  } else {
-    const float ref = a.renormalize ? fminf(warp_max(zs), 0.0f) : 0.0f;
-    if (live) w = __fdiv_rn(expf(__fsub_rn(fminf(zs, 0.0f), ref)), __fadd_rn(1.0f, expf(-fabsf(zs))));
-  }
-  if (a.renormalize) {
-    const float total = warp_sum(w);
-    w = total > 0.0f ? __fdiv_rn(w, total) : 0.0f;
-  }
-  w = live ? __fmul_rn(w, a.scale) : 0.0f;
-  if (bad) w = __uint_as_float(0x7fc00000u);
-  if (lane < K) {
-    const long long o = static_cast<long long>(t) * K + lane;
-    a.indices[o] = mine;
-    a.weights[o] = w;
-    if (a.counts != nullptr && live) atomicAdd(a.counts + mine, 1);
+template <int NE>
+cudaError_t launch_ne(const cudaLaunchConfig_t& cfg, const RouteScoreArgs& a) {
+  switch (a.dtype) {
+    case kBf16: return cudaLaunchKernelEx(&cfg, k_route_scores<NE, kBf16>, a);
+    case kF16: return cudaLaunchKernelEx(&cfg, k_route_scores<NE, kF16>, a);
+    default: return cudaLaunchKernelEx(&cfg, k_route_scores<NE, kF32>, a);
   }
 }
 
@@ -376,19 +540,24 @@ cudaError_t launch_route_scores(RouteScoreArgs a, cudaStream_t st) {
     if (e != cudaSuccess || a.tokens == 0) return e;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((a.tokens + kRouteWarps - 1) / kRouteWarps);
+  // Every row a warp of its own while the GPU has room for all of them
+  // (resident: 16 warps per SM), then a share of the rows each.
+  DeviceAttrs dev;
+  const cudaError_t de = current_device_attrs(&dev);
+  if (de != cudaSuccess) return de;
+  cfg.gridDim = dim3(std::min((a.tokens + kRouteWarps - 1) / kRouteWarps, dev.sms * (16 / kRouteWarps)));
   cfg.blockDim = dim3(32 * kRouteWarps);
-  cfg.dynamicSmemBytes = sizeof(double) * kRouteWarps * (a.experts + 32);
+  cfg.dynamicSmemBytes = sizeof(double) * kRouteWarps * warp_doubles(a.experts) + sizeof(int) * a.experts;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (a.experts <= 128) return cudaLaunchKernelEx(&cfg, k_route_scores<4>, a);
-  if (a.experts <= 256) return cudaLaunchKernelEx(&cfg, k_route_scores<8>, a);
-  if (a.experts <= 512) return cudaLaunchKernelEx(&cfg, k_route_scores<16>, a);
-  return cudaLaunchKernelEx(&cfg, k_route_scores<32>, a);
+  if (a.experts <= 128) return launch_ne<4>(cfg, a);
+  if (a.experts <= 256) return launch_ne<8>(cfg, a);
+  if (a.experts <= 512) return launch_ne<16>(cfg, a);
+  return launch_ne<32>(cfg, a);
 }
 
 }  // namespace fw
