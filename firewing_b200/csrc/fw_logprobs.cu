@@ -12,7 +12,7 @@
 // The reference: each warp takes the maximum of its first batch and changes
 // it only when a later value is over it by kSlack powers of two, which f32
 // sums stand without loss, so that the loop carries no maximum.
-// The alternatives: K values at least are >= `floor` (publish_floor), taken from
+// The alternatives: K values at least are >= `floor` (publish_share), taken from
 // the first batch and raised after 1, 2, 4, ... of them.  Values under it cost
 // one comparison per lane and batch; the few others go to a list in shared
 // memory.  A list that overflows (a row of equal values, an ascending row) is
@@ -36,16 +36,15 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr unsigned kAll = 0xffffffffu;
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
 constexpr int kUnroll = 4;             // 16-byte loads in flight per thread
-constexpr int kSeg = 128;              // candidates a warp holds in the fast pass
-constexpr int kList = kWarps * kSeg;   // and a CTA
-constexpr int kShare = kList / 8;      // keys a part of a split row may hand on
+constexpr int kListPerWarp = 128;      // candidates a CTA of eight warps holds in the fast pass, per warp
+constexpr int kShares = 64;            // values that make a floor
+constexpr int kSplitWarps = 8;         // warps of the CTAs that share a row
+
 constexpr int kRankMost = 384;         // candidates ranked by counting
 constexpr int kSlackLog2 = 16;         // how far over its reference (log2) a term may be
 constexpr int kMaxTop = 32;
-constexpr int kMaxSplits = 8;          // portable cluster size; kShare each fit `merged`
+constexpr int kMaxSplits = 8;          // portable cluster size
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -1.0e4f;     // floor of y: 2^y is 0, and 0 * y stays 0 for y = -inf
@@ -212,19 +211,25 @@ __device__ __forceinline__ Part join(const Part& a, const Part& b, float c) {
   return r;
 }
 
+// W warps work on a row (or a part of one).
+template <int W>
 struct __align__(16) LogprobSmem {
-  uint64_t list[kWarps][kSeg];     // each warp's candidates; all of it: the careful pass's list
-  uint64_t shortlist[kList];       // those of the CTA that reach the floor
-  uint64_t merged[kList];          // first CTA of a cluster: those of every part
+  static constexpr int kList = W == kSplitWarps ? W * kListPerWarp : 512;
+  static constexpr bool kSplit = W == kSplitWarps;
+  static constexpr int kHandOn = kList / kMaxSplits;  // keys a part of a split row may hand on
+  uint64_t list[kList];       // the warps' candidates, an equal run each; all of it: the careful pass's list
+  uint64_t shortlist[kList];  // those of the CTA that reach the floor
+  uint64_t merged[kSplit ? kList : 1];  // first CTA of a cluster: those of every part
   uint64_t best[kMaxTop];
-  uint4 lane_raw[kWarps][kUnroll];  // one lane's batch, looked at by its warp
-  Part part[kWarps];
+  uint4 lane_raw[W][kUnroll];  // one lane's batch, looked at by its warp
+  Part part[W];
   Part whole;
-  float floor[kWarps];
-  float part_floor;
-  int count;         // of list, in the careful pass
+  uint32_t share[kShares];  // maxima of the lanes' groups (publish_share)
+  uint32_t warp_top[W];     // maxima of the warps, at the end
+  float floor;
+  int count;  // of list, in the careful pass
   int short_count, merged_count;
-  int base;          // where this part's keys go in the first CTA's `merged`
+  int base;  // where this part's keys go in the first CTA's `merged`
   int found;
 };
 
@@ -252,10 +257,11 @@ __device__ __forceinline__ int best_of(const uint64_t* list, int n, int K, uint6
 // barriers of the caller; sets sm->found.  A short list is ranked at once, a
 // thread counting the keys above its own (all reads broadcasts); a long one
 // takes one warp K rounds.
-__device__ __forceinline__ void pick_best(LogprobSmem* sm, const uint64_t* list, int n, int K) {
+template <int W>
+__device__ __forceinline__ void pick_best(LogprobSmem<W>* sm, const uint64_t* list, int n, int K) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (n <= kRankMost) {
-    for (int base = warp * 32; base < n; base += kThreads) {
+    for (int base = warp * 32; base < n; base += 32 * W) {
       const int i = base + lane;
       const uint64_t key = i < n ? list[i] : 0ull;
       int above = 0;
@@ -270,32 +276,56 @@ __device__ __forceinline__ void pick_best(LogprobSmem* sm, const uint64_t* list,
   }
 }
 
-// This warp's share of a floor: the r-th largest of its lane maxima.  With
-// r = ceil(K / warps), K values at least reach the lowest share of `warps`
-// warps.  A share only grows, so one that is read late is still a floor.
-__device__ __forceinline__ void publish_floor(LogprobSmem* sm, float high, int r, int warp, int lane) {
-  uint32_t o = ordered(high), v = 0u;
-  for (int i = 0; i < r; ++i) {
-    v = __reduce_max_sync(kAll, o);
-    if (lane == __ffs(__ballot_sync(kAll, o == v)) - 1) o = 0u;
+// The K-th largest (K <= 32) of 64 values, two per lane, in every lane: a
+// bitonic sort, value i in lane i % 32.
+__device__ __forceinline__ uint32_t kth_of_64(uint32_t u, uint32_t v, int K, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 64; k <<= 1) {
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      if (j == 32) {
+        const uint32_t hi = max(u, v), lo = min(u, v);
+        u = hi;
+        v = lo;
+      } else {
+        const uint32_t ou = __shfl_xor_sync(kAll, u, j), ov = __shfl_xor_sync(kAll, v, j);
+        const bool upper = (lane & j) == 0;
+        const bool down_u = (lane & k) == 0, down_v = ((lane + 32) & k) == 0;
+        u = upper == down_u ? max(u, ou) : min(u, ou);
+        v = upper == down_v ? max(v, ov) : min(v, ov);
+      }
+    }
   }
-  if (lane == 0) *reinterpret_cast<volatile float*>(&sm->floor[warp]) = from_ordered(v);
+  return __shfl_sync(kAll, u, K - 1);
 }
-__device__ __forceinline__ float read_floor(const LogprobSmem* sm, int warps) {
-  float floor = INFINITY;
-  for (int i = 0; i < warps; ++i) floor = fminf(floor, *reinterpret_cast<const volatile float*>(&sm->floor[i]));
-  return floor;
+// This warp's shares of a floor: the maxima of 64 / W groups of its lanes.
+// The K-th largest of all 64 shares is reached by K values at least; a share
+// only grows, so that one which is read late still makes a floor.
+template <int W>
+__device__ __forceinline__ void publish_share(LogprobSmem<W>* sm, float high, int warp, int lane) {
+  constexpr int kGroup = W * 32 / kShares;
+  uint32_t o = ordered(high);
+#pragma unroll
+  for (int j = 1; j < kGroup; j <<= 1) o = max(o, __shfl_xor_sync(kAll, o, j));
+  if (lane % kGroup == 0) *reinterpret_cast<volatile uint32_t*>(&sm->share[(warp * 32 + lane) / kGroup]) = o;
+}
+template <int W>
+__device__ __forceinline__ float floor_from_shares(const LogprobSmem<W>* sm, int K, int lane) {
+  const volatile uint32_t* share = sm->share;
+  return from_ordered(kth_of_64(share[lane], share[lane + 32], K, lane));
 }
 
 // The careful pass, for row parts with a warp whose candidates overflowed its
 // list: the part [v0, v1) over again with one list, cut back to its K best
 // whenever the next round might not fit.  The K best end up in sm->best
 // (sm->found of them).  All threads.
-template <int DT>
-__device__ __noinline__ void collect_again(const LogprobArgs& a, long long row, int v0, int v1, LogprobSmem* sm) {
+template <int DT, int W>
+__device__ __noinline__ void collect_again(const LogprobArgs& a, long long row, int v0, int v1, LogprobSmem<W>* sm) {
   constexpr int kEach = 8;  // elements of a thread per step
+  constexpr int kThreads = 32 * W, kList = LogprobSmem<W>::kList;
+  static_assert(kList >= kThreads + kMaxTop, "a round fits beside the K best");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint64_t* list = &sm->list[0][0];
+  uint64_t* list = sm->list;
   __syncthreads();
   if (threadIdx.x == 0) sm->count = 0;
   uint64_t last = 0ull;  // key of the K-th best at the last cut
@@ -333,9 +363,9 @@ __device__ __noinline__ void collect_again(const LogprobArgs& a, long long row, 
     }
     // A step that ends the row may have lanes without values: no floor from it.
     const bool whole = base + kEach * kThreads <= v1;
-    if (whole) publish_floor(sm, high, (a.top_k + kWarps - 1) / kWarps, warp, lane);
+    if (whole) publish_share(sm, high, warp, lane);
     if (!__syncthreads_or(any)) continue;
-    if (whole) floor = fmaxf(floor, read_floor(sm, kWarps));
+    if (whole) floor = fmaxf(floor, floor_from_shares(sm, a.top_k, lane));
 #pragma unroll 1
     for (int i = 0; i < kEach; ++i) {
       cut_if_over(kList - kThreads);
@@ -381,10 +411,11 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   return r;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_constant__ LogprobArgs a) {
+template <int DT, int W>
+__global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_constant__ LogprobArgs a) {
   using R = Row<DT>;
-  __shared__ LogprobSmem sm;
+  constexpr int kThreads = 32 * W, kList = LogprobSmem<W>::kList;
+  __shared__ LogprobSmem<W> sm;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   pdl_wait();
   pdl_launch_dependents();
@@ -422,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
   float m = -INFINITY, limit = -INFINITY, mc = 0.0f, least = 0.0f;
   bool plain = false;
   F2 s2 = pack(0.0f, 0.0f), w2 = pack(0.0f, 0.0f);  // the lane's sums, even and odd elements
-  float seen = -INFINITY;                            // the lane's maximum so far
+  float seen = -INFINITY;  // the lane's maximum so far
   float floor = INFINITY;                            // candidates are >= floor
 
   // (S, W) against the exact reference M.
@@ -471,12 +502,16 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
     s2 = add2(s2, pack(e, 0.0f));
     w2 = fma2(pack(e, 0.0f), pack(y, 0.0f), w2);
   };
-  int held = 0;  // candidates of this warp, listed up to kSeg
+  // The warps that have vectors list their candidates in equal runs.
+  const int with = max(1, min(W, (nvec + 31) / 32));
+  const int run = kList / with;
+  uint64_t* list = sm.list + min(warp, with - 1) * run;
+  int held = 0;  // candidates of this warp, listed up to `run`
   auto offer = [&](float x, int e) {
     const bool in = x >= floor && x > -INFINITY;
     const unsigned who = __ballot_sync(kAll, in);
     const int at = held + __popc(who & ((1u << lane) - 1u));
-    if (in && at < kSeg) sm.list[warp][at] = list_key(x, e);
+    if (in && at < run) list[at] = list_key(x, e);
     held += __popc(who);
   };
 
@@ -494,7 +529,6 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
     }
   }
 
-  const int full = min(kWarps, nvec / 32);  // warps whose lanes all have values
   const uint4 dead = make_uint4(R::kDead, R::kDead, R::kDead, R::kDead);
   uint4 next[kUnroll];
   auto fetch = [&](int j0) {
@@ -510,8 +544,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
     }
   };
   fetch(0);
-  const int share = full > 0 ? (K + full - 1) / full : 0;
-  int raise_at = 1;
+  int raise_at = 1, turn = 0;
   for (int j0 = 0, batch = 1; j0 < nvec; j0 += kThreads * kUnroll, ++batch) {
     uint4 raw[kUnroll];
 #pragma unroll
@@ -521,28 +554,18 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
     cover(high);
     if (K > 0) {
       seen = fmaxf(seen, high);
-      // Raised after 1, 2, 4, ... batches, so that each stretch of the row
-      // leaves about as many candidates as the first batch.  Only the first
-      // time do the warps wait for one another's shares.
+      // The floor rises after 1, 2, 4, ... batches, so that each stretch of
+      // the row leaves about K candidates; the warps take turns at sorting.
+      // Only the first time do they wait for one another.
       if (batch == raise_at) {
-        publish_floor(&sm, seen, share, warp, lane);
+        publish_share(&sm, seen, warp, lane);
         if (batch == 1) __syncthreads();
         else __syncwarp();
-        floor = full > 0 ? read_floor(&sm, full) : -INFINITY;
-        raise_at *= 2;
-      }
-      // A lane that has a candidate shows its batch to the warp, an element
-      // for each lane.
-      for (unsigned who = __ballot_sync(kAll, high >= floor); who != 0u; who &= who - 1u) {
-        const int src = __ffs(who) - 1;
-        __syncwarp();
-        if (lane == src) {
-#pragma unroll
-          for (int u = 0; u < kUnroll; ++u) sm.lane_raw[warp][u] = raw[u];
+        if (warp == turn % W) {
+          const float f = floor_from_shares(&sm, K, lane);
+          if (lane == 0) *reinterpret_cast<volatile float*>(&sm.floor) = f;
         }
-        __syncwarp();
-        const float x = lane < kUnroll * R::N ? R::one(sm.lane_raw[warp], lane) : -INFINITY;
-        offer(x, first + (j0 + lane / R::N * kThreads + warp * 32 + src) * R::N + lane % R::N);
+        turn += 3;
       }
     }
     if (!plain && m > -INFINITY) {
@@ -566,6 +589,26 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
         for (int i = 0; i < R::N; ++i) add_plain(x[i]);
       }
     }
+    if (K > 0) {
+      if (batch == raise_at) {
+        if (batch == 1) __syncthreads();
+        raise_at *= 2;
+      }
+      floor = *reinterpret_cast<const volatile float*>(&sm.floor);
+      // A lane that has a candidate shows its batch to the warp, an element
+      // for each lane.
+      for (unsigned who = __ballot_sync(kAll, high >= floor); who != 0u; who &= who - 1u) {
+        const int src = __ffs(who) - 1;
+        __syncwarp();
+        if (lane == src) {
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u) sm.lane_raw[warp][u] = raw[u];
+        }
+        __syncwarp();
+        const float x = lane < kUnroll * R::N ? R::one(sm.lane_raw[warp], lane) : -INFINITY;
+        offer(x, first + (j0 + lane / R::N * kThreads + warp * 32 + src) * R::N + lane % R::N);
+      }
+    }
   }
   if (K > 0 && warp == 0) {
     if (nvec == 0) floor = -INFINITY;
@@ -583,8 +626,11 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
   acc.s = warp_sum(__fadd_rn(s_even, s_odd));
   acc.w = warp_sum(__fadd_rn(w_even, w_odd));
   if (lane == 0) sm.part[warp] = acc;
-  if (K > 0) publish_floor(&sm, seen, share, warp, lane);
-  const bool over = __syncthreads_or(held > kSeg);
+  if (K > 0 && LogprobSmem<W>::kSplit && a.splits > 1) {
+    const uint32_t top = __reduce_max_sync(kAll, ordered(seen));
+    if (lane == 0) sm.warp_top[warp] = top;
+  }
+  const bool over = __syncthreads_or(held > run);
   const Part none = {-INFINITY, 0.0f, 0.0f};
   // parts[0..n) joined in a fixed order by one warp (n <= 8)
   auto join_all = [&](Part p) {
@@ -598,30 +644,36 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
     }
     return p;
   };
-  if (warp == kWarps - 1) {
-    const Part whole = join_all(lane < kWarps ? sm.part[lane] : none);
+  if (warp == W - 1) {
+    const Part whole = join_all(lane < W ? sm.part[lane] : none);
     if (lane == 0) sm.whole = whole;
   }
   cg::cluster_group cluster = cg::this_cluster();
-  const bool split = a.splits > 1;
+  const bool split = LogprobSmem<W>::kSplit && a.splits > 1;
   if (K > 0) {
+    if (nvec > 0) floor = *reinterpret_cast<const volatile float*>(&sm.floor);
     if (over) {
-      collect_again<DT>(a, row, v0, v1, &sm);
+      collect_again<DT, W>(a, row, v0, v1, &sm);
       const int found = sm.found;
-      floor = found == K ? from_ordered(static_cast<uint32_t>(sm.best[K - 1] >> 32)) : -INFINITY;
       held = warp == 0 ? found : 0;
-      if (warp == 0 && lane < found) sm.list[0][lane] = sm.best[lane];
+      if (warp == 0 && lane < found) sm.list[lane] = sm.best[lane];
       __syncwarp();
-    } else {
-      floor = full > 0 ? read_floor(&sm, full) : -INFINITY;
     }
   }
   if (split) {
-    if (tid == 0) sm.part_floor = floor;
     cluster.sync();
-    if (K > 0)  // K values of the row reach the best part's floor
-      floor = warp_max(lane < a.splits ? cluster.map_shared_rank(&sm, lane)->part_floor : -INFINITY);
-    if (part == 0 && warp == kWarps - 1) {
+    if (K > 0) {
+      // The K-th largest of all parts' warp maxima (64 at most).
+      uint32_t v[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = (lane + 32 * i) / W;
+        v[i] = r < a.splits ? cluster.map_shared_rank(&sm, r)->warp_top[lane % W] : 0u;
+      }
+      const uint32_t kth = kth_of_64(v[0], v[1], K, lane);
+      if (kth != 0u) floor = fmaxf(floor, from_ordered(kth));
+    }
+    if (part == 0 && warp == W - 1) {
       const Part whole = join_all(lane < a.splits ? cluster.map_shared_rank(&sm, lane)->whole : none);
       __syncwarp();
       if (lane == 0) sm.whole = whole;
@@ -631,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
     // This part's candidates that reach the floor.
     const uint64_t least_key = static_cast<uint64_t>(ordered(__fadd_rn(floor, 0.0f))) << 32;
     for (int i = lane; i - lane < held; i += 32) {
-      const uint64_t key = i < held ? sm.list[warp][i] : 0ull;
+      const uint64_t key = i < held ? list[i] : 0ull;
       const bool in = key != 0ull && key >= least_key;
       const unsigned who = __ballot_sync(kAll, in);
       if (who == 0u) continue;
@@ -644,14 +696,14 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
     int n = sm.short_count;
     const uint64_t* keys = sm.shortlist;
     if (split) {
-      // All parts' keys to the first CTA, no more than kShare from each.
-      if (n > kShare) {
+      // All parts' keys to the first CTA, no more than kHandOn from each.
+      if (n > LogprobSmem<W>::kHandOn) {
         pick_best(&sm, keys, n, K);
         __syncthreads();
         keys = sm.best;
         n = sm.found;
       }
-      LogprobSmem* to = cluster.map_shared_rank(&sm, 0);
+      LogprobSmem<W>* to = cluster.map_shared_rank(&sm, 0);
       if (tid == 0) sm.base = n > 0 ? atomicAdd(&to->merged_count, n) : 0;
       __syncthreads();
       if (tid < n) to->merged[sm.base + tid] = keys[tid];
@@ -698,6 +750,14 @@ __global__ void __launch_bounds__(kThreads, 3) k_token_logprobs(const __grid_con
   }
 }
 
+constexpr int kNarrowWarps = 2;
+
+template <int DT>
+cudaError_t launch_width(const cudaLaunchConfig_t& cfg, const LogprobArgs& a, bool narrow) {
+  return narrow ? cudaLaunchKernelEx(&cfg, k_token_logprobs<DT, kNarrowWarps>, a)
+                : cudaLaunchKernelEx(&cfg, k_token_logprobs<DT, kSplitWarps>, a);
+}
+
 }  // namespace
 
 cudaError_t launch_token_logprobs(LogprobArgs a, cudaStream_t st) {
@@ -707,14 +767,21 @@ cudaError_t launch_token_logprobs(LogprobArgs a, cudaStream_t st) {
   a.scale = kLog2e * a.inv_temperature;
   a.slack = static_cast<float>(kSlackLog2) / a.scale;
   a.depth = 20000.0f / a.scale;
-  // Few rows: as many parts as the GPU has room for at once (three CTAs per
-  // SM), of 4096 values at least.
+  // Few rows: as many parts as the GPU has room for at once (three CTAs of
+  // eight warps per SM), of 4096 values at least.
+  // Short rows, and many rows of middling length, get two warps each, so that
+  // more rows are under way and one's beginning and end hide behind others;
+  // long rows keep eight, or too few CTAs would share the end of a launch.
+  // Measured with five alternatives, eight against two warps: 4096 x 2000
+  // bf16 55 and 19 us, 4096 x 32000 93 and 70 us, 600 x 32000 20.0 and 21.5
+  // us, 2048 x 131072 111 and 123 us.
   const int splits = std::max(1, std::min({kMaxSplits, 3 * dev.sms / a.tokens, a.vocab / 4096}));
   a.splits = splits;
   a.part_len = ((a.vocab + splits - 1) / splits + 7) & ~7;
+  const bool narrow = splits == 1 && (a.vocab <= 8192 || (a.vocab <= 65536 && a.tokens >= 12 * dev.sms));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.tokens) * splits);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(32 * (narrow ? kNarrowWarps : kSplitWarps));
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -726,9 +793,9 @@ cudaError_t launch_token_logprobs(LogprobArgs a, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = splits > 1 ? 2 : 1;
   switch (a.dtype) {
-    case kBf16: return cudaLaunchKernelEx(&cfg, k_token_logprobs<kBf16>, a);
-    case kF16: return cudaLaunchKernelEx(&cfg, k_token_logprobs<kF16>, a);
-    default: return cudaLaunchKernelEx(&cfg, k_token_logprobs<kF32>, a);
+    case kBf16: return launch_width<kBf16>(cfg, a, narrow);
+    case kF16: return launch_width<kF16>(cfg, a, narrow);
+    default: return launch_width<kF32>(cfg, a, narrow);
   }
 }
 
