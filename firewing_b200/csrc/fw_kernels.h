@@ -412,7 +412,7 @@ struct RouteScoreArgs {
   int tokens, experts, top_k, dtype, scoring;
   int groups, top_groups, group_top, renormalize;
   float scale;
-  int lanes, group_size, group_inv;  // set by launch_route_scores
+  int lanes, group_size, group_inv, run_shift;  // set by launch_route_scores
 };
 cudaError_t launch_route_scores(RouteScoreArgs a, cudaStream_t st);
 

@@ -26,8 +26,10 @@
 namespace fw {
 namespace {
 
-constexpr int kRouteWarps = 4;  // tokens per CTA
+constexpr int kRouteWarps = 4;     // tokens per CTA
+constexpr int kRouteResident = 4;  // CTAs per SM (half as many with more than 512 experts)
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.402823466e38f;  // below it a key is dead
 constexpr unsigned kAll = 0xffffffffu;
 
 // Bounds of the f32 scores' errors.  z * log2(e) is off by 2^-23.4 |z log2 e|,
@@ -67,8 +69,16 @@ __device__ __forceinline__ float logit_of(const void* p, long long i) {
   return DT == kBf16 ? bf16_to_f32(v) : __half2float(__ushort_as_half(v));
 }
 
+// Maximum over the warp; a NaN loses.
 __device__ __forceinline__ float warp_max(float v) {
-  return from_ordered(__reduce_max_sync(kAll, ordered(v)));
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 template <typename T>
 __device__ __forceinline__ T warp_sum(T v) {
@@ -77,12 +87,38 @@ __device__ __forceinline__ T warp_sum(T v) {
   return v;
 }
 
-// The groups that may be chosen from, as a mask with bit g * lanes set, from
-// the keys in `keys` (group g at g * (size + lanes), dead experts -inf).
-// 32 / bit_ceil(G) lanes read each group; the padding by `lanes` keeps
-// their reads on distinct banks.  *gap: the lowest chosen group's score
-// minus the highest other one's (+inf when there is none), *high the
-// largest magnitude of the scores compared.
+// The groups to choose from, as a mask with bit g * lanes set, from the
+// groups' scores (group g's in lane g * lanes).  *gap: the lowest chosen
+// group's score minus the highest other one's (+inf when there is none),
+// *high the largest magnitude of the scores compared.
+template <typename F>
+__device__ __forceinline__ unsigned rank_groups(F score, const RouteScoreArgs& a, int lanes, int lane, F* gap,
+                                                F* high) {
+  const F none = static_cast<F>(-INFINITY);
+  const int g = lane / lanes;
+  const bool owner = g < a.groups && lane == g * lanes;
+  int before = 0;  // groups that come first
+  for (int h = 0; h < a.groups; ++h) {
+    const F v = __shfl_sync(kAll, score, h * lanes);
+    before += (v > score || (v == score && h < g)) ? 1 : 0;
+  }
+  const bool chosen = owner && before < a.top_groups;
+  F low = chosen ? score : static_cast<F>(INFINITY);
+  F other = owner && !chosen ? score : none;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    low = fmin(low, __shfl_xor_sync(kAll, low, o));
+    other = fmax(other, __shfl_xor_sync(kAll, other, o));
+  }
+  const bool border = other > none;
+  *gap = border ? low - other : static_cast<F>(INFINITY);
+  *high = border ? fmax(fabs(low), fabs(other)) : static_cast<F>(0);
+  return __ballot_sync(kAll, chosen);
+}
+
+// The same from the keys in `keys` (group g at g * (size + lanes), dead experts
+// -inf).  32 / bit_ceil(G) lanes read each group; the padding by `lanes` keeps
+// their reads on distinct banks.
 template <typename F>
 __device__ __forceinline__ unsigned choose_groups(const F* keys, const RouteScoreArgs& a, int lanes, int lane,
                                                   F* gap, F* high) {
@@ -101,23 +137,7 @@ __device__ __forceinline__ unsigned choose_groups(const F* keys, const RouteScor
     m1 = fmax(m1, o1);
   }
   const F score = (a.group_top == 2 && m2 > none) ? m1 + m2 : m1;
-  int before = 0;  // groups that come first
-  for (int h = 0; h < a.groups; ++h) {
-    const F v = __shfl_sync(kAll, score, h * lanes);
-    before += (v > score || (v == score && h < g)) ? 1 : 0;
-  }
-  const bool chosen = g < a.groups && before < a.top_groups;
-  F low = chosen ? score : static_cast<F>(INFINITY);
-  F other = (g < a.groups && !chosen) ? score : none;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    low = fmin(low, __shfl_xor_sync(kAll, low, o));
-    other = fmax(other, __shfl_xor_sync(kAll, other, o));
-  }
-  const bool border = other > none;
-  *gap = border ? low - other : static_cast<F>(INFINITY);
-  *high = border ? fmax(fabs(low), fabs(other)) : static_cast<F>(0);
-  return __ballot_sync(kAll, chosen && l == 0);
+  return rank_groups<F>(g < a.groups && l == 0 ? score : none, a, lanes, lane, gap, high);
 }
 
 // Score (and bias) of a logit in 64 bits; top and sum are the softmax's.
@@ -214,42 +234,42 @@ __device__ __noinline__ int rank_in_64_bits(const RouteScoreArgs& a, long long r
   return mine;
 }
 
-// Lane maxima sorted over the warp, descending: lane k returns the k-th.
-__device__ __forceinline__ uint32_t sort_lanes(uint32_t v, int lane) {
+// Values sorted over the warp, descending: lane k returns the k-th.
+__device__ __forceinline__ float sort_lanes(float v, int lane) {
 #pragma unroll
   for (int k = 2; k <= 32; k <<= 1) {
 #pragma unroll
     for (int j = k >> 1; j > 0; j >>= 1) {
-      const uint32_t o = __shfl_xor_sync(kAll, v, j);
+      const float o = __shfl_xor_sync(kAll, v, j);
       const bool keep_max = ((lane & k) == 0) == ((lane & j) == 0);
-      v = keep_max ? max(v, o) : min(v, o);
+      v = keep_max ? fmaxf(v, o) : fminf(v, o);
     }
   }
   return v;
 }
 
-// The first `rounds` experts in the order of `order` (0: dead) by repeated
+// The first `rounds` experts in the order of `keys` (-inf: dead) by repeated
 // maxima: lane k gets the k-th one's key and id (id -1 when there is none).
 // For the rows whose candidates do not fit the ranking.
 template <int NE>
-__device__ __noinline__ void select_by_rounds(const uint32_t* order_in, int rounds, int lane, uint32_t* key, int* id) {
-  uint32_t last = 0xffffffffu;
-  int last_e = 0x7fffffff;
-  *key = 0u;
+__device__ __noinline__ void select_by_rounds(const float* keys, int rounds, int lane, float* key, int* id) {
+  float last = INFINITY;
+  int last_e = -1;
+  *key = -INFINITY;
   *id = -1;
   for (int k = 0; k < rounds; ++k) {
-    uint32_t b = 0u;
+    float b = -INFINITY;
     int be = 0x7fffffff;
     for (int i = 0; i < NE; ++i) {
       const int e = i * 32 + lane;
-      const uint32_t v = order_in[i];
+      const float v = keys[i];
       if ((v < last || (v == last && e > last_e)) && v > b) {
         b = v;
         be = e;
       }
     }
-    const uint32_t m = __reduce_max_sync(kAll, b);
-    if (m == 0u) break;
+    const float m = warp_max(b);
+    if (m == -INFINITY) break;
     const int e = static_cast<int>(__reduce_min_sync(kAll, b == m ? static_cast<unsigned>(be) : 0x7fffffffu));
     if (lane == k) {
       *key = m;
@@ -270,12 +290,15 @@ __host__ __device__ inline int warp_doubles(int experts) {
 
 // NE experts per lane (E <= 32 * NE), logits of type DT.  A warp takes the
 // rows warp, warp + warps, ...; the next row's logits are on their way while
-// one is routed.
-template <int NE, int DT>
-__global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? 4 : 2) k_route_scores(const __grid_constant__ RouteScoreArgs a) {
+// one is routed.  EVEN: E = 32 * NE and the groups, if any, are made of whole
+// runs of 32 experts, so that a lane has as many of each: their scores then
+// take two reductions each and no shared memory.
+template <int NE, int DT, bool EVEN>
+__global__ void __launch_bounds__(32 * kRouteWarps, kRouteResident / (NE <= 16 ? 1 : 2))
+    k_route_scores(const __grid_constant__ RouteScoreArgs a) {
   extern __shared__ __align__(16) unsigned char route_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int E = a.experts, K = a.top_k;
+  const int E = EVEN ? 32 * NE : a.experts, K = a.top_k;
   double* keys64 = reinterpret_cast<double*>(route_smem) + static_cast<size_t>(warp) * warp_doubles(E);
   float* keys = reinterpret_cast<float*>(keys64);
   uint64_t* ranked = reinterpret_cast<uint64_t*>(keys64);
@@ -284,6 +307,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? 4 : 2) k_route_sc
   const bool biased = a.bias != nullptr;
   const bool grouped = a.groups > 1;
   const int lanes = a.lanes;
+  const int shift = EVEN ? a.run_shift : 0;  // log2 of a group's runs of 32 experts
   const int first = blockIdx.x * kRouteWarps + warp, step = gridDim.x * kRouteWarps;
   if (a.counts != nullptr) {
     for (int e = threadIdx.x; e < E; e += blockDim.x) loads[e] = 0;
@@ -296,9 +320,13 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? 4 : 2) k_route_sc
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int e = i * 32 + lane;
-    next[i] = e < E && first < a.tokens ? logit_of<DT>(a.logits, first * a.stride + e) : -INFINITY;
-    bias[i] = biased && e < E ? a.bias[e] : 0.0f;
+    next[i] = (EVEN || e < E) && first < a.tokens ? logit_of<DT>(a.logits, first * a.stride + e) : -INFINITY;
+    bias[i] = biased && (EVEN || e < E) ? a.bias[e] : 0.0f;
   }
+  bool nan_bias = false;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) nan_bias |= bias[i] != bias[i];
+  nan_bias = __any_sync(kAll, nan_bias);
 
   for (int t = first; t < a.tokens; t += step) {
     const long long row = t * a.stride;
@@ -311,106 +339,147 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? 4 : 2) k_route_sc
       z[i] = __fadd_rn(next[i], 0.0f);  // -0 and +0 are one value
       top = fmaxf(top, z[i]);
     }
-    const bool more = t + step < a.tokens;
-    const long long next_row = (t + static_cast<long long>(step)) * a.stride;
+    if (t + step < a.tokens) {
+      const long long next_row = (t + static_cast<long long>(step)) * a.stride + lane;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int e = i * 32 + lane;
-      next[i] = e < E && more ? logit_of<DT>(a.logits, next_row + e) : -INFINITY;
+      for (int i = 0; i < NE; ++i)
+        if (EVEN || i * 32 + lane < E) next[i] = logit_of<DT>(a.logits, next_row + i * 32);
     }
     top = warp_max(top);
     bad |= softmax && top == INFINITY;
 
-    // Scores and keys.
-    uint32_t order[NE];
-    float sum = 0.0f;
+    // Scores and keys (-inf: out of the question).
+    float key[NE];
+    float sum = 0.0f, inv_sum = 0.0f;
     float error = kSigmoidError;
+    const float ref = top == -INFINITY ? 0.0f : top;
     if (softmax && (biased || grouped || !a.renormalize)) {
-      const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
       for (int i = 0; i < NE; ++i) sum = __fadd_rn(sum, ex2(__fmul_rn(__fsub_rn(z[i], ref), kLog2e)));
       sum = warp_sum(sum);
-      error = __fdividef(kSoftmaxError, sum);
+      inv_sum = rcp(sum);
+      error = __fmul_rn(kSoftmaxError, inv_sum);
     }
     __syncwarp();  // the previous row is done with the shared memory
+    float score = -INFINITY;            // EVEN: lane g's is group g's
+    float m1 = -INFINITY, m2 = -INFINITY;  // the lane's two largest of the group being passed
+    if (biased || grouped) {
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int e = i * 32 + lane;
-      float key = z[i];
-      if (biased || grouped) {
+      for (int i = 0; i < NE; ++i) {
         float s;
-        if (softmax) s = __fdividef(ex2(__fmul_rn(__fsub_rn(z[i], top), kLog2e)), sum);
-        else s = __fdividef(1.0f, __fadd_rn(1.0f, ex2(__fmul_rn(-z[i], kLog2e))));
+        if (softmax) s = __fmul_rn(ex2(__fmul_rn(__fsub_rn(z[i], ref), kLog2e)), inv_sum);
+        else s = rcp(__fadd_rn(1.0f, ex2(__fmul_rn(z[i], -kLog2e))));
+        float k = s;
         if (biased) {
-          key = __fadd_rn(__fadd_rn(s, bias[i]), 0.0f);
-          bad |= key != key && z[i] > -INFINITY;
+          k = __fadd_rn(__fadd_rn(s, bias[i]), 0.0f);
+          if (nan_bias) bad |= k != k && z[i] > -INFINITY;
         }
-        if (z[i] == -INFINITY) key = -INFINITY;
-        if (grouped && e < E) {
-          const int g = (e * a.group_inv) >> 20;
-          keys[e + g * lanes] = biased || z[i] == -INFINITY ? key : s;
+        if (z[i] == -INFINITY) k = -INFINITY;
+        key[i] = biased ? k : z[i];
+        if (grouped) {
+          if (EVEN) {
+            m2 = fmaxf(m2, fminf(m1, k));
+            m1 = fmaxf(m1, k);
+            if ((((i + 1) >> shift) << shift) == i + 1) {
+              const float best = warp_max(m1);
+              float value = best;
+              if (a.group_top == 2) {
+                const unsigned who = __ballot_sync(kAll, m1 == best);
+                const float second = warp_max(lane == __ffs(who) - 1 ? m2 : m1);
+                if (second > -INFINITY) value = __fadd_rn(best, second);
+              }
+              if (lane == i >> shift) score = value;
+              m1 = m2 = -INFINITY;
+            }
+          } else if (i * 32 + lane < E) {
+            const int e = i * 32 + lane;
+            keys[e + ((e * a.group_inv) >> 20) * lanes] = k;
+          }
         }
       }
-      order[i] = key == -INFINITY ? 0u : ordered(key);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NE; ++i) key[i] = z[i];
     }
     bad = __any_sync(kAll, bad);
 
     int mine = -1;  // lane k: the k-th selected expert
     if (!bad && top > -INFINITY) {
-      unsigned allowed = kAll;  // bit i: this lane's expert i is in a chosen group
-      unsigned chosen = kAll;
+      unsigned chosen = kAll;           // bit g * lanes (bit g where `narrow`): group g stays
+      bool narrow = false;
       double top64 = top, sum64 = 0.0;  // the softmax in 64 bits, where it is needed
       if (grouped) {
         __syncwarp();
         float gap, high;
-        chosen = choose_groups<float>(keys, a, lanes, lane, &gap, &high);
+        int spread = lanes;
+        if (EVEN) {
+          chosen = rank_groups<float>(score, a, 1, lane, &gap, &high);
+          spread = 1;  // (widened where the 64-bit functions need it)
+        } else {
+          chosen = choose_groups<float>(keys, a, lanes, lane, &gap, &high);
+        }
         if (!(gap > 2.0f * (a.group_top * error + 3.0f * kAddError * high))) {
           if (softmax) sum64 = softmax_sum_in_64_bits(a.logits, DT, row, E, top64, lane);
           chosen = groups_in_64_bits(a, row, top64, sum64, lanes, keys64, lane);
+          spread = lanes;
         }
-        allowed = 0u;
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
-          const int g = ((i * 32 + lane) * a.group_inv) >> 20;
-          allowed |= ((chosen >> ((g * lanes) & 31)) & 1u) << i;  // (an e >= E is dead anyway)
+          const int g = EVEN ? i >> shift : ((i * 32 + lane) * a.group_inv) >> 20;
+          if (!((chosen >> ((g * spread) & 31)) & 1u)) key[i] = -INFINITY;  // (an e >= E is dead already)
         }
+        narrow = spread != lanes;
+      }
+      float lane_best = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) lane_best = fmaxf(lane_best, key[i]);
+      // K lanes at least reach the K-th largest lane maximum: candidates are
+      // the keys from there on.
+      float floor;
+      if (K <= 16) {
+        floor = lane_best;
+        for (int k = 1;; ++k) {
+          const float best = warp_max(floor);
+          if (k == K) {
+            floor = best;
+            break;
+          }
+          if (floor == best) floor = -INFINITY;  // (equal maxima go together: the floor is lower then)
+        }
+      } else {
+        floor = __shfl_sync(kAll, sort_lanes(lane_best, lane), K - 1);
+      }
+      floor = fmaxf(floor, kLowest);
+      // How many candidates the lane has from `from` on, and where they go.
+      auto place = [&](float from, int* n) {
+        int mine_here = 0;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) mine_here += key[i] >= from ? 1 : 0;
+        int before = mine_here;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(kAll, before, o);
+          if (lane >= o) before += v;
+        }
+        *n = __shfl_sync(kAll, before, 31);
+        return before - mine_here;
+      };
+      int n;
+      int at = place(floor, &n);
+      float my_key = -INFINITY, after = -INFINITY;  // lane k: the k-th key, and the one behind it
+      int after_e = -1;
+      __syncwarp();
+      if (n <= kRanked) {
 #pragma unroll
         for (int i = 0; i < NE; ++i)
-          if (!((allowed >> i) & 1u)) order[i] = 0u;
-      }
-      uint32_t lane_best = 0u;
-#pragma unroll
-      for (int i = 0; i < NE; ++i) lane_best = max(lane_best, order[i]);
-      // The candidates from `floor` on, listed in shared memory; returns how
-      // many there are (listed up to kRanked).
-      auto collect = [&](uint32_t floor, auto put) {
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < NE; ++i) {
-          const bool in = order[i] >= floor;
-          const unsigned who = __ballot_sync(kAll, in);
-          if (who != 0u) {
-            const int at = n + __popc(who & ((1u << lane) - 1u));
-            if (in && at < kRanked) put(at, i);
-            n += __popc(who);
-          }
-        }
+          if (key[i] >= floor)
+            ranked[at++] = (static_cast<uint64_t>(ordered(key[i])) << 32) | static_cast<uint32_t>(~(i * 32 + lane));
         __syncwarp();
-        return n;
-      };
-      // K lanes at least reach the K-th largest lane maximum.
-      const uint32_t floor = max(1u, __shfl_sync(kAll, sort_lanes(lane_best, lane), K - 1));
-      __syncwarp();
-      int n = collect(floor, [&](int at, int i) {
-        ranked[at] = (static_cast<uint64_t>(order[i]) << 32) | static_cast<uint32_t>(~(i * 32 + lane));
-      });
-      uint32_t key = 0u, after = 0u;  // lane k: the k-th key, and the one behind it
-      int after_e = -1;
-      if (n <= kRanked) {
         // Rank each candidate by the number of those before it.
         const uint64_t u = lane < n ? ranked[lane] : 0ull, v = lane + 32 < n ? ranked[lane + 32] : 0ull;
         int ru = 0, rv = 0;
         if (n <= 32) {
+#pragma unroll 4
           for (int j = 0; j < n; ++j) ru += ranked[j] > u ? 1 : 0;
         } else {
           for (int j = 0; j < n; ++j) {
@@ -424,42 +493,41 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? 4 : 2) k_route_sc
         if (lane + 32 < n) ranked[rv] = v;
         __syncwarp();
         if (lane < n) {
-          key = static_cast<uint32_t>(ranked[lane] >> 32);
+          my_key = from_ordered(static_cast<uint32_t>(ranked[lane] >> 32));
           mine = static_cast<int>(~static_cast<uint32_t>(ranked[lane]));
         }
         if (lane + 1 < n) {
-          after = static_cast<uint32_t>(ranked[lane + 1] >> 32);
+          after = from_ordered(static_cast<uint32_t>(ranked[lane + 1] >> 32));
           after_e = static_cast<int>(~static_cast<uint32_t>(ranked[lane + 1]));
         }
         __syncwarp();
       } else {
-        uint32_t copy[NE];
+        float copy[NE];
 #pragma unroll
-        for (int i = 0; i < NE; ++i) copy[i] = order[i];
-        select_by_rounds<NE>(copy, min(K + 1, 32), lane, &key, &mine);
-        after = __shfl_down_sync(kAll, key, 1);
+        for (int i = 0; i < NE; ++i) copy[i] = key[i];
+        select_by_rounds<NE>(copy, min(K + 1, 32), lane, &my_key, &mine);
+        after = __shfl_down_sync(kAll, my_key, 1);
         after_e = __shfl_down_sync(kAll, mine, 1);
         if (lane == 31) {  // K = 32: the key behind has no lane and counts as near
-          after = K == 32 ? key : 0u;
+          after = K == 32 ? my_key : -INFINITY;
           after_e = -1;
         }
       }
       if (biased) {
         // The best key that is no candidate stands behind the last one.
-        if (n <= kRanked && n <= K) {
-          uint32_t below = 0u;
+        if (n <= K) {
+          float below = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < NE; ++i) below = max(below, order[i] < floor ? order[i] : 0u);
-          below = __reduce_max_sync(kAll, below);
+          for (int i = 0; i < NE; ++i) below = fmaxf(below, key[i] < floor ? key[i] : -INFINITY);
+          below = warp_max(below);
           if (lane == n - 1) after = below;
         }
         // Neighbours in the order have to be further apart than their errors,
         // unless they are the same logit and bias.
         bool near = false;
-        if (lane < K && key != 0u && after != 0u) {
-          const float u = from_ordered(key), v = from_ordered(after);
-          near = !(__fsub_rn(u, v) > 2.0f * (error + kAddError * fmaxf(fabsf(u), fabsf(v))));
-          if (near && key == after && after_e >= 0)
+        if (lane < K && after > -INFINITY) {
+          near = !(__fsub_rn(my_key, after) > 2.0f * (error + kAddError * fmaxf(fabsf(my_key), fabsf(after))));
+          if (near && my_key == after && after_e >= 0)
             near = logit_of<DT>(a.logits, row + mine) != logit_of<DT>(a.logits, row + after_e) ||
                    a.bias[mine] != a.bias[after_e];
         }
@@ -467,18 +535,26 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? 4 : 2) k_route_sc
           if (softmax && sum64 == 0.0) sum64 = softmax_sum_in_64_bits(a.logits, DT, row, E, top64, lane);
           // Every expert that may be among the K best: down to the K-th key
           // less both errors.
-          const uint32_t kth = __shfl_sync(kAll, key, K - 1);
-          uint32_t low = 1u;
-          if (kth != 0u) {
-            const float f = from_ordered(kth);
-            const float l = __fsub_rn(f, 2.5f * (error + kAddError * fabsf(f)));
-            if (l > -INFINITY) low = ordered(l);
-          }
+          const float kth = __shfl_sync(kAll, my_key, K - 1);
+          const float low = __fsub_rn(kth, 2.5f * (error + kAddError * fabsf(kth)));
+          const float from = fmaxf(low, kLowest);  // (no K-th key: everything)
           __syncwarp();
           int* id = reinterpret_cast<int*>(keys64 + kRanked);
-          n = collect(low, [&](int at, int i) { id[at] = i * 32 + lane; });
-          mine = n <= kRanked ? rank_in_64_bits(a, row, top64, sum64, n, keys64, id, lane)
-                              : select_in_64_bits(a, row, top64, sum64, chosen, lanes, keys64, lane);
+          at = place(from, &n);
+          if (n <= kRanked) {
+#pragma unroll
+            for (int i = 0; i < NE; ++i)
+              if (key[i] >= from) id[at++] = i * 32 + lane;
+            __syncwarp();
+            mine = rank_in_64_bits(a, row, top64, sum64, n, keys64, id, lane);
+          } else {
+            if (narrow) {
+              unsigned wide = 0u;
+              for (int g = 0; g < a.groups; ++g) wide |= ((chosen >> g) & 1u) << (g * lanes);
+              chosen = wide;
+            }
+            mine = select_in_64_bits(a, row, top64, sum64, chosen, lanes, keys64, lane);
+          }
         }
       }
       if (lane >= K) mine = -1;
@@ -491,16 +567,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? 4 : 2) k_route_sc
     // e^-ref scales numerator and denominator alike, so that scores which
     // all underflow still have their ratios.
     if (softmax) {
-      const float ref = a.renormalize ? warp_max(zs) : top;
-      if (live) w = expf(__fsub_rn(zs, ref));
-      if (!a.renormalize) w = __fdiv_rn(w, sum);
+      const float high = a.renormalize ? warp_max(zs) : top;
+      if (live) w = expf(__fsub_rn(zs, high));
+      if (!a.renormalize) w = __fdividef(w, sum);
     } else {
-      const float ref = a.renormalize ? fminf(warp_max(zs), 0.0f) : 0.0f;
-      if (live) w = __fdiv_rn(expf(__fsub_rn(fminf(zs, 0.0f), ref)), __fadd_rn(1.0f, expf(-fabsf(zs))));
+      const float high = a.renormalize ? fminf(warp_max(zs), 0.0f) : 0.0f;
+      if (live) w = __fdividef(expf(__fsub_rn(fminf(zs, 0.0f), high)), __fadd_rn(1.0f, expf(-fabsf(zs))));
     }
     if (a.renormalize) {
       const float total = warp_sum(w);
-      w = total > 0.0f ? __fdiv_rn(w, total) : 0.0f;
+      w = total > 0.0f ? __fdividef(w, total) : 0.0f;
     }
     w = live ? __fmul_rn(w, a.scale) : 0.0f;
     if (bad) w = __uint_as_float(0x7fc00000u);
@@ -518,13 +594,24 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? 4 : 2) k_route_sc
   }
 }
 
+__global__ void k_clear_counts(int32_t* counts, int experts) {
+  pdl_wait();
+  pdl_launch_dependents();
+  for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[e] = 0;
+}
+
+template <int NE, bool EVEN>
+cudaError_t launch_even(const cudaLaunchConfig_t& cfg, const RouteScoreArgs& a) {
+  switch (a.dtype) {
+    case kBf16: return cudaLaunchKernelEx(&cfg, k_route_scores<NE, kBf16, EVEN>, a);
+    case kF16: return cudaLaunchKernelEx(&cfg, k_route_scores<NE, kF16, EVEN>, a);
+    default: return cudaLaunchKernelEx(&cfg, k_route_scores<NE, kF32, EVEN>, a);
+  }
+}
 template <int NE>
 cudaError_t launch_ne(const cudaLaunchConfig_t& cfg, const RouteScoreArgs& a) {
-  switch (a.dtype) {
-    case kBf16: return cudaLaunchKernelEx(&cfg, k_route_scores<NE, kBf16>, a);
-    case kF16: return cudaLaunchKernelEx(&cfg, k_route_scores<NE, kF16>, a);
-    default: return cudaLaunchKernelEx(&cfg, k_route_scores<NE, kF32>, a);
-  }
+  const bool even = a.experts == 32 * NE && (a.groups == 1 || a.group_size % 32 == 0);
+  return even ? launch_even<NE, true>(cfg, a) : launch_even<NE, false>(cfg, a);
 }
 
 }  // namespace
@@ -534,18 +621,18 @@ cudaError_t launch_route_scores(RouteScoreArgs a, cudaStream_t st) {
   for (int g = 1; g < a.groups; g <<= 1) lanes >>= 1;
   a.lanes = lanes;
   a.group_size = a.experts / a.groups;
+  a.run_shift = 0;
+  while ((64 << a.run_shift) <= a.group_size) ++a.run_shift;
   a.group_inv = (1 << 20) / a.group_size + 1;  // e / group_size = e * inv >> 20 for e, group_size <= 1024
-  if (a.counts != nullptr) {
-    const cudaError_t e = cudaMemsetAsync(a.counts, 0, sizeof(int32_t) * a.experts, st);
-    if (e != cudaSuccess || a.tokens == 0) return e;
-  }
   cudaLaunchConfig_t cfg = {};
-  // Every row a warp of its own while the GPU has room for all of them
-  // (resident: 16 warps per SM), then a share of the rows each.
+  // Every row a warp of its own while the GPU has room for all of them, then
+  // a share of the rows each.  (More resident warps cost registers that the
+  // next row's logits need: 8192 rows of 512 experts in groups took 27 us with
+  // 16 warps per SM, 35 us with 24.)
   DeviceAttrs dev;
   const cudaError_t de = current_device_attrs(&dev);
   if (de != cudaSuccess) return de;
-  cfg.gridDim = dim3(std::min((a.tokens + kRouteWarps - 1) / kRouteWarps, dev.sms * (16 / kRouteWarps)));
+  cfg.gridDim = dim3(std::min((a.tokens + kRouteWarps - 1) / kRouteWarps, dev.sms * kRouteResident));
   cfg.blockDim = dim3(32 * kRouteWarps);
   cfg.dynamicSmemBytes = sizeof(double) * kRouteWarps * warp_doubles(a.experts) + sizeof(int) * a.experts;
   cfg.stream = st;
@@ -554,6 +641,15 @@ cudaError_t launch_route_scores(RouteScoreArgs a, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (a.counts != nullptr) {
+    // A kernel of our own, so that the next one's launch overlaps it.
+    cudaLaunchConfig_t clear = cfg;
+    clear.gridDim = dim3(1);
+    clear.blockDim = dim3(256);
+    clear.dynamicSmemBytes = 0;
+    const cudaError_t e = cudaLaunchKernelEx(&clear, k_clear_counts, a.counts, a.experts);
+    if (e != cudaSuccess || a.tokens == 0) return e;
+  }
   if (a.experts <= 128) return launch_ne<4>(cfg, a);
   if (a.experts <= 256) return launch_ne<8>(cfg, a);
   if (a.experts <= 512) return launch_ne<16>(cfg, a);
