@@ -86,6 +86,42 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
 }
+// The same for a pair of CTAs (issued by the even one): M = 256, A rows and N
+// rows split over the two CTAs' shared memory at the same offsets, D in both
+// CTAs' TMEM; the commit arrives at the same barrier of both.
+__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+// A load into this CTA's shared memory that completes on a barrier of the
+// pair (`bar`: its shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // 32 consecutive f32 columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
@@ -357,14 +393,14 @@ struct Tile {
 };
 // Tiles in groups of kGroup along P, so that those running together share
 // rows of both operands in L2.
-__device__ __forceinline__ Tile tile_of(const LinearArgs& a, int u) {
-  constexpr int kGroup = 16;
+__device__ __forceinline__ Tile tile_of(const LinearArgs& a, int u, int height = kBM) {
+  const int kGroup = 16 * kBM / height;
   const int per = kGroup * a.tiles_q;
   const int g = u / per, rest = u - g * per;
   const int size = min(kGroup, a.tiles_p - g * kGroup);
   Tile t;
   t.q0 = rest / size * a.bn;
-  t.p0 = (g * kGroup + rest % size) * kBM;
+  t.p0 = (g * kGroup + rest % size) * height;
   return t;
 }
 
@@ -645,6 +681,154 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
 }
 
+// ---- pairs of CTAs ----------------------------------------------------------------------
+//
+// k_linear_pair: two CTAs on one 256 x bn tile.  A stage brings 128 P rows and
+// bn / 2 Q rows into each CTA, so a 256 x 256 tile loads 32 KB per CTA for 512
+// cycles of MMA, where a CTA alone with 128 x 256 loads 48 KB: the traffic from
+// L2 was what bound that one.  The even CTA issues the MMAs of both; full and
+// acc_empty barriers are its own, commits arrive at empty and acc_full of both.
+
+__global__ void __launch_bounds__(kMmaThreads, 1)
+    k_linear_pair(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                  const __grid_constant__ LinearArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  unsigned char* ring = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  const int slot = kABytes + a.bn / 2 * kBK * 2;
+  LinearTail* tail = reinterpret_cast<LinearTail*>(ring + a.ring_bytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stages = a.stages;
+  const uint32_t rank = cluster_rank();
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&tail->full[i], 1);
+      mbar_init(&tail->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tail->acc_full[i], 1);
+      mbar_init(&tail->acc_empty[i], 2 * kEpiWarps);
+    }
+    mbar_init(&tail->drained, 1);
+    tail->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tail->tmem_base)),
+                 "r"(a.tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers and TMEM are there
+  tc_fence_after();
+  const uint32_t tmem = tail->tmem_base;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int total = a.tiles_p * a.tiles_q;
+  const int u0 = static_cast<int>(blockIdx.x) / 2, step = static_cast<int>(gridDim.x) / 2;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- producer ----------------
+      int it = 0;
+      bool ok = true;
+      for (int u = u0; ok && u < total; u += step) {
+        const Tile w = tile_of(a, u, 2 * kBM);
+        const int p0 = w.p0 + static_cast<int>(rank) * kBM, q0 = w.q0 + static_cast<int>(rank) * (a.bn / 2);
+        for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
+          const int st = it % stages;
+          if (!mbar_wait_bounded(&tail->empty[st], ((it / stages) & 1) ^ 1u, kWaitNs) || gave_up(tail)) {
+            give_up(tail);
+            ok = false;
+            break;
+          }
+          unsigned char* s = ring + static_cast<size_t>(st) * slot;
+          const uint32_t bar = at_rank(&tail->full[st], 0);
+          if (rank == 0) mbar_arrive_expect_tx(&tail->full[st], static_cast<uint32_t>(2 * slot));
+          tma_load_2d_pair(s, &map_p, kb * kBK, p0, bar);
+          tma_load_2d_pair(s + kABytes, &map_q, kb * kBK, q0, bar);
+        }
+      }
+      // Both CTAs' loads have landed once the MMAs that read them are done, or
+      // (the even CTA, below) once their full barriers have flipped.
+      if (rank == 0)
+        for (int j = it > stages ? it - stages : 0; j < it; ++j)
+          if (!mbar_wait_bounded(&tail->full[j % stages], (j / stages) & 1, kWaitNs)) give_up(tail);
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      // ---------------- MMA, for both CTAs ----------------
+      int it = 0, ai = 0;
+      bool ok = true;
+      const uint32_t idesc = idesc_f16(2 * kBM, a.bn, a.dtype == kBf16);
+      for (int u = u0; ok && u < total; u += step, ++ai) {
+        const int buf = ai & 1;
+        if (gave_up(tail) || !mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u, kWaitNs)) {
+          give_up(tail);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + buf * a.bn;
+        for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
+          const int st = it % stages;
+          if (!mbar_wait_bounded(&tail->full[st], (it / stages) & 1, kWaitNs)) {
+            give_up(tail);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(ring + static_cast<size_t>(st) * slot), sb = sa + kABytes;
+#pragma unroll
+          for (int i = 0; i < kBK / 16; ++i)
+            umma_f16_pair(d, sw128_desc(sa + i * 32), sw128_desc(sb + i * 32), idesc, (kb > 0 || i > 0) ? 1u : 0u);
+          umma_commit_pair(&tail->empty[st]);
+        }
+        if (ok) umma_commit_pair(&tail->acc_full[buf]);
+      }
+      umma_commit_pair(&tail->drained);
+    }
+    // Every MMA has completed once `drained` flips, in either CTA.
+    if (lane == 0 && !mbar_wait_bounded(&tail->drained, 0, 2 * kWaitNs)) give_up(tail);
+  } else {
+    // ---------------- epilogue ----------------
+    const int set = (warp - 2) >> 2;
+    const int q = warp & 3;
+    const int row = q * 32 + lane;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    int ai = 0;
+    for (int u = u0; u < total; u += step, ++ai) {
+      const Tile w = tile_of(a, u, 2 * kBM);
+      const int t = w.p0 + static_cast<int>(rank) * kBM + row;
+      const int valid = min(a.bn, a.q_rows - w.q0);
+      const int buf = ai & 1;
+      const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, kWaitNs);
+      if (!__all_sync(kAll, got)) {
+        if (lane == 0) give_up(tail);
+        break;
+      }
+      tc_fence_after();
+      for (int c0 = 32 * set; c0 < a.bn; c0 += 64) {
+        float v[32];
+        tmem_ld32(lane_base + buf * a.bn + c0, v);
+        if (t < a.p_rows && c0 < valid) finish_run<32>(a, t, w.q0 + c0, v);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_at(at_rank(&tail->acc_empty[buf], 0));
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA leaves while the other's MMAs, copies or arrivals may reach it
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+}
+
 // ---- one to four tokens -------------------------------------------------------------------
 
 constexpr int kRowWarps = 8;
@@ -839,6 +1023,29 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
     a.splits = per;
     const bool al = aligned(w, a.rows == 1 ? 0 : w_stride, kBf16) && aligned(x, a.tokens == 1 ? 0 : x_stride, kBf16);
     return a.dtype == kBf16 ? launch_rows<true>(a, al, st) : launch_rows<false>(a, al, st);
+  }
+
+  {
+    const long long pairs = static_cast<long long>((a.tokens + 255) / 256) * ((a.rows + 255) / 256);
+    if (pairs >= dev.sms / 2 && a.out_dtype != kF32 && tma_can_read(w, a.rows, w_stride) &&
+        tma_can_read(x, a.tokens, x_stride)) {
+      a.p_rows = a.tokens;
+      a.q_rows = a.rows;
+      a.bn = 256;
+      a.tiles_p = (a.tokens + 255) / 256;
+      a.tiles_q = (a.rows + 255) / 256;
+      a.kblocks = (a.cols + kBK - 1) / kBK;
+      const int slot = kABytes + a.bn / 2 * kBK * 2;
+      a.stages = std::min(kMaxStages, (200 * 1024) / slot);
+      a.ring_bytes = a.stages * slot;
+      a.tmem_cols = 512;
+      CUtensorMap mp = {}, mq = {};
+      if (!operand_map(&mp, x, a.cols, a.p_rows, x_stride, kBM, a.dtype) ||
+          !operand_map(&mq, w, a.cols, a.q_rows, w_stride, a.bn / 2, a.dtype))
+        return cudaErrorInvalidValue;
+      const int grid = 2 * static_cast<int>(std::min<long long>(pairs, dev.sms / 2));
+      return launch(k_linear_pair, grid, kMmaThreads, 1024 + a.ring_bytes + sizeof(LinearTail), 2, st, mp, mq, a);
+    }
   }
 
   // Few tokens: w on the M side, all tokens in one N tile, K split over a

@@ -80,6 +80,14 @@ def test_sizes_and_types(size, dtype, out):
     case(*size, dtype=dtype, out=out)
 
 
+@pytest.mark.parametrize("size", [(2600, 2312, 200), (2304, 2304, 64), (4097, 4090, 136), (8192, 640, 1000),
+                                  (20000, 264, 72)])
+def test_many_tiles(size):
+    case(*size, bias="bf16", activation="silu", residual="bf16")
+    case(*size, dtype="f16", residual="f32")
+    case(*size, out="f32", bias="f32")
+
+
 @pytest.mark.parametrize("activation", ACTIVATIONS)
 @pytest.mark.parametrize("size", [(1, 300, 512), (40, 300, 512), (300, 264, 512), (300, 263, 511)])
 def test_activations(activation, size):
