@@ -114,6 +114,18 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       "l"(map), "r"(c0), "r"(c1), "r"(bar)
       : "memory");
 }
+// One lane of a converged warp, always the same.  The producer and MMA warps
+// run their loops with all lanes, so that addresses and descriptors stay in
+// uniform registers, and issue with the elected one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
 __device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
@@ -286,11 +298,145 @@ __device__ __forceinline__ void store_vec(void* p, long long i, int dtype, const
   }
 }
 
-// N consecutive outputs of token t from row r on (bias, activation,
-// residual, rounding).
+// Two f32 values per 64-bit register, one instruction for both.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 pack(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 pack(float a) { return pack(a, a); }
+__device__ __forceinline__ void unpack(F2 p, float* a, float* b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(p.v));
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// x / (1 + 2^z) per half, or 1 / (1 + 2^z): 1 + 2^z = inf gives 0.
+__device__ __forceinline__ F2 gate2(F2 x, F2 z) {
+  float z0, z1;
+  unpack(z, &z0, &z1);
+  unpack(add2(pack(ex2(z0), ex2(z1)), pack(1.0f)), &z0, &z1);
+  return mul2(x, pack(rcp(z0), rcp(z1)));
+}
+// The activations on N packed pairs (see activate).
 template <int N>
-__device__ __forceinline__ void finish_run(const LinearArgs& a, int t, int r, float (&v)[N]) {
-  if (a.vec && r + N <= a.rows) {
+__device__ __forceinline__ void activate_pairs(int act, F2 (&v)[N]) {
+  if (act == kActNone) return;
+  if (act == kActGeluTanh) {
+    // exp(-2u) = 2^(x (c1 + c3 x^2))
+    const F2 c1 = pack(-1.5957691216057308f * kLog2e), c3 = pack(-1.5957691216057308f * 0.044715f * kLog2e);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = gate2(v[j], mul2(v[j], fma2(mul2(v[j], v[j]), c3, c1)));
+  } else if (act == kActSilu) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = gate2(v[j], mul2(v[j], pack(-kLog2e)));
+  } else if (act == kActSigmoid) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = gate2(pack(1.0f), mul2(v[j], pack(-kLog2e)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float x, y;
+      unpack(v[j], &x, &y);
+      v[j] = act == kActRelu ? pack(activate<kActRelu>(x), activate<kActRelu>(y))
+                             : pack(activate<kActGelu>(x), activate<kActGelu>(y));
+    }
+  }
+}
+// Adds 2 N consecutive values from p + i on (16 bytes at a time).
+template <int N>
+__device__ __forceinline__ void add_vec(const void* p, long long i, int dtype, F2 (&v)[N]) {
+  if (dtype == kF32) {
+    const ulonglong2* s = reinterpret_cast<const ulonglong2*>(static_cast<const float*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+      const ulonglong2 u = s[j];
+      v[2 * j] = add2(v[2 * j], F2{u.x});
+      v[2 * j + 1] = add2(v[2 * j + 1], F2{u.y});
+    }
+    return;
+  }
+  const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) {
+    const uint4 u = s[j];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float lo, hi;
+      unpack2(dtype, w[k], &lo, &hi);
+      v[4 * j + k] = add2(v[4 * j + k], pack(lo, hi));
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_pairs(void* p, long long i, int dtype, const F2 (&v)[N]) {
+  if (dtype == kF32) {
+    ulonglong2* d = reinterpret_cast<ulonglong2*>(static_cast<float*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) d[j] = make_ulonglong2(v[2 * j].v, v[2 * j + 1].v);
+    return;
+  }
+  uint32_t w[N];
+  if (dtype == kBf16) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float lo, hi;
+      unpack(v[j], &lo, &hi);
+      w[j] = pack2(kBf16, lo, hi);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float lo, hi;
+      unpack(v[j], &lo, &hi);
+      w[j] = pack2(kF16, lo, hi);
+    }
+  }
+  uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i);
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) d[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+
+// N consecutive outputs of token t from row r on (bias, activation,
+// residual, rounding).  `bias`: this run's bias in f32 in shared memory, or
+// null to read it from global memory.
+template <int N>
+__device__ __forceinline__ void finish_run(const LinearArgs& a, int t, int r, float (&v)[N],
+                                           const float* bias = nullptr) {
+  if (N >= 8 && a.vec && r + N <= a.rows) {
+    constexpr int kPairs = N >= 8 ? N / 2 : 4;
+    F2 p[kPairs];
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) p[j] = pack(v[2 * j], v[2 * j + 1]);
+    if (bias != nullptr) add_vec<kPairs>(bias, 0, kF32, p);
+    else if (a.bias != nullptr) add_vec<kPairs>(a.bias, r, a.bias_dtype, p);
+    activate_pairs<kPairs>(a.act, p);
+    if (a.residual != nullptr) add_vec<kPairs>(a.residual, static_cast<long long>(t) * a.res_stride + r, a.res_dtype, p);
+    store_pairs<kPairs>(a.y, static_cast<long long>(t) * a.y_stride + r, a.out_dtype, p);
+    return;
+  }
+  if (N == 4 && a.vec && r + N <= a.rows) {
     float b[N];
     if (a.bias != nullptr) {
       load_vec<N>(a.bias, r, a.bias_dtype, b);
@@ -380,7 +526,22 @@ struct __align__(16) LinearTail {
   uint64_t drained;
   uint32_t tmem_base;
   int abort;
+  float bias[kEpiWarps][128];  // each epilogue warp's columns of a tile, in f32
 };
+
+// The bias of a warp's 32-column groups c0 = 32 set, + 64, ... (four at most)
+// of the rows from r0 on, into its shared memory; null without a bias.
+__device__ __forceinline__ const float* fetch_bias(const LinearArgs& a, float* mine, int r0, int set, int lane) {
+  if (a.bias == nullptr) return nullptr;
+  __syncwarp();
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int r = r0 + 32 * set + 64 * g + lane;
+    mine[32 * g + lane] = r < a.rows ? load_f32(a.bias, r, a.bias_dtype) : 0.0f;
+  }
+  __syncwarp();
+  return mine;
+}
 
 __device__ __forceinline__ void give_up(LinearTail* t) {
   atomicCAS(&g_status, 0, kErrTimeout);
@@ -532,6 +693,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     for (int u = u0; u < total; u += step) {
       const Tile w = tile_of(a, u);
       const int valid = min(a.bn, a.q_rows - w.q0);
+      const float* bias = nullptr;
       auto finish = [&](int c0, float(&v)[32]) {
         if (a.splits > 1) {
 #pragma unroll
@@ -539,15 +701,16 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
             if (c0 + j < valid) parts[(c0 + j) * kBM + row] = v[j];
         } else if (w.p0 + row < a.p_rows && c0 < valid) {
           if (a.swap) finish_column(a, w.q0 + c0, min(32, valid - c0), w.p0 + row, v);
-          else if (a.bn - c0 >= 32) finish_run<32>(a, w.p0 + row, w.q0 + c0, v);
+          else if (a.bn - c0 >= 32) finish_run<32>(a, w.p0 + row, w.q0 + c0, v, bias != nullptr ? bias + c0 / 64 * 32 : nullptr);
           else {  // the last 16 columns of a tile that is no multiple of 32
             float h[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) h[j] = v[j];
-            finish_run<16>(a, w.p0 + row, w.q0 + c0, h);
+            finish_run<16>(a, w.p0 + row, w.q0 + c0, h, bias != nullptr ? bias + c0 / 64 * 32 : nullptr);
           }
         }
       };
+      if (!a.swap) bias = fetch_bias(a, tail->bias[warp - 2], w.q0, set, lane);
       if (!CHUNKED) {
         const int buf = ai & 1;
         const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, kWaitNs);
@@ -732,67 +895,82 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   const int u0 = static_cast<int>(blockIdx.x) / 2, step = static_cast<int>(gridDim.x) / 2;
 
   if (warp == 0) {
-    if (lane == 0) {
-      // ---------------- producer ----------------
-      int it = 0;
-      bool ok = true;
-      for (int u = u0; ok && u < total; u += step) {
-        const Tile w = tile_of(a, u, 2 * kBM);
-        const int p0 = w.p0 + static_cast<int>(rank) * kBM, q0 = w.q0 + static_cast<int>(rank) * (a.bn / 2);
-        for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
-          const int st = it % stages;
-          if (!mbar_wait_bounded(&tail->empty[st], ((it / stages) & 1) ^ 1u, kWaitNs) || gave_up(tail)) {
-            give_up(tail);
-            ok = false;
-            break;
-          }
-          unsigned char* s = ring + static_cast<size_t>(st) * slot;
-          const uint32_t bar = at_rank(&tail->full[st], 0);
+    // ---------------- producer ----------------
+    int it = 0, st = 0;
+    uint32_t phase = 1u;
+    bool ok = true;
+    for (int u = u0; ok && u < total; u += step) {
+      const Tile w = tile_of(a, u, 2 * kBM);
+      const int p0 = w.p0 + static_cast<int>(rank) * kBM, q0 = w.q0 + static_cast<int>(rank) * (a.bn / 2);
+      for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
+        if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, kWaitNs) && !gave_up(tail))) {
+          give_up(tail);
+          ok = false;
+          break;
+        }
+        unsigned char* s = ring + st * slot;
+        const uint32_t bar = at_rank(&tail->full[st], 0);
+        if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&tail->full[st], static_cast<uint32_t>(2 * slot));
           tma_load_2d_pair(s, &map_p, kb * kBK, p0, bar);
           tma_load_2d_pair(s + kABytes, &map_q, kb * kBK, q0, bar);
         }
+        if (++st == stages) {
+          st = 0;
+          phase ^= 1u;
+        }
       }
-      // Both CTAs' loads have landed once the MMAs that read them are done, or
-      // (the even CTA, below) once their full barriers have flipped.
-      if (rank == 0)
-        for (int j = it > stages ? it - stages : 0; j < it; ++j)
-          if (!mbar_wait_bounded(&tail->full[j % stages], (j / stages) & 1, kWaitNs)) give_up(tail);
     }
+    // Both CTAs' loads have landed once the even CTA's full barriers have
+    // flipped.
+    if (rank == 0)
+      for (int j = it > stages ? it - stages : 0; j < it; ++j)
+        if (!mbar_wait_bounded(&tail->full[j % stages], (j / stages) & 1, kWaitNs)) give_up(tail);
   } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {
+    if (rank == 0) {
       // ---------------- MMA, for both CTAs ----------------
-      int it = 0, ai = 0;
+      int st = 0, ai = 0;
+      uint32_t phase = 0u;
       bool ok = true;
       const uint32_t idesc = idesc_f16(2 * kBM, a.bn, a.dtype == kBf16);
+      const uint64_t desc0 = sw128_desc(smem_u32(ring));
       for (int u = u0; ok && u < total; u += step, ++ai) {
         const int buf = ai & 1;
-        if (gave_up(tail) || !mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u, kWaitNs)) {
+        if (!__all_sync(kAll, !gave_up(tail) &&
+                                  mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u, kWaitNs))) {
           give_up(tail);
           break;
         }
         tc_fence_after();
         const uint32_t d = tmem + buf * a.bn;
-        for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
-          const int st = it % stages;
-          if (!mbar_wait_bounded(&tail->full[st], (it / stages) & 1, kWaitNs)) {
+        for (int kb = 0; kb < a.kblocks; ++kb) {
+          if (!__all_sync(kAll, mbar_wait_bounded(&tail->full[st], phase, kWaitNs))) {
             give_up(tail);
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(ring + static_cast<size_t>(st) * slot), sb = sa + kABytes;
+          const uint64_t da = desc0 + static_cast<uint32_t>(st * slot >> 4), db = da + (kABytes >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int i = 0; i < kBK / 16; ++i)
-            umma_f16_pair(d, sw128_desc(sa + i * 32), sw128_desc(sb + i * 32), idesc, (kb > 0 || i > 0) ? 1u : 0u);
-          umma_commit_pair(&tail->empty[st]);
+            for (int i = 0; i < kBK / 16; ++i)
+              umma_f16_pair(d, da + 2 * i, db + 2 * i, idesc, (kb > 0 || i > 0) ? 1u : 0u);
+            umma_commit_pair(&tail->empty[st]);
+          }
+          __syncwarp();
+          if (++st == stages) {
+            st = 0;
+            phase ^= 1u;
+          }
         }
-        if (ok) umma_commit_pair(&tail->acc_full[buf]);
+        if (ok && elect_one()) umma_commit_pair(&tail->acc_full[buf]);
+        __syncwarp();
       }
-      umma_commit_pair(&tail->drained);
+      if (elect_one()) umma_commit_pair(&tail->drained);
+      __syncwarp();
     }
     // Every MMA has completed once `drained` flips, in either CTA.
-    if (lane == 0 && !mbar_wait_bounded(&tail->drained, 0, 2 * kWaitNs)) give_up(tail);
+    if (!mbar_wait_bounded(&tail->drained, 0, 2 * kWaitNs)) give_up(tail);
   } else {
     // ---------------- epilogue ----------------
     const int set = (warp - 2) >> 2;
@@ -805,6 +983,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const int t = w.p0 + static_cast<int>(rank) * kBM + row;
       const int valid = min(a.bn, a.q_rows - w.q0);
       const int buf = ai & 1;
+      const float* bias = fetch_bias(a, tail->bias[warp - 2], w.q0, set, lane);
       const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, kWaitNs);
       if (!__all_sync(kAll, got)) {
         if (lane == 0) give_up(tail);
@@ -814,7 +993,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       for (int c0 = 32 * set; c0 < a.bn; c0 += 64) {
         float v[32];
         tmem_ld32(lane_base + buf * a.bn + c0, v);
-        if (t < a.p_rows && c0 < valid) finish_run<32>(a, t, w.q0 + c0, v);
+        if (t < a.p_rows && c0 < valid) finish_run<32>(a, t, w.q0 + c0, v, bias != nullptr ? bias + c0 / 64 * 32 : nullptr);
       }
       tc_fence_before();
       __syncwarp();
