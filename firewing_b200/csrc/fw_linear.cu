@@ -179,18 +179,79 @@ __device__ __forceinline__ float ex2(float v) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Two f32 values per 64-bit register, one instruction for both.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 pack(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 pack(float a) { return pack(a, a); }
+__device__ __forceinline__ void unpack(F2 p, float* a, float* b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(p.v));
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float relu(float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+  return r;
+}
+// x/2 (1 + erf(x / sqrt 2)) = max(x, 0) - |x|/2 erfc(|x| / sqrt 2) per half,
+// with erfc(z) = t 2^(-z^2 log2 e + g(t)), t = 1 / (1 + z / 2): t takes z >= 0
+// to (0, 1], where log2(erfc(z) exp(z^2) / t) is smooth.  g is its least
+// squares fit at the Chebyshev points, degree 9: erfc to 1.1e-7 relative for
+// every z, 2.3e-7 in f32.
+__device__ __forceinline__ F2 gelu2(F2 v) {
+  constexpr float g[10] = {-1.82574821f, 1.44272923f,  0.539700329f, 0.139632389f,  -0.268766135f,
+                           0.402343214f, -1.63778341f, 2.14749932f,  -1.18612599f, 0.246519342f};
+  float x, y;
+  unpack(v, &x, &y);
+  const F2 size = pack(fabsf(x), fabsf(y));
+  float t0, t1;
+  unpack(fma2(size, pack(0.35355339059327376f), pack(1.0f)), &t0, &t1);
+  const F2 t = pack(rcp(t0), rcp(t1));
+  F2 p = pack(g[9]);
+#pragma unroll
+  for (int i = 8; i >= 0; --i) p = fma2(p, t, pack(g[i]));
+  p = fma2(mul2(v, v), pack(-0.5f * kLog2e), p);
+  unpack(p, &t0, &t1);
+  const F2 e = mul2(mul2(t, pack(ex2(t0), ex2(t1))), mul2(size, pack(-0.5f)));
+  return add2(pack(relu(x), relu(y)), e);
+}
+
 // The activations in f32.  Those built on exp use x * sigmoid forms, which
 // have no cancellation: their relative error stays near 2^-21 everywhere,
 // far under the rounding of y.  __fdividef(x, y) is 0 for y > 2^126, where
 // the true value is below 2^-118 * |x|.
 template <int ACT>
 __device__ __forceinline__ float activate(float x) {
-  if (ACT == kActRelu) {
-    float r;
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+  if (ACT == kActRelu) return relu(x);
+  if (ACT == kActGelu) {
+    float r, unused;
+    unpack(gelu2(pack(x, 0.0f)), &r, &unused);
     return r;
   }
-  if (ACT == kActGelu) return __fmul_rn(__fmul_rn(0.5f, x), erfcf(__fmul_rn(x, -0.70710678118654752f)));
   if (ACT == kActGeluTanh) {
     // 0.5 x (1 + tanh u) = x / (1 + exp(-2u)), u = sqrt(2/pi) (x + 0.044715 x^3)
     const float u2 = __fmul_rn(__fmul_rn(x, 1.5957691216057308f), __fmaf_rn(__fmul_rn(x, x), 0.044715f, 1.0f));
@@ -298,39 +359,6 @@ __device__ __forceinline__ void store_vec(void* p, long long i, int dtype, const
   }
 }
 
-// Two f32 values per 64-bit register, one instruction for both.
-struct F2 {
-  uint64_t v;
-};
-__device__ __forceinline__ F2 pack(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ F2 pack(float a) { return pack(a, a); }
-__device__ __forceinline__ void unpack(F2 p, float* a, float* b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(p.v));
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ float rcp(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 // x / (1 + 2^z) per half, or 1 / (1 + 2^z): 1 + 2^z = inf gives 0.
 __device__ __forceinline__ F2 gate2(F2 x, F2 z) {
   float z0, z1;
@@ -353,13 +381,15 @@ __device__ __forceinline__ void activate_pairs(int act, F2 (&v)[N]) {
   } else if (act == kActSigmoid) {
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = gate2(pack(1.0f), mul2(v[j], pack(-kLog2e)));
+  } else if (act == kActGelu) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = gelu2(v[j]);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       float x, y;
       unpack(v[j], &x, &y);
-      v[j] = act == kActRelu ? pack(activate<kActRelu>(x), activate<kActRelu>(y))
-                             : pack(activate<kActGelu>(x), activate<kActGelu>(y));
+      v[j] = pack(relu(x), relu(y));
     }
   }
 }
@@ -617,27 +647,29 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
   const int chunk = CHUNKED ? a.chunk : kb1 - kb0;
 
   if (warp == 0) {
-    if (!LOADERS && lane == 0) {
+    if (!LOADERS) {
       // ---------------- producer ----------------
-      int it = 0;
+      int it = 0, st = 0;
+      uint32_t phase = 1u;
       bool ok = true;
       for (int u = u0; ok && u < total; u += step) {
         const Tile w = tile_of(a, u);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int st = it % stages;
-          if (!mbar_wait_bounded(&tail->empty[st], ((it / stages) & 1) ^ 1u, kWaitNs)) {
+          if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, kWaitNs) && !gave_up(tail))) {
             give_up(tail);
             ok = false;
             break;
           }
-          if (gave_up(tail)) {
-            ok = false;
-            break;
+          unsigned char* s = ring + st * slot;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&tail->full[st], static_cast<uint32_t>(slot));
+            tma_load_2d(s, &map_p, kb * kBK, w.p0, &tail->full[st]);
+            tma_load_2d(s + kABytes, &map_q, kb * kBK, w.q0, &tail->full[st]);
           }
-          unsigned char* s = ring + static_cast<size_t>(st) * slot;
-          mbar_arrive_expect_tx(&tail->full[st], static_cast<uint32_t>(slot));
-          tma_load_2d(s, &map_p, kb * kBK, w.p0, &tail->full[st]);
-          tma_load_2d(s + kABytes, &map_q, kb * kBK, w.q0, &tail->full[st]);
+          if (++st == stages) {
+            st = 0;
+            phase ^= 1u;
+          }
         }
       }
       // Copies already issued land before the CTA can exit.
@@ -646,42 +678,51 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     }
   } else if (warp == 1) {
     // ---------------- MMA ----------------
-    if (lane == 0) {
-      int it = 0, ai = 0;
-      bool ok = true;
-      const uint32_t idesc = idesc_f16(kBM, a.bn, a.dtype == kBf16);
-      for (int u = u0; ok && u < total; u += step) {
-        for (int k = kb0; ok && k < kb1; k += chunk, ++ai) {
-          const int buf = ai & 1;
-          if (gave_up(tail) || !mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u, kWaitNs)) {
+    int st = 0, ai = 0;
+    uint32_t phase = 0u;
+    bool ok = true;
+    const uint32_t idesc = idesc_f16(kBM, a.bn, a.dtype == kBf16);
+    const uint64_t desc0 = sw128_desc(smem_u32(ring));
+    for (int u = u0; ok && u < total; u += step) {
+      for (int k = kb0; ok && k < kb1; k += chunk, ++ai) {
+        const int buf = ai & 1;
+        if (!__all_sync(kAll, !gave_up(tail) &&
+                                  mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u, kWaitNs))) {
+          give_up(tail);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + buf * acc_cols;
+        const int end = min(kb1, k + chunk);
+        for (int kb = k; kb < end; ++kb) {
+          if (!__all_sync(kAll, mbar_wait_bounded(&tail->full[st], phase, kWaitNs))) {
             give_up(tail);
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t d = tmem + buf * acc_cols;
-          const int end = min(kb1, k + chunk);
-          for (int kb = k; kb < end; ++kb, ++it) {
-            const int st = it % stages;
-            if (!mbar_wait_bounded(&tail->full[st], (it / stages) & 1, kWaitNs)) {
-              give_up(tail);
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t sa = smem_u32(ring + static_cast<size_t>(st) * slot), sb = sa + kABytes;
+          const uint64_t da = desc0 + static_cast<uint32_t>(st * slot >> 4), db = da + (kABytes >> 4);
+          if (elect_one()) {
 #pragma unroll
             for (int i = 0; i < kBK / 16; ++i)
-              umma_f16(d, sw128_desc(sa + i * 32), sw128_desc(sb + i * 32), idesc, (kb > k || i > 0) ? 1u : 0u);
+              umma_f16(d, da + 2 * i, db + 2 * i, idesc, (kb > k || i > 0) ? 1u : 0u);
             umma_commit(&tail->empty[st]);
           }
-          if (ok) umma_commit(&tail->acc_full[buf]);
+          __syncwarp();
+          if (++st == stages) {
+            st = 0;
+            phase ^= 1u;
+          }
         }
+        if (ok && elect_one()) umma_commit(&tail->acc_full[buf]);
+        __syncwarp();
       }
-      // Every MMA issued has completed once `drained` flips.
-      umma_commit(&tail->drained);
-      if (!mbar_wait_bounded(&tail->drained, 0, kWaitNs)) give_up(tail);
     }
+    // Every MMA issued has completed once `drained` flips.
+    if (elect_one()) umma_commit(&tail->drained);
+    __syncwarp();
+    if (!mbar_wait_bounded(&tail->drained, 0, kWaitNs)) give_up(tail);
   } else if (warp < 2 + kEpiWarps) {
     // ---------------- epilogue ----------------
     const int set = (warp - 2) >> 2;
