@@ -26,6 +26,7 @@
 // exits; fw_primitive_status reports it.
 #include <algorithm>
 #include <cstdint>
+#include <map>
 #include <mutex>
 
 #include <cudaTypedefs.h>
@@ -43,8 +44,18 @@ constexpr int kABytes = kBM * kBK * 2;    // 16 KB
 constexpr int kMaxStages = 8;
 constexpr int kEpiWarps = 8;
 constexpr int kLoadWarps = 8;
+constexpr int kWarpRows = 24;                         // rows of a stage that a loader warp fills
+constexpr int kLoadBn = kLoadWarps * kWarpRows - kBM;  // so N tiles are this wide at most (64)
+constexpr int kAhead = 3;                             // stages that loaders fetch ahead
+constexpr int kRawBytes = kWarpRows * 144;            // a warp's words of a stage
+constexpr int kLoadStages = 3;                        // operand stages beside them
+constexpr int kRawTotal = kLoadWarps * (kAhead + 1) * kRawBytes;
 constexpr int kMmaThreads = 32 * (2 + kEpiWarps);
-constexpr int kLoaderThreads = kMmaThreads + 32 * kLoadWarps;
+// With loaders half the epilogue warps: registers for 14 warps, not 18, and
+// N tiles are narrow then.
+constexpr int kLoaderEpiWarps = 4;
+constexpr int kLoaderThreads = 32 * (2 + kLoaderEpiWarps + kLoadWarps);
+constexpr int kChunk = 4;  // stages per accumulation for f32 outputs
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -261,33 +272,6 @@ __device__ __forceinline__ float activate(float x) {
   if (ACT == kActSigmoid) return __fdividef(1.0f, __fadd_rn(1.0f, ex2(__fmul_rn(x, -kLog2e))));
   return x;
 }
-template <int N>
-__device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
-  switch (act) {
-    case kActRelu:
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = activate<kActRelu>(v[j]);
-      break;
-    case kActGelu:
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = activate<kActGelu>(v[j]);
-      break;
-    case kActGeluTanh:
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = activate<kActGeluTanh>(v[j]);
-      break;
-    case kActSilu:
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = activate<kActSilu>(v[j]);
-      break;
-    case kActSigmoid:
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = activate<kActSigmoid>(v[j]);
-      break;
-    default: break;
-  }
-}
-
 __device__ __forceinline__ float load_f32(const void* p, long long i, int dtype) {
   if (dtype == kF32) return static_cast<const float*>(p)[i];
   const uint16_t v = static_cast<const uint16_t*>(p)[i];
@@ -314,51 +298,6 @@ __device__ __forceinline__ void unpack2(int dtype, uint32_t w, float* lo, float*
     *hi = __half2float(__ushort_as_half(static_cast<uint16_t>(w >> 16)));
   }
 }
-// N (4 or a multiple of 8) consecutive values as f32, 8 or 16 bytes at a
-// time: p + i aligned to that.
-template <int N>
-__device__ __forceinline__ void load_vec(const void* p, long long i, int dtype, float (&v)[N]) {
-  if (dtype == kF32) {
-    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-#pragma unroll
-    for (int j = 0; j < N / 4; ++j) {
-      const float4 f = s[j];
-      v[4 * j] = f.x, v[4 * j + 1] = f.y, v[4 * j + 2] = f.z, v[4 * j + 3] = f.w;
-    }
-  } else if (N == 4) {
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-    unpack2(dtype, u.x, &v[0], &v[1]);
-    unpack2(dtype, u.y, &v[2], &v[3]);
-  } else {
-    const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-#pragma unroll
-    for (int j = 0; j < N / 8; ++j) {
-      const uint4 u = s[j];
-      unpack2(dtype, u.x, &v[8 * j], &v[8 * j + 1]);
-      unpack2(dtype, u.y, &v[8 * j + 2], &v[8 * j + 3]);
-      unpack2(dtype, u.z, &v[8 * j + 4], &v[8 * j + 5]);
-      unpack2(dtype, u.w, &v[8 * j + 6], &v[8 * j + 7]);
-    }
-  }
-}
-template <int N>
-__device__ __forceinline__ void store_vec(void* p, long long i, int dtype, const float (&v)[N]) {
-  if (dtype == kF32) {
-    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
-#pragma unroll
-    for (int j = 0; j < N / 4; ++j) d[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  } else if (N == 4) {
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) =
-        make_uint2(pack2(dtype, v[0], v[1]), pack2(dtype, v[2], v[3]));
-  } else {
-    uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i);
-#pragma unroll
-    for (int j = 0; j < N / 8; ++j)
-      d[j] = make_uint4(pack2(dtype, v[8 * j], v[8 * j + 1]), pack2(dtype, v[8 * j + 2], v[8 * j + 3]),
-                        pack2(dtype, v[8 * j + 4], v[8 * j + 5]), pack2(dtype, v[8 * j + 6], v[8 * j + 7]));
-  }
-}
-
 // x / (1 + 2^z) per half, or 1 / (1 + 2^z): 1 + 2^z = inf gives 0.
 __device__ __forceinline__ F2 gate2(F2 x, F2 z) {
   float z0, z1;
@@ -448,83 +387,80 @@ __device__ __forceinline__ void store_pairs(void* p, long long i, int dtype, con
   for (int j = 0; j < N / 4; ++j) d[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
 }
 
-// N consecutive outputs of token t from row r on (bias, activation,
-// residual, rounding).  `bias`: this run's bias in f32 in shared memory, or
-// null to read it from global memory.
-template <int N>
-__device__ __forceinline__ void finish_run(const LinearArgs& a, int t, int r, float (&v)[N],
-                                           const float* bias = nullptr) {
-  if (N >= 8 && a.vec && r + N <= a.rows) {
-    constexpr int kPairs = N >= 8 ? N / 2 : 4;
-    F2 p[kPairs];
-#pragma unroll
-    for (int j = 0; j < N / 2; ++j) p[j] = pack(v[2 * j], v[2 * j + 1]);
-    if (bias != nullptr) add_vec<kPairs>(bias, 0, kF32, p);
-    else if (a.bias != nullptr) add_vec<kPairs>(a.bias, r, a.bias_dtype, p);
-    activate_pairs<kPairs>(a.act, p);
-    if (a.residual != nullptr) add_vec<kPairs>(a.residual, static_cast<long long>(t) * a.res_stride + r, a.res_dtype, p);
-    store_pairs<kPairs>(a.y, static_cast<long long>(t) * a.y_stride + r, a.out_dtype, p);
-    return;
-  }
-  if (N == 4 && a.vec && r + N <= a.rows) {
-    float b[N];
-    if (a.bias != nullptr) {
-      load_vec<N>(a.bias, r, a.bias_dtype, b);
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], b[j]);
-    }
-    activate_all(a.act, v);
-    if (a.residual != nullptr) {
-      load_vec<N>(a.residual, static_cast<long long>(t) * a.res_stride + r, a.res_dtype, b);
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], b[j]);
-    }
-    store_vec<N>(a.y, static_cast<long long>(t) * a.y_stride + r, a.out_dtype, v);
-    return;
-  }
-  const int n = min(N, a.rows - r);
-  if (a.bias != nullptr) {
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) v[j] = __fadd_rn(v[j], load_f32(a.bias, r + j, a.bias_dtype));
-  }
-  activate_all(a.act, v);
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    if (j >= n) break;
-    if (a.residual != nullptr)
-      v[j] = __fadd_rn(v[j], load_f32(a.residual, static_cast<long long>(t) * a.res_stride + r + j, a.res_dtype));
-    store_f32(a.y, static_cast<long long>(t) * a.y_stride + r + j, a.out_dtype, v[j]);
-  }
+// Output (t, r) from its sum: the form for every size, stride and type.  Its
+// many cases are long code: callers loop over it.
+__device__ __forceinline__ void finish_one(const LinearArgs& a, int t, int r, float v) {
+  if (a.bias != nullptr) v = __fadd_rn(v, load_f32(a.bias, r, a.bias_dtype));
+  F2 p[1] = {pack(v, 0.0f)};
+  activate_pairs<1>(a.act, p);
+  float unused;
+  unpack(p[0], &v, &unused);
+  if (a.residual != nullptr)
+    v = __fadd_rn(v, load_f32(a.residual, static_cast<long long>(t) * a.res_stride + r, a.res_dtype));
+  store_f32(a.y, static_cast<long long>(t) * a.y_stride + r, a.out_dtype, v);
 }
-// 32 tokens from t on of row r (lanes of a warp hold consecutive rows).
-__device__ __forceinline__ void finish_column(const LinearArgs& a, int t, int n, int r, float (&v)[32]) {
-  const float b = a.bias != nullptr ? load_f32(a.bias, r, a.bias_dtype) : 0.0f;
-  if (a.bias != nullptr) {
+// 32 outputs of token t from row r on, where 16-byte accesses serve (a.vec,
+// all 32 rows there).  `bias`: their bias in f32 in shared memory, or null.
+__device__ __forceinline__ void finish_run(const LinearArgs& a, int t, int r, const float (&v)[32],
+                                           const float* bias) {
+  F2 p[16];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], b);
+  for (int j = 0; j < 16; ++j) p[j] = pack(v[2 * j], v[2 * j + 1]);
+  if (bias != nullptr) add_vec<16>(bias, 0, kF32, p);
+  activate_pairs<16>(a.act, p);
+  if (a.residual != nullptr) add_vec<16>(a.residual, static_cast<long long>(t) * a.res_stride + r, a.res_dtype, p);
+  store_pairs<16>(a.y, static_cast<long long>(t) * a.y_stride + r, a.out_dtype, p);
+}
+// Four outputs of token t from row r on (from shared memory's partial sums).
+__device__ __forceinline__ void finish_four(const LinearArgs& a, int t, int r, float4 v) {
+  if (a.vec && a.out_dtype != kF32 && a.residual == nullptr && r + 4 <= a.rows) {
+    F2 p[2] = {pack(v.x, v.y), pack(v.z, v.w)};
+    if (a.bias != nullptr) {
+      p[0] = add2(p[0], pack(load_f32(a.bias, r, a.bias_dtype), load_f32(a.bias, r + 1, a.bias_dtype)));
+      p[1] = add2(p[1], pack(load_f32(a.bias, r + 2, a.bias_dtype), load_f32(a.bias, r + 3, a.bias_dtype)));
+    }
+    activate_pairs<2>(a.act, p);
+    float w[4];
+    unpack(p[0], &w[0], &w[1]);
+    unpack(p[1], &w[2], &w[3]);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + static_cast<long long>(t) * a.y_stride + r) =
+        make_uint2(pack2(a.out_dtype, w[0], w[1]), pack2(a.out_dtype, w[2], w[3]));
+    return;
   }
-  activate_all(a.act, v);
+#pragma unroll 1
+  for (int i = 0; i < 4 && r + i < a.rows; ++i)
+    finish_one(a, t, r + i, i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
+}
+// A warp's 32 lanes by 32 columns of a tile from (p0, q0) on, through shared
+// memory eight columns at a time, so that neighbouring lanes have
+// neighbouring outputs and the loop over them stays short code.  swap: lanes
+// are rows and columns tokens; p_end, q_end: where the tile's end.
+constexpr int kStageFloats = 32 * 9;
+__device__ __forceinline__ void finish_block(const LinearArgs& a, int p0, int q0, int p_end, int q_end,
+                                             const float (&v)[32], float* stage, int lane) {
+#pragma unroll 1
+  for (int g = 0; g < 4 && q0 + 8 * g < q_end; ++g) {
+    __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    if (j >= n) break;
-    if (a.residual != nullptr)
-      v[j] = __fadd_rn(v[j], load_f32(a.residual, static_cast<long long>(t + j) * a.res_stride + r, a.res_dtype));
-    store_f32(a.y, static_cast<long long>(t + j) * a.y_stride + r, a.out_dtype, v[j]);
+    for (int j = 0; j < 8; ++j) {
+      const float x = g == 0 ? v[j] : g == 1 ? v[8 + j] : g == 2 ? v[16 + j] : v[24 + j];
+      stage[a.swap ? 33 * j + lane : 9 * lane + j] = x;
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const int row = a.swap ? lane : 4 * i + lane / 8, col = a.swap ? i : lane % 8;
+      const int p = p0 + row, q = q0 + 8 * g + col;
+      if (p < p_end && q < q_end) finish_one(a, a.swap ? q : p, a.swap ? p : q, stage[a.swap ? 33 * i + lane : 9 * row + col]);
+    }
   }
 }
 
 // ---- operands that TMA cannot read ----------------------------------------------------
 
-// The n (0..8) 16-bit elements at p, the others 0, from the one or two
-// aligned 16-byte words that hold them (no other word is read).
-__device__ __forceinline__ uint4 load_chunk(const uint16_t* p, int n) {
-  if (n <= 0) return make_uint4(0, 0, 0, 0);
-  const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
-  const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) - off);
-  const uint4 a = __ldg(s);
-  uint4 b = make_uint4(0, 0, 0, 0);
-  if (off + 2 * n > 16) b = __ldg(s + 1);
+// Eight 16-bit elements that start `off` bytes (even, under 16) into the
+// aligned words a, b.
+__device__ __forceinline__ uint4 realign(uint4 a, uint4 b, uint32_t off) {
   uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   if (off & 8) {
 #pragma unroll
@@ -535,15 +471,31 @@ __device__ __forceinline__ uint4 load_chunk(const uint16_t* p, int n) {
     for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
   }
   const uint32_t sh = (off & 2) * 8;
-  uint32_t o[4];
+  return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh), __funnelshift_r(w[2], w[3], sh),
+                    __funnelshift_r(w[3], w[4], sh));
+}
+// The first n (below 8) of eight elements, the others 0.
+__device__ __forceinline__ uint4 first_of(uint4 v, int n) {
+  uint32_t o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    o[i] = __funnelshift_r(w[i], w[i + 1], sh);
     const int left = n - 2 * i;  // elements of this word that exist
     if (left <= 0) o[i] = 0u;
     else if (left == 1) o[i] &= 0xffffu;
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
+}
+// The n (0..8) 16-bit elements at p, the others 0, from the one or two
+// aligned 16-byte words that hold them (no other word is read).
+__device__ __forceinline__ uint4 load_chunk(const uint16_t* p, int n) {
+  if (n <= 0) return make_uint4(0, 0, 0, 0);
+  const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+  const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) - off);
+  const uint4 a = __ldg(s);
+  uint4 b = make_uint4(0, 0, 0, 0);
+  if (off + 2 * n > 16) b = __ldg(s + 1);
+  const uint4 v = realign(a, b, off);
+  return n < 8 ? first_of(v, n) : v;
 }
 
 // ---- the tensor-core kernel -------------------------------------------------------------
@@ -556,17 +508,19 @@ struct __align__(16) LinearTail {
   uint64_t drained;
   uint32_t tmem_base;
   int abort;
-  float bias[kEpiWarps][128];  // each epilogue warp's columns of a tile, in f32
+  float bias[kEpiWarps][128];            // each epilogue warp's columns of a tile, in f32
+  float stage[kEpiWarps][kStageFloats];  // each epilogue warp's block (finish_block)
 };
 
-// The bias of a warp's 32-column groups c0 = 32 set, + 64, ... (four at most)
-// of the rows from r0 on, into its shared memory; null without a bias.
-__device__ __forceinline__ const float* fetch_bias(const LinearArgs& a, float* mine, int r0, int set, int lane) {
+// The bias of a warp's 32-column groups set, set + sets, ... (four at most) of
+// the rows from r0 on, into its shared memory; null without a bias.
+__device__ __forceinline__ const float* fetch_bias(const LinearArgs& a, float* mine, int r0, int set, int sets,
+                                                   int lane) {
   if (a.bias == nullptr) return nullptr;
   __syncwarp();
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const int r = r0 + 32 * set + 64 * g + lane;
+    const int r = r0 + 32 * (set + sets * g) + lane;
     mine[32 * g + lane] = r < a.rows ? load_f32(a.bias, r, a.bias_dtype) : 0.0f;
   }
   __syncwarp();
@@ -601,6 +555,7 @@ template <bool LOADERS, bool CHUNKED>
 __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     k_linear_mma(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                  const __grid_constant__ LinearArgs a) {
+  constexpr int kEpi = LOADERS ? kLoaderEpiWarps : kEpiWarps, kSets = kEpi / 4;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   unsigned char* ring = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
@@ -617,7 +572,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tail->acc_full[i], 1);
-      mbar_init(&tail->acc_empty[i], kEpiWarps);
+      mbar_init(&tail->acc_empty[i], kEpi);
     }
     mbar_init(&tail->drained, 1);
     tail->abort = 0;
@@ -723,7 +678,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     if (elect_one()) umma_commit(&tail->drained);
     __syncwarp();
     if (!mbar_wait_bounded(&tail->drained, 0, kWaitNs)) give_up(tail);
-  } else if (warp < 2 + kEpiWarps) {
+  } else if (warp < 2 + kEpi) {
     // ---------------- epilogue ----------------
     const int set = (warp - 2) >> 2;
     const int q = warp & 3;  // TMEM lane quarter this warp may read
@@ -740,18 +695,14 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j)
             if (c0 + j < valid) parts[(c0 + j) * kBM + row] = v[j];
-        } else if (w.p0 + row < a.p_rows && c0 < valid) {
-          if (a.swap) finish_column(a, w.q0 + c0, min(32, valid - c0), w.p0 + row, v);
-          else if (a.bn - c0 >= 32) finish_run<32>(a, w.p0 + row, w.q0 + c0, v, bias != nullptr ? bias + c0 / 64 * 32 : nullptr);
-          else {  // the last 16 columns of a tile that is no multiple of 32
-            float h[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) h[j] = v[j];
-            finish_run<16>(a, w.p0 + row, w.q0 + c0, h, bias != nullptr ? bias + c0 / 64 * 32 : nullptr);
-          }
+        } else if (!a.swap && a.vec && c0 + 32 <= valid) {
+          if (w.p0 + row < a.p_rows)
+            finish_run(a, w.p0 + row, w.q0 + c0, v, bias != nullptr ? bias + c0 / (32 * kSets) * 32 : nullptr);
+        } else {
+          finish_block(a, w.p0 + 32 * q, w.q0 + c0, a.p_rows, w.q0 + valid, v, tail->stage[warp - 2], lane);
         }
       };
-      if (!a.swap) bias = fetch_bias(a, tail->bias[warp - 2], w.q0, set, lane);
+      if (!a.swap) bias = fetch_bias(a, tail->bias[warp - 2], w.q0, set, kSets, lane);
       if (!CHUNKED) {
         const int buf = ai & 1;
         const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, kWaitNs);
@@ -760,7 +711,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
           break;
         }
         tc_fence_after();
-        for (int c0 = 32 * set; c0 < a.bn; c0 += 64) {
+        for (int c0 = 32 * set; c0 < a.bn; c0 += 32 * kSets) {
           float v[32];
           tmem_ld32(lane_base + buf * acc_cols + c0, v);
           finish(c0, v);
@@ -770,9 +721,10 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
         if (lane == 0) mbar_arrive(&tail->acc_empty[buf]);
         ++ai;
       } else {
-        float acc[2][32];
+        constexpr int kGroups = LOADERS ? kLoadBn / 32 : 2;  // 32-column groups of this warp
+        float acc[kGroups][32];
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < kGroups; ++g)
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[g][j] = 0.0f;
         bool ok = true;
@@ -786,8 +738,8 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
           }
           tc_fence_after();
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const int c0 = 32 * set + 64 * g;
+          for (int g = 0; g < kGroups; ++g) {
+            const int c0 = 32 * (set + kSets * g);
             if (c0 < a.bn) {
               float v[32];
               tmem_ld32(lane_base + buf * acc_cols + c0, v);
@@ -801,54 +753,115 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
         }
         if (!ok) break;
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const int c0 = 32 * set + 64 * g;
+        for (int g = 0; g < kGroups; ++g) {
+          const int c0 = 32 * (set + kSets * g);
           if (c0 < a.bn) finish(c0, acc[g]);
         }
       }
     }
   } else if (LOADERS) {
     // ---------------- loaders ----------------
-    const int ltid = threadIdx.x - kMmaThreads;
-    const int chunks = (kBM + a.bn) * 8;  // 16-byte chunks of a stage
-    int it = 0;
+    // Each warp serves 24 of a stage's rows.  A row's 64 columns lie in nine
+    // aligned 16-byte words at most; these come into the warp's own buffers
+    // by cp.async, kAhead stages ahead, and are then cut into the operand's
+    // 16-byte chunks.  A stage moves every row on by 128 bytes, so a row's
+    // offset in its words stays the same over a tile.  Words without an
+    // element of the operand are not read (size 0: zeros).
+    const int lw = warp - (2 + kEpi);
+    unsigned char* mine = ring + stages * slot + lw * (kAhead + 1) * kRawBytes;
+    const auto row_at = [&](const Tile& w, int r, bool* there) {
+      const bool side_p = r < kBM;
+      const int grow = side_p ? w.p0 + r : w.q0 + r - kBM;
+      *there = r < kBM + a.bn && grow < (side_p ? a.p_rows : a.q_rows);
+      return reinterpret_cast<uintptr_t>((side_p ? a.p : a.q) +
+                                         (*there ? grow * (side_p ? a.p_stride : a.q_stride) : 0));
+    };
+    // What is being fetched: tile iu, block ik; the lane's word in each step.
+    constexpr int kFetch = (kWarpRows * 9 + 31) / 32, kCut = kWarpRows * 8 / 32;
+    int iu = u0, ik = kb0, issued = 0;
+    uintptr_t word[kFetch];
+    uint32_t word_off = 0u, word_there = 0u;  // 4 bits, 1 bit a step
+    const auto aim = [&]() {
+      const Tile w = tile_of(a, iu);
+      word_off = word_there = 0u;
+#pragma unroll
+      for (int j = 0; j < kFetch; ++j) {
+        const int g = lane + 32 * j;
+        bool there;
+        const uintptr_t at = row_at(w, lw * kWarpRows + g / 9, &there);
+        there = there && g < kWarpRows * 9;
+        word[j] = (at & ~uintptr_t(15)) + 16 * (g % 9);
+        word_off |= static_cast<uint32_t>(at & 15u) << (4 * j);
+        word_there |= static_cast<uint32_t>(there) << j;
+      }
+    };
+    const auto issue = [&]() {
+      if (iu < total && kb0 < kb1) {
+        if (ik == kb0) aim();
+        const int bytes = 2 * min(kBK, a.cols - ik * kBK);  // of a row in this block
+        unsigned char* to = mine + issued % (kAhead + 1) * kRawBytes;
+#pragma unroll
+        for (int j = 0; j < kFetch; ++j) {
+          const int g = lane + 32 * j;
+          const int end = static_cast<int>((word_off >> (4 * j)) & 15u) + bytes;
+          const uint32_t size = ((word_there >> j) & 1u) && 16 * (g % 9) < end ? 16u : 0u;
+          if (g < kWarpRows * 9)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to) + 16 * g),
+                         "l"(word[j] + static_cast<uintptr_t>(ik) * (2 * kBK)), "r"(size)
+                         : "memory");
+        }
+        ++issued;
+        if (++ik == kb1) {
+          ik = kb0;
+          iu += step;
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int st = 0, done = 0;
+    uint32_t phase = 1u;
     bool ok = true;
+    for (int i = 0; i < kAhead; ++i) issue();
     for (int u = u0; ok && u < total; u += step) {
       const Tile w = tile_of(a, u);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int st = it % stages;
-        const bool got = mbar_wait_bounded(&tail->empty[st], ((it / stages) & 1) ^ 1u, kWaitNs) && !gave_up(tail);
-        if (!__all_sync(kAll, got)) {
-          if (lane == 0) give_up(tail);
+      uint32_t cut_off = 0u;
+#pragma unroll
+      for (int j = 0; j < kCut; ++j) {
+        bool there;
+        cut_off |= static_cast<uint32_t>(row_at(w, lw * kWarpRows + (lane + 32 * j) / 8, &there) & 15u) << (4 * j);
+      }
+      for (int kb = kb0; kb < kb1; ++kb) {
+        issue();
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+        __syncwarp();
+        if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, kWaitNs) && !gave_up(tail))) {
+          give_up(tail);
           ok = false;
           break;
         }
-        unsigned char* s = ring + static_cast<size_t>(st) * slot;
-        for (int base = ltid; base < chunks; base += 4 * 32 * kLoadWarps) {
-          uint4 v[4];
+        const unsigned char* from = mine + done % (kAhead + 1) * kRawBytes;
+        unsigned char* s = ring + st * slot;
+        const int count = min(kBK, a.cols - kb * kBK);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int id = base + i * 32 * kLoadWarps;
-            const int r = id >> 3, k = kb * kBK + (id & 7) * 8;
-            const bool side_p = r < kBM;
-            const int grow = side_p ? w.p0 + r : w.q0 + r - kBM;
-            const bool there = id < chunks && grow < (side_p ? a.p_rows : a.q_rows);
-            const uint16_t* src = side_p ? a.p : a.q;
-            const long long stride = side_p ? a.p_stride : a.q_stride;
-            v[i] = load_chunk(src + (there ? grow * stride + k : 0), there ? min(8, a.cols - k) : 0);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int id = base + i * 32 * kLoadWarps;
-            const int r = id >> 3, c = id & 7;
-            // row r of P at slot, row r - 128 of Q at slot + 16 KB: r * 128 either way
-            if (id < chunks) *reinterpret_cast<uint4*>(s + r * 128 + ((c ^ (r & 7)) << 4)) = v[i];
-          }
+        for (int j = 0; j < kCut; ++j) {
+          const int h = lane + 32 * j, c = h & 7, r = lw * kWarpRows + (h >> 3);
+          const uint4* v = reinterpret_cast<const uint4*>(from + (h >> 3) * 144 + c * 16);
+          uint4 o = realign(v[0], v[1], (cut_off >> (4 * j)) & 15u);
+          if (count < kBK) o = first_of(o, count - 8 * c);
+          // row r of P at slot, row r - 128 of Q at slot + 16 KB: r * 128 either way
+          if (r < kBM + a.bn) *reinterpret_cast<uint4*>(s + r * 128 + ((c ^ (r & 7)) << 4)) = o;
         }
         fence_proxy_async_smem();
         mbar_arrive(&tail->full[st]);
+        __syncwarp();  // the buffer has been read before it is filled again
+        ++done;
+        if (++st == stages) {
+          st = 0;
+          phase ^= 1u;
+        }
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
 
   if (a.splits > 1) {
@@ -857,11 +870,11 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     // happened before.)
     __syncwarp();
     cluster_sync_all();
-    if (warp >= 2 && warp < 2 + kEpiWarps && !gave_up(tail)) {
+    if (warp >= 2 && warp < 2 + kEpi && !gave_up(tail)) {
       const Tile w = tile_of(a, u0);
       const int valid = min(a.bn, a.q_rows - w.q0);
       const uint32_t parts = smem_u32(ring);
-      for (int c = rank + (warp - 2) * a.splits; c < valid; c += kEpiWarps * a.splits) {
+      for (int c = rank + (warp - 2) * a.splits; c < valid; c += kEpi * a.splits) {
         const uint32_t at = parts + (c * kBM + 4 * lane) * 4;
         float4 sum = ld_cluster_f4(at, 0);
         for (int r = 1; r < a.splits; ++r) {
@@ -871,8 +884,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
           sum.z = __fadd_rn(sum.z, o.z);
           sum.w = __fadd_rn(sum.w, o.w);
         }
-        float v[4] = {sum.x, sum.y, sum.z, sum.w};
-        if (w.p0 + 4 * lane < a.p_rows) finish_run<4>(a, w.q0 + c, w.p0 + 4 * lane, v);
+        finish_four(a, w.q0 + c, w.p0 + 4 * lane, sum);
       }
     }
     __syncwarp();
@@ -1024,7 +1036,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const int t = w.p0 + static_cast<int>(rank) * kBM + row;
       const int valid = min(a.bn, a.q_rows - w.q0);
       const int buf = ai & 1;
-      const float* bias = fetch_bias(a, tail->bias[warp - 2], w.q0, set, lane);
+      const float* bias = fetch_bias(a, tail->bias[warp - 2], w.q0, set, 2, lane);
       const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, kWaitNs);
       if (!__all_sync(kAll, got)) {
         if (lane == 0) give_up(tail);
@@ -1034,7 +1046,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       for (int c0 = 32 * set; c0 < a.bn; c0 += 64) {
         float v[32];
         tmem_ld32(lane_base + buf * a.bn + c0, v);
-        if (t < a.p_rows && c0 < valid) finish_run<32>(a, t, w.q0 + c0, v, bias != nullptr ? bias + c0 / 64 * 32 : nullptr);
+        if (a.vec && c0 + 32 <= valid) {
+          if (t < a.p_rows) finish_run(a, t, w.q0 + c0, v, bias != nullptr ? bias + c0 / 64 * 32 : nullptr);
+        } else {
+          finish_block(a, t - lane, w.q0 + c0, a.p_rows, w.q0 + valid, v, tail->stage[warp - 2], lane);
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -1129,17 +1145,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) k_linear_rows(const __grid_con
     for (int t = 0; t < NT; ++t)
       for (int s = 1; s < per_row; ++s) acc[t] = __fadd_rn(acc[t], part[warp + s][t]);
   }
-  if (r >= a.rows) return;
+  float mine = acc[0];  // lane t finishes token t
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-    if (lane == t) {
-      float v[1] = {acc[t]};
-      if (a.bias != nullptr) v[0] = __fadd_rn(v[0], load_f32(a.bias, r, a.bias_dtype));
-      activate_all(a.act, v);
-      if (a.residual != nullptr)
-        v[0] = __fadd_rn(v[0], load_f32(a.residual, static_cast<long long>(t) * a.res_stride + r, a.res_dtype));
-      store_f32(a.y, static_cast<long long>(t) * a.y_stride + r, a.out_dtype, v[0]);
-    }
+  for (int t = 1; t < NT; ++t) mine = lane == t ? acc[t] : mine;
+  if (r < a.rows && lane < NT) finish_one(a, lane, r, mine);
 }
 
 // ---- host ------------------------------------------------------------------------------------
@@ -1217,6 +1226,125 @@ cudaError_t launch_rows(const LinearArgs& a, bool aligned, cudaStream_t st) {
   }
 }
 
+// Clusters of each size that the current device runs at once with one CTA per
+// SM (large ones do not fill it: its SMs come in groups of unequal size, and
+// 15 clusters of 7 or 8 is what B200 has room for); asked once per device.
+struct ClusterRoom {
+  int clusters[9] = {};
+};
+cudaError_t cluster_room(int sms, ClusterRoom* out) {
+  static std::mutex mu;
+  static std::map<int, ClusterRoom> known;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  const auto it = known.find(device);
+  if (it != known.end()) {
+    *out = it->second;
+    return cudaSuccess;
+  }
+  constexpr int kSmem = 190 * 1024;
+  const auto kern = k_linear_mma<false, false>;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  ClusterRoom r;
+  r.clusters[1] = sms;
+  for (int size = 2; size <= 8; ++size) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(kMmaThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if ((e = cudaOccupancyMaxActiveClusters(&r.clusters[size], kern, &cfg)) != cudaSuccess) return e;
+  }
+  known.emplace(device, r);
+  *out = r;
+  return cudaSuccess;
+}
+
+// How a product is tiled.
+struct Plan {
+  bool pair = false;  // k_linear_pair
+  bool swap = false;  // w on the M side
+  int bn = 64;        // N tile
+  int splits = 1;     // CTAs that share a tile's columns
+  int ring = 0;       // bytes of the operand ring
+};
+
+// The plan with the shortest estimate, over the tile widths, sides and splits
+// that exist.  A CTA brings 130 bytes per ns into its shared memory (measured;
+// loaders 50), a stage of the pair is bound by its MMAs (270 ns at bn = 256);
+// partial tiles cost 1.2 us and more with their width, the last tile's
+// epilogue in a CTA 0.6 us and 5 ns per column.  The ring is 96 KB, so
+// that the next launch's CTAs can move in beside this one's; 200 KB was no
+// faster but for the pair and for CTAs that run through many tiles.
+// Measured against the best of a sweep (us): 64 x 8192 x 2048 10.5 / 10.5,
+// 128 x 2048 x 2048 8.1 / 8.1, 512 x 2048 x 2048 11.0 / 11.0.
+Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const ClusterRoom& room) {
+  const int kblocks = (a.cols + kBK - 1) / kBK;
+  const double rate = tma ? 130.0 : 50.0;
+  Plan best;
+  double least = 1e30;
+  const auto consider = [&](bool swap, int bn, int splits) {
+    const long long p = swap ? a.rows : a.tokens, q = swap ? a.tokens : a.rows;
+    const long long tiles = ((p + kBM - 1) / kBM) * ((q + bn - 1) / bn);
+    if (splits > 1) {
+      // one wave, and two blocks at least for each CTA
+      if (tiles > room.clusters[splits] || kblocks < 2 * splits) return;
+    }
+    const double waves = static_cast<double>((tiles * splits + sms - 1) / sms);
+    const double stage = (kABytes + 128.0 * bn) / rate;
+    double t = waves * ((kblocks + splits - 1) / splits) * stage + waves * 5.0 * bn + 600.0;
+    if (splits > 1) t += 1200.0 + 10.0 * bn;
+    // direct stores of the swapped epilogue are two bytes wide
+    else if (swap) t += waves * 10.0 * bn;
+    if (t < least) {
+      least = t;
+      best.swap = swap;
+      best.bn = bn;
+      best.splits = splits;
+      best.pair = false;
+      best.ring = (waves > 2 ? 200 : 96) * 1024;
+    }
+  };
+  const int widest = !tma ? kLoadBn : chunked ? 128 : 256;
+  const int tokens16 = (a.tokens + 15) & ~15, rows16 = (a.rows + 15) & ~15;
+  if (a.tokens <= 1024) {
+    for (int bn : {16, 32, 64, 96, 128, 192, 256}) {
+      const int n = std::min(bn, tokens16);
+      if (n > widest) break;
+      for (int s = 1; s <= 8; ++s) consider(true, n, s);
+      if (n < bn) break;
+    }
+  }
+  for (int bn : {64, 128, 256}) {
+    const int n = std::min(bn, rows16);
+    if (n > widest) break;
+    consider(false, n, 1);
+    if (n < bn) break;
+  }
+  if (tma && !chunked && a.tokens > 128 && a.rows > 128) {
+    const long long tiles = static_cast<long long>((a.tokens + 255) / 256) * ((a.rows + 255) / 256);
+    const double waves = static_cast<double>((tiles + sms / 2 - 1) / (sms / 2));
+    const double t = waves * kblocks * 270.0 + 600.0 + 5.0 * 256 * 2;
+    if (t < least) {
+      best.pair = true;
+      best.swap = false;
+      best.bn = 256;
+      best.splits = 1;
+      best.ring = 200 * 1024;
+    }
+  }
+  return best;
+}
+
 }  // namespace
 
 cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_stride, const uint16_t* x,
@@ -1245,32 +1373,12 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
     return a.dtype == kBf16 ? launch_rows<true>(a, al, st) : launch_rows<false>(a, al, st);
   }
 
-  {
-    const long long pairs = static_cast<long long>((a.tokens + 255) / 256) * ((a.rows + 255) / 256);
-    if (pairs >= dev.sms / 2 && a.out_dtype != kF32 && tma_can_read(w, a.rows, w_stride) &&
-        tma_can_read(x, a.tokens, x_stride)) {
-      a.p_rows = a.tokens;
-      a.q_rows = a.rows;
-      a.bn = 256;
-      a.tiles_p = (a.tokens + 255) / 256;
-      a.tiles_q = (a.rows + 255) / 256;
-      a.kblocks = (a.cols + kBK - 1) / kBK;
-      const int slot = kABytes + a.bn / 2 * kBK * 2;
-      a.stages = std::min(kMaxStages, (200 * 1024) / slot);
-      a.ring_bytes = a.stages * slot;
-      a.tmem_cols = 512;
-      CUtensorMap mp = {}, mq = {};
-      if (!operand_map(&mp, x, a.cols, a.p_rows, x_stride, kBM, a.dtype) ||
-          !operand_map(&mq, w, a.cols, a.q_rows, w_stride, a.bn / 2, a.dtype))
-        return cudaErrorInvalidValue;
-      const int grid = 2 * static_cast<int>(std::min<long long>(pairs, dev.sms / 2));
-      return launch(k_linear_pair, grid, kMmaThreads, 1024 + a.ring_bytes + sizeof(LinearTail), 2, st, mp, mq, a);
-    }
-  }
-
-  // Few tokens: w on the M side, all tokens in one N tile, K split over a
-  // cluster until the GPU is full.  Otherwise tokens on the M side.
-  a.swap = a.tokens <= 128;
+  const bool tma = tma_can_read(w, a.rows, w_stride) && tma_can_read(x, a.tokens, x_stride);
+  const bool chunked = a.out_dtype == kF32;
+  ClusterRoom room;
+  if ((e = cluster_room(dev.sms, &room)) != cudaSuccess) return e;
+  const Plan plan = make_plan(a, tma, chunked, dev.sms, room);
+  a.swap = plan.swap;
   const uint16_t* p = a.swap ? w : x;
   const uint16_t* q = a.swap ? x : w;
   a.p = p;
@@ -1279,49 +1387,39 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
   a.q_rows = a.swap ? a.tokens : a.rows;
   a.p_stride = a.swap ? w_stride : x_stride;
   a.q_stride = a.swap ? x_stride : w_stride;
-  const bool chunked = a.out_dtype == kF32;
-  a.bn = std::min(chunked ? 128 : 256, (a.q_rows + 15) & ~15);
-  a.tiles_p = (a.p_rows + kBM - 1) / kBM;
-  if (!a.swap) {
-    // A tile width that leaves the fewest waves' worth of columns idle
-    long long best = -1;
-    for (int bn : {256, 128, 64}) {
-      if (bn > a.bn && bn != 64) continue;
-      const long long tiles = static_cast<long long>(a.tiles_p) * ((a.q_rows + bn - 1) / bn);
-      const long long cost = (tiles + dev.sms - 1) / dev.sms * (bn + 32);  // 32: what a tile costs beside its columns
-      if (best < 0 || cost < best) {
-        best = cost;
-        a.bn = std::min(bn, (a.q_rows + 15) & ~15);
-      }
-    }
-  }
+  a.bn = plan.bn;
+  a.splits = plan.splits;
+  const int height = plan.pair ? 2 * kBM : kBM;
+  a.tiles_p = (a.p_rows + height - 1) / height;
   a.tiles_q = (a.q_rows + a.bn - 1) / a.bn;
   a.kblocks = (a.cols + kBK - 1) / kBK;
-  a.chunk = 4;
-  const long long tiles = static_cast<long long>(a.tiles_p) * a.tiles_q;
-  a.splits = 1;
-  if (a.swap)
-    while (a.splits < 8 && tiles * a.splits * 2 <= dev.sms && a.kblocks >= 4 * a.splits) a.splits *= 2;
-  const int slot = kABytes + a.bn * kBK * 2;
-  a.stages = std::min(kMaxStages, (200 * 1024) / slot);
-  a.ring_bytes = std::max(a.stages * slot, a.splits > 1 ? a.bn * kBM * 4 : 0);
+  a.chunk = kChunk;
+  const int slot = kABytes + (plan.pair ? a.bn / 2 : a.bn) * kBK * 2;
+  a.stages = tma ? std::min(kMaxStages, plan.ring / slot) : kLoadStages;
+  a.ring_bytes = std::max(a.stages * slot + (tma ? 0 : kRawTotal), a.splits > 1 ? a.bn * kBM * 4 : 0);
   int cols = 32;
   while (cols < 2 * ((a.bn + 31) & ~31)) cols *= 2;
   a.tmem_cols = cols;
   const size_t smem = 1024 + a.ring_bytes + sizeof(LinearTail);
-  const int grid = a.splits > 1 ? static_cast<int>(tiles) * a.splits
-                                : static_cast<int>(std::min<long long>(tiles, dev.sms));
+  const long long tiles = static_cast<long long>(a.tiles_p) * a.tiles_q;
 
   CUtensorMap mp = {}, mq = {};
-  const long long ps = a.p_rows == 1 ? (a.cols + 7) / 8 * 8 : a.p_stride;
-  const long long qs = a.q_rows == 1 ? (a.cols + 7) / 8 * 8 : a.q_stride;
-  if (tma_can_read(p, a.p_rows, a.p_stride) && tma_can_read(q, a.q_rows, a.q_stride)) {
+  if (tma) {
+    const long long ps = a.p_rows == 1 ? (a.cols + 7) / 8 * 8 : a.p_stride;
+    const long long qs = a.q_rows == 1 ? (a.cols + 7) / 8 * 8 : a.q_stride;
     if (!operand_map(&mp, p, a.cols, a.p_rows, ps, kBM, a.dtype) ||
-        !operand_map(&mq, q, a.cols, a.q_rows, qs, a.bn, a.dtype))
+        !operand_map(&mq, q, a.cols, a.q_rows, qs, plan.pair ? a.bn / 2 : a.bn, a.dtype))
       return cudaErrorInvalidValue;
+  }
+  if (plan.pair) {
+    const int grid = 2 * static_cast<int>(std::min<long long>(tiles, dev.sms / 2));
+    return launch(k_linear_pair, grid, kMmaThreads, smem, 2, st, mp, mq, a);
+  }
+  const int grid = a.splits > 1 ? static_cast<int>(tiles) * a.splits
+                                : static_cast<int>(std::min<long long>(tiles, dev.sms));
+  if (tma)
     return chunked ? launch(k_linear_mma<false, true>, grid, kMmaThreads, smem, a.splits, st, mp, mq, a)
                    : launch(k_linear_mma<false, false>, grid, kMmaThreads, smem, a.splits, st, mp, mq, a);
-  }
   return chunked ? launch(k_linear_mma<true, true>, grid, kLoaderThreads, smem, a.splits, st, mp, mq, a)
                  : launch(k_linear_mma<true, false>, grid, kLoaderThreads, smem, a.splits, st, mp, mq, a);
 }
