@@ -11,9 +11,10 @@
 //     warp 1      tcgen05.mma kind::f16 into one of two TMEM accumulators
 //     warps 2-9   epilogue, two sets of four (set s takes the 32-column
 //                 groups s, s + 2, ...)
-//     warps 10-17 only where TMA cannot read an operand (a row stride or base
-//                 that is no multiple of 16 bytes): loaders that realign
-//                 16-byte chunks in registers and write the same layout
+//     Where TMA cannot read an operand (a row stride or base that is no
+//     multiple of 16 bytes) warps 6-19 are loaders, which bring the rows into
+//     shared memory by cp.async, realign them in registers and write the same
+//     layout; warps 2-5 are the epilogue then
 //   Few tokens: w is the M side and the K range is split over the CTAs of a
 //   cluster, which exchange their partial tiles through distributed shared
 //   memory and add them in rank order (no workspace, repeatable sums).
@@ -43,16 +44,16 @@ constexpr int kBK = 64;                   // columns per stage (one 128-byte swi
 constexpr int kABytes = kBM * kBK * 2;    // 16 KB
 constexpr int kMaxStages = 8;
 constexpr int kEpiWarps = 8;
-constexpr int kLoadWarps = 8;
-constexpr int kWarpRows = 24;                         // rows of a stage that a loader warp fills
-constexpr int kLoadBn = kLoadWarps * kWarpRows - kBM;  // so N tiles are this wide at most (64)
+constexpr int kLoadWarps = 14;
+constexpr int kWarpRows = 14;              // rows of a stage that a loader warp fills (four words a lane)
+constexpr int kLoadBn = 64;                // N tiles are this wide at most
+static_assert(kLoadWarps * kWarpRows >= kBM + kLoadBn, "every row of a stage has a loader");
 constexpr int kAhead = 3;                             // stages that loaders fetch ahead
-constexpr int kRawBytes = kWarpRows * 144;            // a warp's words of a stage
+constexpr int kRawBytes = (kWarpRows + 2) * 144;      // a warp's words of a stage (whole steps of four rows are read)
 constexpr int kLoadStages = 3;                        // operand stages beside them
 constexpr int kRawTotal = kLoadWarps * (kAhead + 1) * kRawBytes;
 constexpr int kMmaThreads = 32 * (2 + kEpiWarps);
-// With loaders half the epilogue warps: registers for 14 warps, not 18, and
-// N tiles are narrow then.
+// With loaders half the epilogue warps: N tiles are narrow then.
 constexpr int kLoaderEpiWarps = 4;
 constexpr int kLoaderThreads = 32 * (2 + kLoaderEpiWarps + kLoadWarps);
 constexpr int kChunk = 4;  // stages per accumulation for f32 outputs
@@ -433,7 +434,7 @@ __device__ __forceinline__ void finish_four(const LinearArgs& a, int t, int r, f
 }
 // A warp's 32 lanes by 32 columns of a tile from (p0, q0) on, through shared
 // memory eight columns at a time, so that neighbouring lanes have
-// neighbouring outputs and the loop over them stays short code.  swap: lanes
+// neighbouring outputs whatever the sizes, strides and types.  swap: lanes
 // are rows and columns tokens; p_end, q_end: where the tile's end.
 constexpr int kStageFloats = 32 * 9;
 __device__ __forceinline__ void finish_block(const LinearArgs& a, int p0, int q0, int p_end, int q_end,
@@ -447,12 +448,34 @@ __device__ __forceinline__ void finish_block(const LinearArgs& a, int p0, int q0
       stage[a.swap ? 33 * j + lane : 9 * lane + j] = x;
     }
     __syncwarp();
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-      const int row = a.swap ? lane : 4 * i + lane / 8, col = a.swap ? i : lane % 8;
-      const int p = p0 + row, q = q0 + 8 * g + col;
-      if (p < p_end && q < q_end) finish_one(a, a.swap ? q : p, a.swap ? p : q, stage[a.swap ? 33 * i + lane : 9 * row + col]);
+    // The lane's row r of eight tokens t, t + step, ...
+    const int r = a.swap ? p0 + lane : q0 + 8 * g + (lane & 7);
+    const int t = a.swap ? q0 + 8 * g : p0 + (lane >> 3), step = a.swap ? 1 : 4;
+    const int t_end = a.swap ? q_end : p_end;
+    const int at = a.swap ? lane : 9 * (lane >> 3) + (lane & 7), apart = a.swap ? 33 : 36;
+    if (r >= (a.swap ? p_end : q_end)) continue;
+    const float b = a.bias != nullptr ? load_f32(a.bias, r, a.bias_dtype) : 0.0f;
+    F2 p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = pack(stage[at + 2 * i * apart], stage[at + (2 * i + 1) * apart]);
+    if (a.bias != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = add2(p[i], pack(b));
     }
+    activate_pairs<4>(a.act, p);
+    float o[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack(p[i], &o[2 * i], &o[2 * i + 1]);
+    if (a.residual != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (t + i * step < t_end)
+          o[i] = __fadd_rn(o[i], load_f32(a.residual, static_cast<long long>(t + i * step) * a.res_stride + r, a.res_dtype));
+    }
+    const long long first = static_cast<long long>(t) * a.y_stride + r, on = a.y_stride * step;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (t + i * step < t_end) store_f32(a.y, first + i * on, a.out_dtype, o[i]);
   }
 }
 
@@ -567,7 +590,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < stages; ++i) {
-      mbar_init(&tail->full[i], LOADERS ? 32 * kLoadWarps : 1);
+      mbar_init(&tail->full[i], LOADERS ? kLoadWarps : 1);
       mbar_init(&tail->empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -761,7 +784,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     }
   } else if (LOADERS) {
     // ---------------- loaders ----------------
-    // Each warp serves 24 of a stage's rows.  A row's 64 columns lie in nine
+    // Each warp serves kWarpRows of a stage's rows.  A row's 64 columns lie in nine
     // aligned 16-byte words at most; these come into the warp's own buffers
     // by cp.async, kAhead stages ahead, and are then cut into the operand's
     // 16-byte chunks.  A stage moves every row on by 128 bytes, so a row's
@@ -777,13 +800,14 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
                                          (*there ? grow * (side_p ? a.p_stride : a.q_stride) : 0));
     };
     // What is being fetched: tile iu, block ik; the lane's word in each step.
-    constexpr int kFetch = (kWarpRows * 9 + 31) / 32, kCut = kWarpRows * 8 / 32;
+    constexpr int kFetch = (kWarpRows * 9 + 31) / 32, kCut = (kWarpRows * 8 + 31) / 32;
     int iu = u0, ik = kb0, issued = 0;
     uintptr_t word[kFetch];
     uint32_t word_off = 0u, word_there = 0u;  // 4 bits, 1 bit a step
+    uint32_t word_full = 0u;                  // words that hold elements of a whole block
     const auto aim = [&]() {
       const Tile w = tile_of(a, iu);
-      word_off = word_there = 0u;
+      word_off = word_there = word_full = 0u;
 #pragma unroll
       for (int j = 0; j < kFetch; ++j) {
         const int g = lane + 32 * j;
@@ -793,21 +817,31 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
         word[j] = (at & ~uintptr_t(15)) + 16 * (g % 9);
         word_off |= static_cast<uint32_t>(at & 15u) << (4 * j);
         word_there |= static_cast<uint32_t>(there) << j;
+        word_full |= static_cast<uint32_t>(there && (g % 9 < 8 || (at & 15u) != 0)) << j;
       }
     };
     const auto issue = [&]() {
       if (iu < total && kb0 < kb1) {
         if (ik == kb0) aim();
-        const int bytes = 2 * min(kBK, a.cols - ik * kBK);  // of a row in this block
-        unsigned char* to = mine + issued % (kAhead + 1) * kRawBytes;
+        uint32_t read = word_full;
+        if (a.cols - ik * kBK < kBK) {  // the last block: words that start before a row's end
+          const int bytes = 2 * (a.cols - ik * kBK);
+          read = 0u;
+#pragma unroll
+          for (int j = 0; j < kFetch; ++j) {
+            const int end = static_cast<int>((word_off >> (4 * j)) & 15u) + bytes;
+            read |= static_cast<uint32_t>(16 * ((lane + 32 * j) % 9) < end) << j;
+          }
+          read &= word_there;
+        }
+        const uint32_t to = smem_u32(mine) + issued % (kAhead + 1) * kRawBytes + 16 * lane;
+        const uintptr_t on = static_cast<uintptr_t>(ik) * (2 * kBK);
 #pragma unroll
         for (int j = 0; j < kFetch; ++j) {
-          const int g = lane + 32 * j;
-          const int end = static_cast<int>((word_off >> (4 * j)) & 15u) + bytes;
-          const uint32_t size = ((word_there >> j) & 1u) && 16 * (g % 9) < end ? 16u : 0u;
-          if (g < kWarpRows * 9)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to) + 16 * g),
-                         "l"(word[j] + static_cast<uintptr_t>(ik) * (2 * kBK)), "r"(size)
+          const uint32_t size = ((read >> j) & 1u) * 16u;
+          if (lane + 32 * j < kWarpRows * 9)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 512 * j), "l"(word[j] + on),
+                         "r"(size)
                          : "memory");
         }
         ++issued;
@@ -828,7 +862,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
 #pragma unroll
       for (int j = 0; j < kCut; ++j) {
         bool there;
-        cut_off |= static_cast<uint32_t>(row_at(w, lw * kWarpRows + (lane + 32 * j) / 8, &there) & 15u) << (4 * j);
+        cut_off |= static_cast<uint32_t>(row_at(w, lw * kWarpRows + (lane >> 3) + 4 * j, &there) & 15u) << (4 * j);
       }
       for (int kb = kb0; kb < kb1; ++kb) {
         issue();
@@ -839,21 +873,24 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
           ok = false;
           break;
         }
-        const unsigned char* from = mine + done % (kAhead + 1) * kRawBytes;
-        unsigned char* s = ring + st * slot;
-        const int count = min(kBK, a.cols - kb * kBK);
+        // The lane's chunk c of rows r, r + 4, ...: row r of P at slot, row
+        // r - 128 of Q at slot + 16 KB, r * 128 either way, its chunks swapped
+        // by the row's low three bits.
+        const int c = lane & 7, r = lw * kWarpRows + (lane >> 3);
+        const unsigned char* from = mine + done % (kAhead + 1) * kRawBytes + (lane >> 3) * 144 + c * 16;
+        unsigned char* to = ring + st * slot + r * 128;
+        const int count = a.cols - kb * kBK;
 #pragma unroll
         for (int j = 0; j < kCut; ++j) {
-          const int h = lane + 32 * j, c = h & 7, r = lw * kWarpRows + (h >> 3);
-          const uint4* v = reinterpret_cast<const uint4*>(from + (h >> 3) * 144 + c * 16);
+          const uint4* v = reinterpret_cast<const uint4*>(from + 4 * 144 * j);
           uint4 o = realign(v[0], v[1], (cut_off >> (4 * j)) & 15u);
           if (count < kBK) o = first_of(o, count - 8 * c);
-          // row r of P at slot, row r - 128 of Q at slot + 16 KB: r * 128 either way
-          if (r < kBM + a.bn) *reinterpret_cast<uint4*>(s + r * 128 + ((c ^ (r & 7)) << 4)) = o;
+          if ((lane >> 3) + 4 * j < kWarpRows && r + 4 * j < kBM + a.bn)
+            *reinterpret_cast<uint4*>(to + 512 * j + ((c ^ ((r + 4 * j) & 7)) << 4)) = o;
         }
         fence_proxy_async_smem();
-        mbar_arrive(&tail->full[st]);
-        __syncwarp();  // the buffer has been read before it is filled again
+        __syncwarp();  // (and the buffer has been read before it is filled again)
+        if (lane == 0) mbar_arrive(&tail->full[st]);
         ++done;
         if (++st == stages) {
           st = 0;
@@ -1271,6 +1308,7 @@ cudaError_t cluster_room(int sms, ClusterRoom* out) {
 
 // How a product is tiled.
 struct Plan {
+  double ns = 1e30;   // estimate, without the launch
   bool pair = false;  // k_linear_pair
   bool swap = false;  // w on the M side
   int bn = 64;        // N tile
@@ -1280,7 +1318,7 @@ struct Plan {
 
 // The plan with the shortest estimate, over the tile widths, sides and splits
 // that exist.  A CTA brings 130 bytes per ns into its shared memory (measured;
-// loaders 50), a stage of the pair is bound by its MMAs (270 ns at bn = 256);
+// loaders 26), a stage of the pair is bound by its MMAs (270 ns at bn = 256);
 // partial tiles cost 1.2 us and more with their width, the last tile's
 // epilogue in a CTA 0.6 us and 5 ns per column.  The ring is 96 KB, so
 // that the next launch's CTAs can move in beside this one's; 200 KB was no
@@ -1289,9 +1327,8 @@ struct Plan {
 // 128 x 2048 x 2048 8.1 / 8.1, 512 x 2048 x 2048 11.0 / 11.0.
 Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const ClusterRoom& room) {
   const int kblocks = (a.cols + kBK - 1) / kBK;
-  const double rate = tma ? 130.0 : 50.0;
+  const double rate = tma ? 130.0 : 26.0;
   Plan best;
-  double least = 1e30;
   const auto consider = [&](bool swap, int bn, int splits) {
     const long long p = swap ? a.rows : a.tokens, q = swap ? a.tokens : a.rows;
     const long long tiles = ((p + kBM - 1) / kBM) * ((q + bn - 1) / bn);
@@ -1303,10 +1340,9 @@ Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const Clust
     const double stage = (kABytes + 128.0 * bn) / rate;
     double t = waves * ((kblocks + splits - 1) / splits) * stage + waves * 5.0 * bn + 600.0;
     if (splits > 1) t += 1200.0 + 10.0 * bn;
-    // direct stores of the swapped epilogue are two bytes wide
-    else if (swap) t += waves * 10.0 * bn;
-    if (t < least) {
-      least = t;
+    else if (swap) t += waves * 10.0 * bn;  // narrow stores
+    if (t < best.ns) {
+      best.ns = t;
       best.swap = swap;
       best.bn = bn;
       best.splits = splits;
@@ -1334,7 +1370,8 @@ Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const Clust
     const long long tiles = static_cast<long long>((a.tokens + 255) / 256) * ((a.rows + 255) / 256);
     const double waves = static_cast<double>((tiles + sms / 2 - 1) / (sms / 2));
     const double t = waves * kblocks * 270.0 + 600.0 + 5.0 * 256 * 2;
-    if (t < least) {
+    if (t < best.ns) {
+      best.ns = t;
       best.pair = true;
       best.swap = false;
       best.bn = 256;
@@ -1359,7 +1396,19 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
   a.vec = aligned(a.y, a.y_stride, a.out_dtype) && aligned(a.bias, 0, a.bias_dtype) &&
           aligned(a.residual, a.res_stride, a.res_dtype);
 
-  if (a.tokens <= kRowTokens) {
+  const bool tma = tma_can_read(w, a.rows, w_stride) && tma_can_read(x, a.tokens, x_stride);
+  const bool chunked = a.out_dtype == kF32;
+  ClusterRoom room;
+  if ((e = cluster_room(dev.sms, &room)) != cudaSuccess) return e;
+  const Plan plan = make_plan(a, tma, chunked, dev.sms, room);
+  // One to four tokens on the CUDA cores, where that is faster: 2.6 us and
+  // the weights at 5.5 TB/s, slower with every token more, against 4 us and
+  // the plan (measured, one token: 512 x 2048 3.2 and 5.3 us, 2048 x 2048 3.8
+  // and 5.9, 8192 x 2048 9.7 and 7.8; four: 5.5 and 5.4, 6.2 and 5.9, 15 and
+  // 7.8).
+  const double row_ns = 2600.0 + 500.0 * (a.tokens - 1) +
+                        2.0 * a.rows * a.cols / 5500.0 * (0.7 + 0.3 * a.tokens);
+  if (a.tokens <= kRowTokens && row_ns < 4000.0 + plan.ns) {
     a.p = w;
     a.p_stride = w_stride;
     a.q = x;
@@ -1373,11 +1422,6 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
     return a.dtype == kBf16 ? launch_rows<true>(a, al, st) : launch_rows<false>(a, al, st);
   }
 
-  const bool tma = tma_can_read(w, a.rows, w_stride) && tma_can_read(x, a.tokens, x_stride);
-  const bool chunked = a.out_dtype == kF32;
-  ClusterRoom room;
-  if ((e = cluster_room(dev.sms, &room)) != cudaSuccess) return e;
-  const Plan plan = make_plan(a, tma, chunked, dev.sms, room);
   a.swap = plan.swap;
   const uint16_t* p = a.swap ? w : x;
   const uint16_t* q = a.swap ? x : w;
