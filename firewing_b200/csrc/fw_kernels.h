@@ -450,7 +450,7 @@ struct LogprobArgs {
   int tokens, vocab, dtype, targets_per_row, top_k;
   float inv_temperature;
   int splits, part_len;  // set by launch_token_logprobs, as are:
-  float scale, slack, depth;  // log2(e) / temperature; 16 and 20000 over it
+  float scale, depth;    // log2(e) / temperature; 20000 over it
 };
 cudaError_t launch_token_logprobs(LogprobArgs a, cudaStream_t st);
 

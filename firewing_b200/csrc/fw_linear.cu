@@ -26,6 +26,7 @@
 // time-out, lets its copies and MMAs drain (bounded), frees its TMEM and
 // exits; fw_primitive_status reports it.
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <map>
 #include <mutex>
@@ -414,23 +415,35 @@ __device__ __forceinline__ void finish_run(const LinearArgs& a, int t, int r, co
 }
 // Four outputs of token t from row r on (from shared memory's partial sums).
 __device__ __forceinline__ void finish_four(const LinearArgs& a, int t, int r, float4 v) {
-  if (a.vec && a.out_dtype != kF32 && a.residual == nullptr && r + 4 <= a.rows) {
-    F2 p[2] = {pack(v.x, v.y), pack(v.z, v.w)};
-    if (a.bias != nullptr) {
-      p[0] = add2(p[0], pack(load_f32(a.bias, r, a.bias_dtype), load_f32(a.bias, r + 1, a.bias_dtype)));
-      p[1] = add2(p[1], pack(load_f32(a.bias, r + 2, a.bias_dtype), load_f32(a.bias, r + 3, a.bias_dtype)));
-    }
-    activate_pairs<2>(a.act, p);
-    float w[4];
-    unpack(p[0], &w[0], &w[1]);
-    unpack(p[1], &w[2], &w[3]);
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + static_cast<long long>(t) * a.y_stride + r) =
-        make_uint2(pack2(a.out_dtype, w[0], w[1]), pack2(a.out_dtype, w[2], w[3]));
+  const int n = a.rows - r;
+  if (n <= 0) return;
+  F2 p[2] = {pack(v.x, v.y), pack(v.z, v.w)};
+  if (a.bias != nullptr) {
+    float b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = i < n ? load_f32(a.bias, r + i, a.bias_dtype) : 0.0f;
+    p[0] = add2(p[0], pack(b[0], b[1]));
+    p[1] = add2(p[1], pack(b[2], b[3]));
+  }
+  activate_pairs<2>(a.act, p);
+  float o[4];
+  unpack(p[0], &o[0], &o[1]);
+  unpack(p[1], &o[2], &o[3]);
+  if (a.residual != nullptr) {
+    const long long at = static_cast<long long>(t) * a.res_stride + r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) o[i] = __fadd_rn(o[i], load_f32(a.residual, at + i, a.res_dtype));
+  }
+  const long long at = static_cast<long long>(t) * a.y_stride + r;
+  if (a.vec && a.out_dtype != kF32 && n >= 4) {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) =
+        make_uint2(pack2(a.out_dtype, o[0], o[1]), pack2(a.out_dtype, o[2], o[3]));
     return;
   }
-#pragma unroll 1
-  for (int i = 0; i < 4 && r + i < a.rows; ++i)
-    finish_one(a, t, r + i, i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) store_f32(a.y, at + i, a.out_dtype, o[i]);
 }
 // A warp's 32 lanes by 32 columns of a tile from (p0, q0) on, through shared
 // memory eight columns at a time, so that neighbouring lanes have
@@ -1222,13 +1235,23 @@ bool tma_can_read(const void* base, int rows, long long stride) {
   return reinterpret_cast<uintptr_t>(base) % 16 == 0 && (rows == 1 || stride % 8 == 0) && stride < (1ll << 38);
 }
 
-template <typename Kern, typename... Args>
-cudaError_t launch(Kern kern, int grid, int threads, size_t smem, int cluster, cudaStream_t st,
+constexpr int kMostSmem = 227 * 1024;
+
+template <auto Kern, typename... Args>
+cudaError_t launch(int grid, int threads, size_t smem, int cluster, cudaStream_t st,
                    const Args&... args) {
   if (smem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // Once per kernel and device, to the most that any plan asks for.
+    static std::atomic<uint64_t> raised{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
+    const uint64_t bit = device < 64 ? 1ull << device : 0ull;
+    if ((raised.load(std::memory_order_relaxed) & bit) == 0) {
+      e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+      if (e != cudaSuccess) return e;
+      raised.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -1244,14 +1267,14 @@ cudaError_t launch(Kern kern, int grid, int threads, size_t smem, int cluster, c
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
+  return cudaLaunchKernelEx(&cfg, Kern, args...);
 }
 
 template <bool BF16, int NT>
 cudaError_t launch_rows(const LinearArgs& a, bool aligned, cudaStream_t st) {
   const int grid = static_cast<int>((static_cast<long long>(a.rows) * a.splits + kRowWarps - 1) / kRowWarps);
-  return aligned ? launch(k_linear_rows<BF16, NT, true>, grid, 32 * kRowWarps, 0, 1, st, a)
-                 : launch(k_linear_rows<BF16, NT, false>, grid, 32 * kRowWarps, 0, 1, st, a);
+  return aligned ? launch<k_linear_rows<BF16, NT, true>>(grid, 32 * kRowWarps, 0, 1, st, a)
+                 : launch<k_linear_rows<BF16, NT, false>>(grid, 32 * kRowWarps, 0, 1, st, a);
 }
 template <bool BF16>
 cudaError_t launch_rows(const LinearArgs& a, bool aligned, cudaStream_t st) {
@@ -1329,13 +1352,7 @@ Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const Clust
   const int kblocks = (a.cols + kBK - 1) / kBK;
   const double rate = tma ? 130.0 : 26.0;
   Plan best;
-  const auto consider = [&](bool swap, int bn, int splits) {
-    const long long p = swap ? a.rows : a.tokens, q = swap ? a.tokens : a.rows;
-    const long long tiles = ((p + kBM - 1) / kBM) * ((q + bn - 1) / bn);
-    if (splits > 1) {
-      // one wave, and two blocks at least for each CTA
-      if (tiles > room.clusters[splits] || kblocks < 2 * splits) return;
-    }
+  const auto consider = [&](bool swap, int bn, long long tiles, int splits) {
     const double waves = static_cast<double>((tiles * splits + sms - 1) / sms);
     const double stage = (kABytes + 128.0 * bn) / rate;
     double t = waves * ((kblocks + splits - 1) / splits) * stage + waves * 5.0 * bn + 600.0;
@@ -1350,20 +1367,26 @@ Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const Clust
       best.ring = (waves > 2 ? 200 : 96) * 1024;
     }
   };
+  const long long rows128 = (a.rows + kBM - 1) / kBM, tokens128 = (a.tokens + kBM - 1) / kBM;
   const int widest = !tma ? kLoadBn : chunked ? 128 : 256;
   const int tokens16 = (a.tokens + 15) & ~15, rows16 = (a.rows + 15) & ~15;
   if (a.tokens <= 1024) {
     for (int bn : {16, 32, 64, 96, 128, 192, 256}) {
       const int n = std::min(bn, tokens16);
       if (n > widest) break;
-      for (int s = 1; s <= 8; ++s) consider(true, n, s);
+      const long long tiles = rows128 * ((a.tokens + n - 1) / n);
+      consider(true, n, tiles, 1);
+      // The most CTAs to a tile that run in one wave and have two blocks each.
+      int s = std::min(8, kblocks / 2);
+      while (s > 1 && tiles > room.clusters[s]) --s;
+      if (s > 1) consider(true, n, tiles, s);
       if (n < bn) break;
     }
   }
   for (int bn : {64, 128, 256}) {
     const int n = std::min(bn, rows16);
     if (n > widest) break;
-    consider(false, n, 1);
+    consider(false, n, tokens128 * ((a.rows + n - 1) / n), 1);
     if (n < bn) break;
   }
   if (tma && !chunked && a.tokens > 128 && a.rows > 128) {
@@ -1398,17 +1421,21 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
 
   const bool tma = tma_can_read(w, a.rows, w_stride) && tma_can_read(x, a.tokens, x_stride);
   const bool chunked = a.out_dtype == kF32;
-  ClusterRoom room;
-  if ((e = cluster_room(dev.sms, &room)) != cudaSuccess) return e;
-  const Plan plan = make_plan(a, tma, chunked, dev.sms, room);
+  const double row_ns = a.tokens > kRowTokens ? 1e30
+                                              : 2600.0 + 500.0 * (a.tokens - 1) +
+                                                    2.0 * a.rows * a.cols / 5500.0 * (0.7 + 0.3 * a.tokens);
+  Plan plan;
+  if (row_ns > 4000.0) {  // (no plan is faster than that)
+    ClusterRoom room;
+    if ((e = cluster_room(dev.sms, &room)) != cudaSuccess) return e;
+    plan = make_plan(a, tma, chunked, dev.sms, room);
+  }
   // One to four tokens on the CUDA cores, where that is faster: 2.6 us and
   // the weights at 5.5 TB/s, slower with every token more, against 4 us and
   // the plan (measured, one token: 512 x 2048 3.2 and 5.3 us, 2048 x 2048 3.8
   // and 5.9, 8192 x 2048 9.7 and 7.8; four: 5.5 and 5.4, 6.2 and 5.9, 15 and
   // 7.8).
-  const double row_ns = 2600.0 + 500.0 * (a.tokens - 1) +
-                        2.0 * a.rows * a.cols / 5500.0 * (0.7 + 0.3 * a.tokens);
-  if (a.tokens <= kRowTokens && row_ns < 4000.0 + plan.ns) {
+  if (row_ns < 4000.0 + plan.ns) {
     a.p = w;
     a.p_stride = w_stride;
     a.q = x;
@@ -1457,15 +1484,15 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
   }
   if (plan.pair) {
     const int grid = 2 * static_cast<int>(std::min<long long>(tiles, dev.sms / 2));
-    return launch(k_linear_pair, grid, kMmaThreads, smem, 2, st, mp, mq, a);
+    return launch<k_linear_pair>(grid, kMmaThreads, smem, 2, st, mp, mq, a);
   }
   const int grid = a.splits > 1 ? static_cast<int>(tiles) * a.splits
                                 : static_cast<int>(std::min<long long>(tiles, dev.sms));
   if (tma)
-    return chunked ? launch(k_linear_mma<false, true>, grid, kMmaThreads, smem, a.splits, st, mp, mq, a)
-                   : launch(k_linear_mma<false, false>, grid, kMmaThreads, smem, a.splits, st, mp, mq, a);
-  return chunked ? launch(k_linear_mma<true, true>, grid, kLoaderThreads, smem, a.splits, st, mp, mq, a)
-                 : launch(k_linear_mma<true, false>, grid, kLoaderThreads, smem, a.splits, st, mp, mq, a);
+    return chunked ? launch<k_linear_mma<false, true>>(grid, kMmaThreads, smem, a.splits, st, mp, mq, a)
+                   : launch<k_linear_mma<false, false>>(grid, kMmaThreads, smem, a.splits, st, mp, mq, a);
+  return chunked ? launch<k_linear_mma<true, true>>(grid, kLoaderThreads, smem, a.splits, st, mp, mq, a)
+                 : launch<k_linear_mma<true, false>>(grid, kLoaderThreads, smem, a.splits, st, mp, mq, a);
 }
 
 cudaError_t take_linear_status(int* code, cudaStream_t st) {

@@ -9,9 +9,10 @@
 // reference of its own; parts are joined by rescaling.  One pass over the
 // row keeps S, W and the candidates for the alternatives.
 //
-// The reference: each warp takes the maximum of its first batch and changes
-// it only when a later value is over it by kSlack powers of two, which f32
-// sums stand without loss, so that the loop carries no maximum.
+// The reference is the warp's maximum so far: with one far below the row's,
+// log2 S and W / S would be large and nearly equal, and their difference, the
+// entropy, inexact.  It changes about log(batches) times per row, one vote per
+// batch.
 // The alternatives: K values at least are >= `floor` (publish_share), taken from
 // the first batch and raised after 1, 2, 4, ... of them.  Values under it cost
 // one comparison per lane and batch; the few others go to a list in shared
@@ -42,7 +43,6 @@ constexpr int kShares = 64;            // values that make a floor
 constexpr int kSplitWarps = 8;         // warps of the CTAs that share a row
 
 constexpr int kRankMost = 384;         // candidates ranked by counting
-constexpr int kSlackLog2 = 16;         // how far over its reference (log2) a term may be
 constexpr int kMaxTop = 32;
 constexpr int kMaxSplits = 8;          // portable cluster size
 constexpr float kLog2e = 1.4426950408889634f;
@@ -443,14 +443,14 @@ __global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_
   }
 
   if (tid == 0) sm.short_count = sm.merged_count = 0;
-  // The warp's reference M; a value from `limit` on changes it.  With mc =
+  // The warp's reference M, its maximum so far.  With mc =
   // fl(M c) the terms are y = fma(z, c, -mc), which is (z - M) c + off for
   // one small `off` common to the warp: taken out again at the end.  Values
   // are raised to `least`, far enough below M for 2^y to be 0, so that a
   // masked -inf adds 0 * y = 0.  Where the type has no such number (M near
   // its lowest value, or a high temperature), or M c overflows, `plain` terms
   // are computed as max((z - M) c, kLowest).
-  float m = -INFINITY, limit = -INFINITY, mc = 0.0f, least = 0.0f;
+  float m = -INFINITY, mc = 0.0f, least = 0.0f;
   bool plain = false;
   F2 s2 = pack(0.0f, 0.0f), w2 = pack(0.0f, 0.0f);  // the lane's sums, even and odd elements
   float seen = -INFINITY;  // the lane's maximum so far
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_
   };
   // The warp's reference covers `high` (lane maxima).
   auto cover = [&](float high) {
-    if (!__any_sync(kAll, high > limit)) return;
+    if (!__any_sync(kAll, high > m)) return;
     const float to = warp_max(high);
     if (m > -INFINITY) {
       settle();
@@ -476,7 +476,6 @@ __global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_
       s2 = mul2(s2, f);
     }
     m = to;
-    limit = __fadd_rn(to, a.slack);
     mc = __fmul_rn(m, c);
     least = R::at_least(__fsub_rn(m, a.depth));
     plain = !(fabsf(mc) < 1e30f && __fmul_rn(__fsub_rn(least, m), c) < -1000.0f);
@@ -765,7 +764,6 @@ cudaError_t launch_token_logprobs(LogprobArgs a, cudaStream_t st) {
   const cudaError_t e = current_device_attrs(&dev);
   if (e != cudaSuccess) return e;
   a.scale = kLog2e * a.inv_temperature;
-  a.slack = static_cast<float>(kSlackLog2) / a.scale;
   a.depth = 20000.0f / a.scale;
   // Few rows: as many parts as the GPU has room for at once (three CTAs of
   // eight warps per SM), of 4096 values at least.

@@ -459,66 +459,80 @@ def route_bf16(logits, tokens: int, experts: int, top_k: int, indices, scores, s
 
 # ---- primitives over torch tensors: shapes, types and strides are the tensors' own ----
 
+_torch = None  # imported with the first call
 _dtype_codes: dict = {}
+_16_BITS = (DTYPE_BF16, DTYPE_F16)
+_FLOATS = (DTYPE_BF16, DTYPE_F16, DTYPE_F32)
+_INT32 = -1
 
 
-def _codes() -> dict:
-    if not _dtype_codes:
-        import torch
+def _import_torch() -> None:
+    global _torch
+    import torch
 
-        _dtype_codes.update({torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32,
-                             torch.int32: -1})
-    return _dtype_codes
+    _dtype_codes.update({torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32,
+                         torch.int32: _INT32})
+    _torch = torch
 
 
-def _rows(t, name: str, codes: tuple, rows: Optional[int] = None, cols: Optional[int] = None,
-          device: Optional[int] = None):
-    """(pointer, dtype code, rows, cols, row stride) of a 2-D CUDA tensor with
-    unit column stride, after checking it."""
-    if not hasattr(t, "data_ptr") or t.dim() != 2:
-        raise ValueError(f"{name} must be a 2-D tensor")
-    if not t.is_cuda:
+def _rows(t, name: str, codes: tuple, device: int = -1):
+    """(dtype code, rows, columns, row stride, device) of a 2-D CUDA tensor
+    with consecutive columns, after checking it (on `device`, if given)."""
+    try:
+        r, c = t.shape
+        s0, s1 = t.stride()
+        code, dev = _dtype_codes.get(t.dtype), t.get_device()
+    except (AttributeError, ValueError):
+        raise ValueError(f"{name} must be a 2-D tensor") from None
+    if dev < 0:
         raise ValueError(f"{name} must be on a CUDA device")
-    code = _codes().get(t.dtype)
     if code not in codes:
         raise ValueError(f"{name}: unsupported element type {t.dtype}")
-    r, c = t.shape
-    if (rows is not None and r != rows) or (cols is not None and c != cols):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({rows}, {cols})")
-    if device is not None and t.get_device() != device:
+    if dev != device and device >= 0:
         raise ValueError(f"{name} is on another device")
-    s0, s1 = t.stride()
     if s1 != 1 and c > 1:
         raise ValueError(f"{name} must have consecutive columns")
     if r <= 1:
         s0 = c
     elif s0 < c:
         raise ValueError(f"{name} has overlapping rows")
-    return t.data_ptr(), code, r, c, s0
+    return code, r, c, s0, dev
 
 
 def _dense(t, name: str, code: int, shape: tuple, device: int) -> Optional[int]:
     """Pointer of a contiguous CUDA tensor of exactly this shape (None stays None)."""
     if t is None:
         return None
-    if not hasattr(t, "data_ptr") or not t.is_cuda or t.get_device() != device:
-        raise ValueError(f"{name} must be a tensor on the operator's device")
-    if tuple(t.shape) != shape or not t.is_contiguous():
+    try:
+        fits = t.shape == shape and t.is_contiguous()
+        found, dev = _dtype_codes.get(t.dtype), t.get_device()
+    except AttributeError:
+        raise ValueError(f"{name} must be a tensor") from None
+    if dev != device:
+        raise ValueError(f"{name} must be on the operator's device")
+    if not fits:
         raise ValueError(f"{name} must be contiguous with shape {shape}")
-    if _codes().get(t.dtype) != code:
+    if found != code:
         raise ValueError(f"{name}: unsupported element type {t.dtype}")
     return t.data_ptr()
 
 
+def _columns(t, name: str) -> int:
+    try:
+        return t.shape[1] if t.dim() == 2 else -1
+    except (AttributeError, IndexError):
+        raise ValueError(f"{name} must be a 2-D tensor") from None
+
+
 def _call(device: int, function, *args) -> None:
     """The C entry point on `device`, which stays current only for the call."""
-    import torch
-
-    if torch.cuda.current_device() == device:
-        _check(function(*args))
+    if _torch.cuda.current_device() == device:
+        rc = function(*args)
     else:
-        with torch.cuda.device(device):
-            _check(function(*args))
+        with _torch.cuda.device(device):
+            rc = function(*args)
+    if rc != FW_OK:
+        _check(rc)
 
 
 def linear_epilogue(w, x, y, bias=None, activation: str = "none", residual=None, stream=None) -> None:
@@ -530,24 +544,33 @@ def linear_epilogue(w, x, y, bias=None, activation: str = "none", residual=None,
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {tuple(_ACTIVATIONS)}")
-    pw, code, N, K, ws = _rows(w, "w", (DTYPE_BF16, DTYPE_F16))
-    dev = w.get_device()
-    px, _, T, _, xs = _rows(x, "x", (code,), None, K, dev)
-    py, out, _, _, ys = _rows(y, "y", (code, DTYPE_F32), T, N, dev)
+    if _torch is None:
+        _import_torch()
+    code, N, K, ws, dev = _rows(w, "w", _16_BITS)
+    xcode, T, Kx, xs, _ = _rows(x, "x", _16_BITS, dev)
+    out, Ty, Ny, ys, _ = _rows(y, "y", _FLOATS, dev)
+    if xcode != code or Kx != K:
+        raise ValueError(f"x must have w's element type and {K} columns")
+    if Ty != T or Ny != N or (out != code and out != DTYPE_F32):
+        raise ValueError(f"y must have shape ({T}, {N}) and w's element type or float32")
     pb = pr = None
     bcode = rcode = code
     rs = N
     if bias is not None:
-        bcode = _codes().get(bias.dtype, -1)
-        if bcode < 0:
-            raise ValueError(f"bias: unsupported element type {bias.dtype}")
+        bcode = _dtype_codes.get(getattr(bias, "dtype", None), _INT32)
+        if bcode not in _FLOATS:
+            raise ValueError("bias: unsupported element type")
         pb = _dense(bias, "bias", bcode, (N,), dev)
     if residual is not None:
-        pr, rcode, _, _, rs = _rows(residual, "residual", (DTYPE_BF16, DTYPE_F16, DTYPE_F32), T, N, dev)
+        rcode, Tr, Nr, rs, _ = _rows(residual, "residual", _FLOATS, dev)
+        if Tr != T or Nr != N:
+            raise ValueError(f"residual must have shape ({T}, {N})")
+        pr = residual.data_ptr()
     if T == 0:
         return
     c = _LinearConfig(N, K, code, out, bcode, rcode, act, ws, xs, rs, ys)
-    _call(dev, library().fw_linear_epilogue, ctypes.byref(c), pw, px, T, pb, pr, py, _stream(stream))
+    _call(dev, library().fw_linear_epilogue, ctypes.byref(c), w.data_ptr(), x.data_ptr(), T, pb, pr, y.data_ptr(),
+          _stream(stream))
 
 
 def primitive_status(stream=None) -> None:
@@ -568,20 +591,21 @@ def route_scores(logits, indices, weights, scoring: str = "softmax", bias=None, 
     selection and scaled.  `counts` ([E] int32) receives how many tokens
     selected each expert.  Experts at -inf are out; empty places are -1 with
     weight 0."""
-    if scoring not in _SCORES:
+    score = _SCORES.get(scoring)
+    if score is None:
         raise ValueError(f"scoring must be one of {tuple(_SCORES)}")
-    p, code, T, E, stride = _rows(logits, "logits", (DTYPE_BF16, DTYPE_F16, DTYPE_F32))
-    dev = logits.get_device()
-    if not hasattr(indices, "dim") or indices.dim() != 2:
-        raise ValueError("indices must be a 2-D tensor")
-    K = indices.shape[1]
-    args = (_dense(bias, "bias", DTYPE_F32, (E,), dev), _dense(indices, "indices", -1, (T, K), dev),
-            _dense(weights, "weights", DTYPE_F32, (T, K), dev), _dense(counts, "counts", -1, (E,), dev))
+    if _torch is None:
+        _import_torch()
+    code, T, E, stride, dev = _rows(logits, "logits", _FLOATS)
+    K = _columns(indices, "indices")
+    pb = _dense(bias, "bias", DTYPE_F32, (E,), dev)
+    pi = _dense(indices, "indices", _INT32, (T, K), dev)
+    pw = _dense(weights, "weights", DTYPE_F32, (T, K), dev)
+    pc = _dense(counts, "counts", _INT32, (E,), dev)
     if T == 0 and counts is None:
         return
-    c = _RouteConfig(E, K, code, _SCORES[scoring], groups, top_groups, group_top, 1 if renormalize else 0, scale,
-                     stride)
-    _call(dev, library().fw_route_scores, ctypes.byref(c), p, T, *args, _stream(stream))
+    c = _RouteConfig(E, K, code, score, groups, top_groups, group_top, 1 if renormalize else 0, scale, stride)
+    _call(dev, library().fw_route_scores, ctypes.byref(c), logits.data_ptr(), T, pb, pi, pw, pc, _stream(stream))
 
 
 def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_idx=None, top_logprobs=None,
@@ -594,22 +618,27 @@ def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_idx=No
     f32 (a negative target: 0); entropy [T] f32; top_idx [T][K] int32 and
     top_logprobs [T][K] f32, K <= 32, best first.  Leave out what is not
     wanted."""
-    p, code, T, V, stride = _rows(logits, "logits", (DTYPE_BF16, DTYPE_F16, DTYPE_F32))
-    dev = logits.get_device()
     if (targets is None) != (logprobs is None) or (top_idx is None) != (top_logprobs is None):
         raise ValueError("targets and logprobs, top_idx and top_logprobs go together")
-    for t, name in ((targets, "targets"), (top_idx, "top_idx")):
-        if t is not None and (not hasattr(t, "dim") or t.dim() != 2):
-            raise ValueError(f"{name} must be a 2-D tensor")
-    C = 0 if targets is None else targets.shape[1]
-    K = 0 if top_idx is None else top_idx.shape[1]
-    args = (_dense(targets, "targets", -1, (T, C), dev), _dense(logprobs, "logprobs", DTYPE_F32, (T, C), dev),
-            _dense(entropy, "entropy", DTYPE_F32, (T,), dev), _dense(top_idx, "top_idx", -1, (T, K), dev),
-            _dense(top_logprobs, "top_logprobs", DTYPE_F32, (T, K), dev))
+    if _torch is None:
+        _import_torch()
+    code, T, V, stride, dev = _rows(logits, "logits", _FLOATS)
+    C = K = 0
+    pt = pl = pi = pq = None
+    if targets is not None:
+        C = _columns(targets, "targets")
+        pt = _dense(targets, "targets", _INT32, (T, C), dev)
+        pl = _dense(logprobs, "logprobs", DTYPE_F32, (T, C), dev)
+    if top_idx is not None:
+        K = _columns(top_idx, "top_idx")
+        pi = _dense(top_idx, "top_idx", _INT32, (T, K), dev)
+        pq = _dense(top_logprobs, "top_logprobs", DTYPE_F32, (T, K), dev)
+    pe = _dense(entropy, "entropy", DTYPE_F32, (T,), dev)
     if T == 0:
         return
     c = _LogprobConfig(V, code, C, K, temperature, stride)
-    _call(dev, library().fw_token_logprobs, ctypes.byref(c), p, T, *args, _stream(stream))
+    _call(dev, library().fw_token_logprobs, ctypes.byref(c), logits.data_ptr(), T, pt, pl, pe, pi, pq,
+          _stream(stream))
 
 
 def topk_bf16(values: np.ndarray, k: int):

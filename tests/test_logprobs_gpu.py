@@ -60,8 +60,8 @@ def check(z, top_k=0, targets=None, temperature=1.0, seed=0):
         # y itself: the logit's difference, log2(e) / temperature and their
         # product, four roundings
         np.testing.assert_allclose(lp[t], want[ids[t]], rtol=4 * EPS, atol=s + 4 * EPS * 64)
-        # log2 S and W / S each up to log2(vocab) + the reference's slack of 16
-        assert abs(h[t] - want_h) <= 3 * s * (math.log2(V) + 16 + 1)
+        # log2 S and W / S each up to log2(vocab)
+        assert abs(h[t] - want_h) <= 3 * s * (math.log2(V) + 1)
         if top_k:
             order = np.lexsort((np.arange(V), -zz[t]))[:top_k]
             k = int(live[order].sum())
