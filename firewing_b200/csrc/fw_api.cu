@@ -1388,8 +1388,8 @@ int fw_primitive_status(void* stream) {
 int fw_route_scores(const fw_route_config* c, const void* logits, int32_t tokens, const float* bias,
                     int32_t* indices, float* weights, int32_t* counts, void* stream) {
   if (!c || (tokens != 0 && (!logits || !indices || !weights))) return fail(FW_EINVAL, "null argument");
-  if (c->experts < 1 || c->experts > 1024 || c->top_k < 1 || c->top_k > 32 || tokens < 0)
-    return fail(FW_EINVAL, "route_scores: experts 1..1024, top_k 1..32, tokens not negative");
+  if (c->experts < 1 || c->experts > 1024 || c->top_k < 1 || c->top_k > 32 || tokens < 0 || tokens > (1 << 30))
+    return fail(FW_EINVAL, "route_scores: experts 1..1024, top_k 1..32, tokens 0..2^30");
   if (c->groups < 1 || c->groups > 32 || c->experts % c->groups != 0 || c->top_groups < 1 ||
       c->top_groups > c->groups || (c->group_top != 1 && c->group_top != 2) ||
       c->top_k > c->top_groups * (c->experts / c->groups))
@@ -1400,7 +1400,8 @@ int fw_route_scores(const fw_route_config* c, const void* logits, int32_t tokens
     return fail(FW_EINVAL, "route_scores: unknown scoring");
   if (!known_dtype(c->dtype)) return fail(FW_EINVAL, "route_scores: unknown dtype");
   if (!std::isfinite(c->scale)) return fail(FW_EINVAL, "route_scores: scale is not finite");
-  if (c->logit_stride < c->experts) return fail(FW_EINVAL, "route_scores: logit_stride below experts");
+  if (c->logit_stride < c->experts || c->logit_stride > (1ll << 37))
+    return fail(FW_EINVAL, "route_scores: logit_stride below experts or above 2^37");
   if (!aligned_to(logits, dtype_bytes(c->dtype)) || !aligned_to(bias, 4) || !aligned_to(indices, 4) ||
       !aligned_to(weights, 4) || !aligned_to(counts, 4))
     return fail(FW_EINVAL, "route_scores: a buffer is not aligned to its type");
@@ -1430,15 +1431,16 @@ int fw_route_scores(const fw_route_config* c, const void* logits, int32_t tokens
 int fw_token_logprobs(const fw_logprob_config* c, const void* logits, int32_t tokens, const int32_t* targets,
                       float* logprobs, float* entropy, int32_t* top_idx, float* top_logprobs, void* stream) {
   if (!c || (tokens != 0 && !logits)) return fail(FW_EINVAL, "null argument");
-  if (c->vocab < 1 || tokens < 0 || c->targets < 0 || c->targets > 65536)
-    return fail(FW_EINVAL, "token_logprobs: vocab at least 1, tokens not negative, targets 0..65536");
+  if (c->vocab < 1 || c->vocab > (1 << 30) || tokens < 0 || tokens > (1 << 28) || c->targets < 0 ||
+      c->targets > 65536)
+    return fail(FW_EINVAL, "token_logprobs: vocab 1..2^30, tokens 0..2^28, targets 0..65536");
   if (c->top_k < 0 || c->top_k > 32 || c->top_k > c->vocab)
     return fail(FW_EINVAL, "token_logprobs: top_k 0..min(32, vocab)");
-  if (tokens > (1 << 28)) return fail(FW_EINVAL, "token_logprobs: too many tokens");
   if (!known_dtype(c->dtype)) return fail(FW_EINVAL, "token_logprobs: unknown dtype");
   if (!(c->temperature >= 1e-6f && c->temperature <= 1e6f))
     return fail(FW_EINVAL, "token_logprobs: temperature 1e-6..1e6");
-  if (c->logit_stride < c->vocab) return fail(FW_EINVAL, "token_logprobs: logit_stride below vocab");
+  if (c->logit_stride < c->vocab || c->logit_stride > (1ll << 37))
+    return fail(FW_EINVAL, "token_logprobs: logit_stride below vocab or above 2^37");
   if (tokens != 0 &&
       ((c->targets > 0 && (!targets || !logprobs)) || (c->top_k > 0 && (!top_idx || !top_logprobs))))
     return fail(FW_EINVAL, "token_logprobs: targets or alternatives asked for without their buffers");

@@ -28,7 +28,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
-#include <map>
 #include <mutex>
 
 #include <cudaTypedefs.h>
@@ -57,7 +56,11 @@ constexpr int kMmaThreads = 32 * (2 + kEpiWarps);
 // With loaders half the epilogue warps: N tiles are narrow then.
 constexpr int kLoaderEpiWarps = 4;
 constexpr int kLoaderThreads = 32 * (2 + kLoaderEpiWarps + kLoadWarps);
-constexpr int kChunk = 4;  // stages per accumulation for f32 outputs
+// Stages per accumulation for f32 outputs: the tensor cores truncate, which
+// left K = 8192 1.4e-6 off in one accumulation, 4.4e-7 in pieces of 512 columns
+// added in registers (an f32 product on the CUDA cores: 9.6e-7).
+constexpr int kChunk = 8;
+constexpr int kMostSmem = 227 * 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -1235,8 +1238,6 @@ bool tma_can_read(const void* base, int rows, long long stride) {
   return reinterpret_cast<uintptr_t>(base) % 16 == 0 && (rows == 1 || stride % 8 == 0) && stride < (1ll << 38);
 }
 
-constexpr int kMostSmem = 227 * 1024;
-
 template <auto Kern, typename... Args>
 cudaError_t launch(int grid, int threads, size_t smem, int cluster, cudaStream_t st,
                    const Args&... args) {
@@ -1293,38 +1294,36 @@ struct ClusterRoom {
   int clusters[9] = {};
 };
 cudaError_t cluster_room(int sms, ClusterRoom* out) {
+  constexpr int kDevices = 64;
   static std::mutex mu;
-  static std::map<int, ClusterRoom> known;
+  static ClusterRoom known[kDevices];  // clusters[1] is set last
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
+  if (device >= kDevices) return cudaErrorInvalidDevice;
   std::lock_guard<std::mutex> lock(mu);
-  const auto it = known.find(device);
-  if (it != known.end()) {
-    *out = it->second;
-    return cudaSuccess;
+  ClusterRoom& r = known[device];
+  if (r.clusters[1] == 0) {
+    constexpr int kSmem = 190 * 1024;
+    const auto kern = k_linear_mma<false, false>;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+    if (e != cudaSuccess) return e;
+    for (int size = 2; size <= 8; ++size) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(size);
+      cfg.blockDim = dim3(kMmaThreads);
+      cfg.dynamicSmemBytes = kSmem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = size;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if ((e = cudaOccupancyMaxActiveClusters(&r.clusters[size], kern, &cfg)) != cudaSuccess) return e;
+    }
+    r.clusters[1] = sms;
   }
-  constexpr int kSmem = 190 * 1024;
-  const auto kern = k_linear_mma<false, false>;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (e != cudaSuccess) return e;
-  ClusterRoom r;
-  r.clusters[1] = sms;
-  for (int size = 2; size <= 8; ++size) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(size);
-    cfg.blockDim = dim3(kMmaThreads);
-    cfg.dynamicSmemBytes = kSmem;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = size;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if ((e = cudaOccupancyMaxActiveClusters(&r.clusters[size], kern, &cfg)) != cudaSuccess) return e;
-  }
-  known.emplace(device, r);
   *out = r;
   return cudaSuccess;
 }
@@ -1468,8 +1467,14 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
   const int slot = kABytes + (plan.pair ? a.bn / 2 : a.bn) * kBK * 2;
   a.stages = tma ? std::min(kMaxStages, plan.ring / slot) : kLoadStages;
   a.ring_bytes = std::max(a.stages * slot + (tma ? 0 : kRawTotal), a.splits > 1 ? a.bn * kBM * 4 : 0);
+  // Two accumulators, but one where a CTA has one tile and one accumulation.
+  // CTAs of a cluster wait for one another while they hold TMEM: with at most
+  // 256 of the 512 columns each, and shared memory for two per SM, no two
+  // clusters on two streams can each hold what the other one needs.  (The
+  // pair kernel takes all columns, and an SM to itself.)
+  const bool single = a.splits > 1 && !chunked;
   int cols = 32;
-  while (cols < 2 * ((a.bn + 31) & ~31)) cols *= 2;
+  while (cols < (single ? 1 : 2) * ((a.bn + 31) & ~31)) cols *= 2;
   a.tmem_cols = cols;
   const size_t smem = 1024 + a.ring_bytes + sizeof(LinearTail);
   const long long tiles = static_cast<long long>(a.tiles_p) * a.tiles_q;

@@ -397,8 +397,9 @@ int fw_route_bf16(const uint16_t* logits, int32_t tokens, int32_t experts, int32
  * -1 and weight NaN throughout.
  * 1 <= experts <= 1024; 1 <= top_k <= 32; 1 <= groups <= 32 dividing
  * experts; 1 <= top_groups <= groups; top_k <= top_groups * experts/groups;
- * scale finite.  Device pointers of the current device; outputs must not
- * overlap inputs.  FW_EINVAL otherwise; tokens = 0 only clears counts. */
+ * scale finite; 0 <= tokens <= 2^30.  Device pointers of the current device;
+ * outputs must not overlap inputs.  FW_EINVAL otherwise; tokens = 0 only
+ * clears counts. */
 #define FW_SCORE_SOFTMAX 0
 #define FW_SCORE_SIGMOID 1
 typedef struct fw_route_config {
@@ -431,9 +432,9 @@ int fw_route_scores(const fw_route_config* config, const void* logits, int32_t t
  * alternatives is -1 with -inf).  A row of nothing but -inf has -inf, entropy
  * 0 and no alternatives; a row with a NaN or +inf has NaN throughout and
  * alternatives -1.
- * vocab >= 1; 0 <= targets <= 65536; 0 <= top_k <= min(32, vocab);
- * temperature positive, at least 1e-6 and at most 1e6.  Device pointers of
- * the current device, logits aligned to their type; outputs must not overlap
+ * 1 <= vocab <= 2^30; 0 <= tokens <= 2^28; 0 <= targets <= 65536;
+ * 0 <= top_k <= min(32, vocab); temperature 1e-6 to 1e6.  Device pointers of
+ * the current device, aligned to their types; outputs must not overlap
  * inputs.  FW_EINVAL otherwise. */
 typedef struct fw_logprob_config {
     int32_t vocab;

@@ -26,7 +26,7 @@ def route(**kw):
     dict(top_groups=1, top_k=9), dict(scoring=2), dict(dtype=3), dict(dtype=-1), dict(scale=float("nan")),
     dict(scale=float("inf")), dict(logit_stride=63), dict(tokens=-1), dict(logits=None), dict(indices=None),
     dict(weights=None), dict(logits=FAKE + 2), dict(bias=FAKE + 1), dict(indices=FAKE + 2), dict(weights=FAKE + 2),
-    dict(counts=FAKE + 2), dict(dtype=0, logits=FAKE + 1)])
+    dict(counts=FAKE + 2), dict(dtype=0, logits=FAKE + 1), dict(tokens=(1 << 30) + 1), dict(logit_stride=1 << 38)])
 def test_route_scores_refusals(bad):
     assert route(**bad) == fw.FW_EINVAL
     assert fw.library().fw_last_error()
@@ -52,7 +52,8 @@ def logprobs(**kw):
     dict(temperature=1e-7), dict(temperature=1e7), dict(logit_stride=99), dict(tokens=-1), dict(logits=None),
     dict(ids=None), dict(logprobs=None), dict(top_idx=None), dict(top_logprobs=None), dict(logits=FAKE + 1),
     dict(ids=FAKE + 2), dict(logprobs=FAKE + 2), dict(entropy=FAKE + 2), dict(top_idx=FAKE + 1),
-    dict(top_logprobs=FAKE + 3), dict(targets=0, top_k=0, entropy=None), dict(tokens=1 << 30)])
+    dict(top_logprobs=FAKE + 3), dict(targets=0, top_k=0, entropy=None), dict(tokens=1 << 30),
+    dict(vocab=(1 << 30) + 1, logit_stride=1 << 31), dict(logit_stride=1 << 38)])
 def test_token_logprobs_refusals(bad):
     assert logprobs(**bad) == fw.FW_EINVAL
     assert fw.library().fw_last_error()
