@@ -45,11 +45,15 @@ constexpr int kABytes = kBM * kBK * 2;    // 16 KB
 constexpr int kMaxStages = 8;
 constexpr int kEpiWarps = 8;
 constexpr int kLoadWarps = 14;
-constexpr int kWarpRows = 14;              // rows of a stage that a loader warp fills (four words a lane)
+// The loaders are two groups that take turns at stages: what a warp waits for
+// in a stage (its words, the slot, the fence) would otherwise bound it.
+constexpr int kLoadGroups = 2;
+constexpr int kGroupWarps = kLoadWarps / kLoadGroups;
+constexpr int kWarpRows = 28;              // rows of a stage that a loader warp fills
 constexpr int kLoadBn = 64;                // N tiles are this wide at most
-static_assert(kLoadWarps * kWarpRows >= kBM + kLoadBn, "every row of a stage has a loader");
-constexpr int kAhead = 3;                             // stages that loaders fetch ahead
-constexpr int kRawBytes = (kWarpRows + 2) * 144;      // a warp's words of a stage (whole steps of four rows are read)
+static_assert(kGroupWarps * kWarpRows >= kBM + kLoadBn, "every row of a stage has a loader");
+constexpr int kAhead = 1;                             // stages of its own that a group fetches ahead
+constexpr int kRawBytes = kWarpRows * 144;            // a warp's words of a stage
 constexpr int kLoadStages = 3;                        // operand stages beside them
 constexpr int kRawTotal = kLoadWarps * (kAhead + 1) * kRawBytes;
 constexpr int kMmaThreads = 32 * (2 + kEpiWarps);
@@ -606,7 +610,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < stages; ++i) {
-      mbar_init(&tail->full[i], LOADERS ? kLoadWarps : 1);
+      mbar_init(&tail->full[i], LOADERS ? kGroupWarps : 1);
       mbar_init(&tail->empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -806,8 +810,16 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     // 16-byte chunks.  A stage moves every row on by 128 bytes, so a row's
     // offset in its words stays the same over a tile.  Words without an
     // element of the operand are not read (size 0: zeros).
-    const int lw = warp - (2 + kEpi);
-    unsigned char* mine = ring + stages * slot + lw * (kAhead + 1) * kRawBytes;
+    const int group = (warp - (2 + kEpi)) / kGroupWarps, lw = (warp - (2 + kEpi)) % kGroupWarps;
+    unsigned char* mine = ring + stages * slot + (warp - (2 + kEpi)) * (kAhead + 1) * kRawBytes;
+    // The stage after the next one of the other group.
+    const auto advance = [&](int* u, int* kb, int by) {
+      for (int i = 0; i < by; ++i)
+        if (++*kb == kb1) {
+          *kb = kb0;
+          *u += step;
+        }
+    };
     const auto row_at = [&](const Tile& w, int r, bool* there) {
       const bool side_p = r < kBM;
       const int grow = side_p ? w.p0 + r : w.q0 + r - kBM;
@@ -817,7 +829,8 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     };
     // What is being fetched: tile iu, block ik; the lane's word in each step.
     constexpr int kFetch = (kWarpRows * 9 + 31) / 32, kCut = (kWarpRows * 8 + 31) / 32;
-    int iu = u0, ik = kb0, issued = 0;
+    int iu = u0, ik = kb0, issued = 0, aimed = -1;
+    advance(&iu, &ik, group);
     uintptr_t word[kFetch];
     uint32_t word_off = 0u, word_there = 0u;  // 4 bits, 1 bit a step
     uint32_t word_full = 0u;                  // words that hold elements of a whole block
@@ -837,8 +850,9 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
       }
     };
     const auto issue = [&]() {
-      if (iu < total && kb0 < kb1) {
-        if (ik == kb0) aim();
+      if (iu < total) {
+        if (iu != aimed) aim();
+        aimed = iu;
         uint32_t read = word_full;
         if (a.cols - ik * kBK < kBK) {  // the last block: words that start before a row's end
           const int bytes = 2 * (a.cols - ik * kBK);
@@ -861,58 +875,57 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
                          : "memory");
         }
         ++issued;
-        if (++ik == kb1) {
-          ik = kb0;
-          iu += step;
-        }
+        advance(&iu, &ik, kLoadGroups);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    int st = 0, done = 0;
-    uint32_t phase = 1u;
-    bool ok = true;
+    int u = u0, kb = kb0, st = group, done = 0, cut = -1;
+    uint32_t phase = 1u, cut_off = 0u;
+    advance(&u, &kb, group);
     for (int i = 0; i < kAhead; ++i) issue();
-    for (int u = u0; ok && u < total; u += step) {
-      const Tile w = tile_of(a, u);
-      uint32_t cut_off = 0u;
-#pragma unroll
-      for (int j = 0; j < kCut; ++j) {
-        bool there;
-        cut_off |= static_cast<uint32_t>(row_at(w, lw * kWarpRows + (lane >> 3) + 4 * j, &there) & 15u) << (4 * j);
-      }
-      for (int kb = kb0; kb < kb1; ++kb) {
-        issue();
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
-        __syncwarp();
-        if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, kWaitNs) && !gave_up(tail))) {
-          give_up(tail);
-          ok = false;
-          break;
-        }
-        // The lane's chunk c of rows r, r + 4, ...: row r of P at slot, row
-        // r - 128 of Q at slot + 16 KB, r * 128 either way, its chunks swapped
-        // by the row's low three bits.
-        const int c = lane & 7, r = lw * kWarpRows + (lane >> 3);
-        const unsigned char* from = mine + done % (kAhead + 1) * kRawBytes + (lane >> 3) * 144 + c * 16;
-        unsigned char* to = ring + st * slot + r * 128;
-        const int count = a.cols - kb * kBK;
+    while (u < total) {
+      if (u != cut) {
+        const Tile w = tile_of(a, u);
+        cut = u;
+        cut_off = 0u;
 #pragma unroll
         for (int j = 0; j < kCut; ++j) {
-          const uint4* v = reinterpret_cast<const uint4*>(from + 4 * 144 * j);
-          uint4 o = realign(v[0], v[1], (cut_off >> (4 * j)) & 15u);
-          if (count < kBK) o = first_of(o, count - 8 * c);
-          if ((lane >> 3) + 4 * j < kWarpRows && r + 4 * j < kBM + a.bn)
-            *reinterpret_cast<uint4*>(to + 512 * j + ((c ^ ((r + 4 * j) & 7)) << 4)) = o;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();  // (and the buffer has been read before it is filled again)
-        if (lane == 0) mbar_arrive(&tail->full[st]);
-        ++done;
-        if (++st == stages) {
-          st = 0;
-          phase ^= 1u;
+          bool there;
+          cut_off |= static_cast<uint32_t>(row_at(w, lw * kWarpRows + (lane >> 3) + 4 * j, &there) & 15u) << (4 * j);
         }
       }
+      issue();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+      __syncwarp();
+      if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, kWaitNs) && !gave_up(tail))) {
+        give_up(tail);
+        break;
+      }
+      // The lane's chunk c of rows r, r + 4, ...: row r of P at slot, row
+      // r - 128 of Q at slot + 16 KB, r * 128 either way, its chunks swapped
+      // by the row's low three bits.
+      const int c = lane & 7, r = lw * kWarpRows + (lane >> 3);
+      const unsigned char* from = mine + done % (kAhead + 1) * kRawBytes + (lane >> 3) * 144 + c * 16;
+      unsigned char* to = ring + st * slot + r * 128;
+      const int count = a.cols - kb * kBK;
+#pragma unroll
+      for (int j = 0; j < kCut; ++j) {
+        const uint4* v = reinterpret_cast<const uint4*>(from + 4 * 144 * j);
+        uint4 o = realign(v[0], v[1], (cut_off >> (4 * j)) & 15u);
+        if (count < kBK) o = first_of(o, count - 8 * c);
+        if ((lane >> 3) + 4 * j < kWarpRows && r + 4 * j < kBM + a.bn)
+          *reinterpret_cast<uint4*>(to + 512 * j + ((c ^ ((r + 4 * j) & 7)) << 4)) = o;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();  // (and the buffer has been read before it is filled again)
+      if (lane == 0) mbar_arrive(&tail->full[st]);
+      ++done;
+      st += kLoadGroups;
+      if (st >= stages) {
+        st -= stages;
+        phase ^= 1u;
+      }
+      advance(&u, &kb, kLoadGroups);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
@@ -923,11 +936,11 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     // happened before.)
     __syncwarp();
     cluster_sync_all();
-    if (warp >= 2 && warp < 2 + kEpi && !gave_up(tail)) {
+    if (!gave_up(tail)) {  // all warps: the roles are over
       const Tile w = tile_of(a, u0);
       const int valid = min(a.bn, a.q_rows - w.q0);
       const uint32_t parts = smem_u32(ring);
-      for (int c = rank + (warp - 2) * a.splits; c < valid; c += kEpi * a.splits) {
+      for (int c = rank + warp * a.splits; c < valid; c += static_cast<int>(blockDim.x >> 5) * a.splits) {
         const uint32_t at = parts + (c * kBM + 4 * lane) * 4;
         float4 sum = ld_cluster_f4(at, 0);
         for (int r = 1; r < a.splits; ++r) {
