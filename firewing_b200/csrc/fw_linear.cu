@@ -420,6 +420,78 @@ __device__ __forceinline__ void finish_run(const LinearArgs& a, int t, int r, co
   if (a.residual != nullptr) add_vec<16>(a.residual, static_cast<long long>(t) * a.res_stride + r, a.res_dtype, p);
   store_pairs<16>(a.y, static_cast<long long>(t) * a.y_stride + r, a.out_dtype, p);
 }
+// finish_run for a whole warp's 32 tokens t0 + lane, 16-bit outputs.  A
+// lane's 64 bytes lie a row's stride from its neighbour's, so they change
+// hands in shared memory (`stage`, 2 KB; 16-byte chunks swapped by the row so
+// that both sides are free of bank conflicts): a store then covers eight
+// tokens' 64 bytes each instead of 16 bytes of 32 tokens, and a 16-bit
+// residual comes in the same way.
+constexpr int kRowBytes = 64;
+__device__ __forceinline__ void finish_warp(const LinearArgs& a, int t0, int t_end, int r, const float (&v)[32],
+                                            const float* bias, unsigned char* stage, int lane) {
+  const auto chunk = [&](int row, int c) {
+    return reinterpret_cast<uint4*>(stage + row * kRowBytes + ((c ^ ((row >> 1) & 3)) << 4));
+  };
+  const int row8 = lane >> 2, c4 = lane & 3;  // of a pass over eight tokens
+  const bool moved = a.residual != nullptr && a.res_dtype != kF32;
+  __syncwarp();
+  if (moved) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = t0 + 8 * i + row8;
+      if (t < t_end)
+        *chunk(8 * i + row8, c4) = *reinterpret_cast<const uint4*>(
+            static_cast<const uint16_t*>(a.residual) + static_cast<long long>(t) * a.res_stride + r + 8 * c4);
+    }
+    __syncwarp();
+  }
+  F2 p[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) p[j] = pack(v[2 * j], v[2 * j + 1]);
+  if (bias != nullptr) add_vec<16>(bias, 0, kF32, p);
+  activate_pairs<16>(a.act, p);
+  if (moved) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint4 u = *chunk(lane, c);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float lo, hi;
+        unpack2(a.res_dtype, w[k], &lo, &hi);
+        p[4 * c + k] = add2(p[4 * c + k], pack(lo, hi));
+      }
+    }
+  } else if (a.residual != nullptr && t0 + lane < t_end) {
+    add_vec<16>(a.residual, static_cast<long long>(t0 + lane) * a.res_stride + r, a.res_dtype, p);
+  }
+  uint32_t w[16];
+  if (a.out_dtype == kBf16) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float lo, hi;
+      unpack(p[j], &lo, &hi);
+      w[j] = pack2(kBf16, lo, hi);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float lo, hi;
+      unpack(p[j], &lo, &hi);
+      w[j] = pack2(kF16, lo, hi);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) *chunk(lane, c) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = t0 + 8 * i + row8;
+    if (t < t_end)
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + static_cast<long long>(t) * a.y_stride + r + 8 * c4) =
+          *chunk(8 * i + row8, c4);
+  }
+}
 // Four outputs of token t from row r on (from shared memory's partial sums).
 __device__ __forceinline__ void finish_four(const LinearArgs& a, int t, int r, float4 v) {
   const int n = a.rows - r;
@@ -543,7 +615,7 @@ __device__ __forceinline__ uint4 load_chunk(const uint16_t* p, int n) {
 
 // ---- the tensor-core kernel -------------------------------------------------------------
 
-struct __align__(16) LinearTail {
+struct __align__(128) LinearTail {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
   uint64_t acc_full[2];
@@ -552,8 +624,11 @@ struct __align__(16) LinearTail {
   uint32_t tmem_base;
   int abort;
   float bias[kEpiWarps][128];            // each epilogue warp's columns of a tile, in f32
-  float stage[kEpiWarps][kStageFloats];  // each epilogue warp's block (finish_block)
 };
+// Behind the tail: each epilogue warp's memory for finish_block (kStageFloats)
+// or, in the pair kernel, finish_warp.
+constexpr int kPairStageBytes = 32 * kRowBytes;
+static_assert(kPairStageBytes >= 4 * kStageFloats, "finish_block fits too");
 
 // The bias of a warp's 32-column groups set, set + sets, ... (four at most) of
 // the rows from r0 on, into its shared memory; null without a bias.
@@ -742,7 +817,8 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
           if (w.p0 + row < a.p_rows)
             finish_run(a, w.p0 + row, w.q0 + c0, v, bias != nullptr ? bias + c0 / (32 * kSets) * 32 : nullptr);
         } else {
-          finish_block(a, w.p0 + 32 * q, w.q0 + c0, a.p_rows, w.q0 + valid, v, tail->stage[warp - 2], lane);
+          finish_block(a, w.p0 + 32 * q, w.q0 + c0, a.p_rows, w.q0 + valid, v,
+                       reinterpret_cast<float*>(tail + 1) + (warp - 2) * kStageFloats, lane);
         }
       };
       if (!a.swap) bias = fetch_bias(a, tail->bias[warp - 2], w.q0, set, kSets, lane);
@@ -1094,12 +1170,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     // ---------------- epilogue ----------------
     const int set = (warp - 2) >> 2;
     const int q = warp & 3;
-    const int row = q * 32 + lane;
+    unsigned char* stage = reinterpret_cast<unsigned char*>(tail + 1) + (warp - 2) * kPairStageBytes;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
     int ai = 0;
     for (int u = u0; u < total; u += step, ++ai) {
       const Tile w = tile_of(a, u, 2 * kBM);
-      const int t = w.p0 + static_cast<int>(rank) * kBM + row;
+      const int t0 = w.p0 + static_cast<int>(rank) * kBM + 32 * q;  // this warp's tokens
       const int valid = min(a.bn, a.q_rows - w.q0);
       const int buf = ai & 1;
       const float* bias = fetch_bias(a, tail->bias[warp - 2], w.q0, set, 2, lane);
@@ -1112,11 +1188,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       for (int c0 = 32 * set; c0 < a.bn; c0 += 64) {
         float v[32];
         tmem_ld32(lane_base + buf * a.bn + c0, v);
-        if (a.vec && c0 + 32 <= valid) {
-          if (t < a.p_rows) finish_run(a, t, w.q0 + c0, v, bias != nullptr ? bias + c0 / 64 * 32 : nullptr);
-        } else {
-          finish_block(a, t - lane, w.q0 + c0, a.p_rows, w.q0 + valid, v, tail->stage[warp - 2], lane);
-        }
+        if (a.vec && c0 + 32 <= valid)
+          finish_warp(a, t0, a.p_rows, w.q0 + c0, v, bias != nullptr ? bias + c0 / 64 * 32 : nullptr, stage, lane);
+        else
+          finish_block(a, t0, w.q0 + c0, a.p_rows, w.q0 + valid, v, reinterpret_cast<float*>(stage), lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -1489,7 +1564,8 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
   int cols = 32;
   while (cols < (single ? 1 : 2) * ((a.bn + 31) & ~31)) cols *= 2;
   a.tmem_cols = cols;
-  const size_t smem = 1024 + a.ring_bytes + sizeof(LinearTail);
+  const size_t smem = 1024 + a.ring_bytes + sizeof(LinearTail) +
+                      kEpiWarps * (plan.pair ? kPairStageBytes : sizeof(float) * kStageFloats);
   const long long tiles = static_cast<long long>(a.tiles_p) * a.tiles_q;
 
   CUtensorMap mp = {}, mq = {};
