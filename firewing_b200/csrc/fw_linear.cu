@@ -492,17 +492,15 @@ __device__ __forceinline__ void finish_warp(const LinearArgs& a, int t0, int t_e
           *chunk(8 * i + row8, c4);
   }
 }
-// Four outputs of token t from row r on (from shared memory's partial sums).
-__device__ __forceinline__ void finish_four(const LinearArgs& a, int t, int r, float4 v) {
+// Four outputs of token t from row r on (from shared memory's partial sums),
+// `b` their bias.
+__device__ __forceinline__ void finish_four(const LinearArgs& a, int t, int r, float4 v, const F2 (&b)[2]) {
   const int n = a.rows - r;
   if (n <= 0) return;
   F2 p[2] = {pack(v.x, v.y), pack(v.z, v.w)};
   if (a.bias != nullptr) {
-    float b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = i < n ? load_f32(a.bias, r + i, a.bias_dtype) : 0.0f;
-    p[0] = add2(p[0], pack(b[0], b[1]));
-    p[1] = add2(p[1], pack(b[2], b[3]));
+    p[0] = add2(p[0], b[0]);
+    p[1] = add2(p[1], b[1]);
   }
   activate_pairs<2>(a.act, p);
   float o[4];
@@ -1010,10 +1008,21 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     // Partial tiles lie in the CTAs' rings; CTA r adds up columns r,
     // r + splits, ... in rank order.  (Every thread comes here, whatever
     // happened before.)
+    const Tile w = tile_of(a, u0);
+    F2 bias[2] = {pack(0.0f), pack(0.0f)};  // of the lane's four rows, on its way during the barrier
+    if (a.bias != nullptr) {
+      float b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = w.p0 + 4 * lane + i;
+        b[i] = r < a.rows ? load_f32(a.bias, r, a.bias_dtype) : 0.0f;
+      }
+      bias[0] = pack(b[0], b[1]);
+      bias[1] = pack(b[2], b[3]);
+    }
     __syncwarp();
     cluster_sync_all();
     if (!gave_up(tail)) {  // all warps: the roles are over
-      const Tile w = tile_of(a, u0);
       const int valid = min(a.bn, a.q_rows - w.q0);
       const uint32_t parts = smem_u32(ring);
       for (int c = rank + warp * a.splits; c < valid; c += static_cast<int>(blockDim.x >> 5) * a.splits) {
@@ -1026,7 +1035,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
           sum.z = __fadd_rn(sum.z, o.z);
           sum.w = __fadd_rn(sum.w, o.w);
         }
-        finish_four(a, w.q0 + c, w.p0 + 4 * lane, sum);
+        finish_four(a, w.q0 + c, w.p0 + 4 * lane, sum, bias);
       }
     }
     __syncwarp();
