@@ -27,17 +27,17 @@ namespace fw {
 namespace {
 
 constexpr int kRouteWarps = 4;     // tokens per CTA
-constexpr int kRouteResident = 4;  // CTAs per SM (half as many with more than 512 experts)
+constexpr int kRouteResident = 7;  // CTAs per SM (half as many with more than 512 experts)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.402823466e38f;  // below it a key is dead
 constexpr unsigned kAll = 0xffffffffu;
 
 // Bounds of the f32 scores' errors.  z * log2(e) is off by 2^-23.4 |z log2 e|,
 // ex2.approx by 2^-22 relative; for the sigmoid both reach s scaled by
-// s (1 - s) (at most 1/4, and 0.224 / |z|), 1 + t adds 2^-24 and the quotient
-// 2^-22: under 2^-21.3 in all.  For the softmax the sum of at most 32 terms per lane and 5 tree
-// steps adds 37 * 2^-24 relative: under 2^-18.3 of s.
-constexpr float kSigmoidError = 0x1p-21f;          // absolute
+// s (1 - s) (at most 1/4, and 0.224 / |z|), 1 + t adds 2^-24 and rcp.approx
+// 2^-23: 2.6e-7 in all.  For the softmax the sum of at most 32 terms per lane
+// and 5 tree steps adds 37 * 2^-24 relative: under 2^-18.3 of s.
+constexpr float kSigmoidError = 0x1.4p-22f;        // absolute, 3e-7
 constexpr float kSoftmaxError = 0x1p-18f;          // relative to the row's largest score
 constexpr float kAddError = 0x1p-23f;              // one f32 addition, relative to its result
 
@@ -140,11 +140,20 @@ __device__ __forceinline__ unsigned choose_groups(const F* keys, const RouteScor
   return rank_groups<F>(g < a.groups && l == 0 ? score : none, a, lanes, lane, gap, high);
 }
 
-// Score (and bias) of a logit in 64 bits; top and sum are the softmax's.
+// Score (and bias) of a logit in 64 bits; top and sum are the softmax's.  One
+// exp and one quotient for both kinds: this code runs rarely, and fetching it
+// is most of what it costs.
 __device__ __forceinline__ double key_in_64_bits(const RouteScoreArgs& a, double z, int e, double top, double sum) {
-  double key = a.scoring == kScoreSoftmax ? exp(z - top) / sum : 1.0 / (1.0 + exp(-z));
+  const bool softmax = a.scoring == kScoreSoftmax;
+  const double x = exp(softmax ? z - top : -z);
+  double key = (softmax ? x : 1.0) / (softmax ? sum : 1.0 + x);
   if (a.bias != nullptr) key += static_cast<double>(a.bias[e]);
   return z == -INFINITY ? -INFINITY : key;
+}
+// Unsigned order of 64-bit values (-0 is +0).
+__device__ __forceinline__ uint64_t ordered64(double v) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+  return b ^ ((b >> 63) != 0 ? ~0ull : 1ull << 63);
 }
 __device__ __noinline__ double softmax_sum_in_64_bits(const void* logits, int dtype, long long row, int E, double top,
                                                       int lane) {
@@ -210,26 +219,26 @@ __device__ __noinline__ int select_in_64_bits(const RouteScoreArgs& a, long long
 // The `n` candidates (ids in id[0..n)) ranked by 64-bit keys: lane k returns
 // the k-th.
 __device__ __noinline__ int rank_in_64_bits(const RouteScoreArgs& a, long long row, double top, double sum, int n,
-                                            double* keys, const int* id, int lane) {
-  const int eu = lane < n ? id[lane] : 0, ev = lane + 32 < n ? id[lane + 32] : 0;
-  const double u = key_in_64_bits(a, load_logit(a.logits, row + eu, a.dtype), eu, top, sum);
-  const double v = key_in_64_bits(a, load_logit(a.logits, row + ev, a.dtype), ev, top, sum);
-  keys[lane] = u;
-  keys[lane + 32] = v;
+                                            uint64_t* keys, int* id, int lane) {
+#pragma unroll 1
+  for (int i = lane; i < n; i += 32)
+    keys[i] = ordered64(key_in_64_bits(a, load_logit(a.logits, row + id[i], a.dtype), id[i], top, sum));
   __syncwarp();
-  int ru = 0, rv = 0;
-  for (int j = 0; j < n; ++j) {
-    const double o = keys[j];
-    const int e = id[j];
-    ru += (o > u || (o == u && e < eu)) ? 1 : 0;
-    rv += (o > v || (o == v && e < ev)) ? 1 : 0;
+  int mine = -1;
+#pragma unroll 1
+  for (int base = 0; base < n; base += 32) {
+    const int i = base + lane;
+    const uint64_t key = i < n ? keys[i] : 0ull;
+    const int e = i < n ? id[i] : 0;
+    int before = 0;
+    for (int j = 0; j < n; ++j) before += (keys[j] > key || (keys[j] == key && id[j] < e)) ? 1 : 0;
+    // The candidate of rank k goes to lane k.
+    for (int k = 0; k < a.top_k; ++k) {
+      const unsigned who = __ballot_sync(kAll, i < n && before == k);
+      const int v = __shfl_sync(kAll, e, who != 0u ? __ffs(who) - 1 : 0);
+      if (who != 0u && lane == k) mine = v;
+    }
   }
-  __syncwarp();
-  int* order = reinterpret_cast<int*>(keys);
-  if (lane < n) order[ru] = eu;
-  if (lane + 32 < n) order[rv] = ev;
-  __syncwarp();
-  const int mine = lane < n ? order[lane] : -1;
   __syncwarp();
   return mine;
 }
@@ -289,12 +298,11 @@ __host__ __device__ inline int warp_doubles(int experts) {
 }
 
 // NE experts per lane (E <= 32 * NE), logits of type DT.  A warp takes the
-// rows warp, warp + warps, ...; the next row's logits are on their way while
-// one is routed.  EVEN: E = 32 * NE and the groups, if any, are made of whole
+// rows warp, warp + warps, ....  EVEN: E = 32 * NE and the groups, if any, are made of whole
 // runs of 32 experts, so that a lane has as many of each: their scores then
 // take two reductions each and no shared memory.
 template <int NE, int DT, bool EVEN>
-__global__ void __launch_bounds__(32 * kRouteWarps, kRouteResident / (NE <= 16 ? 1 : 2))
+__global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? kRouteResident : kRouteResident / 2)
     k_route_scores(const __grid_constant__ RouteScoreArgs a) {
   extern __shared__ __align__(16) unsigned char route_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -316,17 +324,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps, kRouteResident / (NE <= 16 ?
   pdl_wait();
   pdl_launch_dependents();
 
-  float next[NE], bias[NE];
-#pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const int e = i * 32 + lane;
-    next[i] = (EVEN || e < E) && first < a.tokens ? logit_of<DT>(a.logits, first * a.stride + e) : -INFINITY;
-    bias[i] = biased && (EVEN || e < E) ? a.bias[e] : 0.0f;
-  }
+  float* biases = reinterpret_cast<float*>(loads + E);
   bool nan_bias = false;
-#pragma unroll
-  for (int i = 0; i < NE; ++i) nan_bias |= bias[i] != bias[i];
-  nan_bias = __any_sync(kAll, nan_bias);
+  if (biased) {
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+      const float v = a.bias[e];
+      biases[e] = v;
+      nan_bias |= v != v;
+    }
+    nan_bias = __syncthreads_or(nan_bias);
+  }
 
   for (int t = first; t < a.tokens; t += step) {
     const long long row = t * a.stride;
@@ -334,16 +341,13 @@ __global__ void __launch_bounds__(32 * kRouteWarps, kRouteResident / (NE <= 16 ?
     bool bad = false;
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      bad |= next[i] != next[i];
-      z[i] = __fadd_rn(next[i], 0.0f);  // -0 and +0 are one value
-      top = fmaxf(top, z[i]);
-    }
-    if (t + step < a.tokens) {
-      const long long next_row = (t + static_cast<long long>(step)) * a.stride + lane;
+    for (int i = 0; i < NE; ++i)
+      z[i] = EVEN || i * 32 + lane < E ? logit_of<DT>(a.logits, row + lane + i * 32) : -INFINITY;
 #pragma unroll
-      for (int i = 0; i < NE; ++i)
-        if (EVEN || i * 32 + lane < E) next[i] = logit_of<DT>(a.logits, next_row + i * 32);
+    for (int i = 0; i < NE; ++i) {
+      bad |= z[i] != z[i];
+      z[i] = __fadd_rn(z[i], 0.0f);  // -0 and +0 are one value
+      top = fmaxf(top, z[i]);
     }
     top = warp_max(top);
     bad |= softmax && top == INFINITY;
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, kRouteResident / (NE <= 16 ?
         else s = rcp(__fadd_rn(1.0f, ex2(__fmul_rn(z[i], -kLog2e))));
         float k = s;
         if (biased) {
-          k = __fadd_rn(__fadd_rn(s, bias[i]), 0.0f);
+          k = __fadd_rn(__fadd_rn(s, EVEN || i * 32 + lane < E ? biases[i * 32 + lane] : 0.0f), 0.0f);
           if (nan_bias) bad |= k != k && z[i] > -INFINITY;
         }
         if (z[i] == -INFINITY) k = -INFINITY;
@@ -546,7 +550,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, kRouteResident / (NE <= 16 ?
             for (int i = 0; i < NE; ++i)
               if (key[i] >= from) id[at++] = i * 32 + lane;
             __syncwarp();
-            mine = rank_in_64_bits(a, row, top64, sum64, n, keys64, id, lane);
+            mine = rank_in_64_bits(a, row, top64, sum64, n, ranked, id, lane);
           } else {
             if (narrow) {
               unsigned wide = 0u;
@@ -626,15 +630,16 @@ cudaError_t launch_route_scores(RouteScoreArgs a, cudaStream_t st) {
   a.group_inv = (1 << 20) / a.group_size + 1;  // e / group_size = e * inv >> 20 for e, group_size <= 1024
   cudaLaunchConfig_t cfg = {};
   // Every row a warp of its own while the GPU has room for all of them, then
-  // a share of the rows each.  (More resident warps cost registers that the
-  // next row's logits need: 8192 rows of 512 experts in groups took 27 us with
-  // 16 warps per SM, 35 us with 24.)
+  // a share of the rows each.  A row is a long chain of dependent steps, so
+  // resident warps count: 8192 rows of 512 experts took 11.4 us with 16 per SM,
+  // 8.7 us with 28 (sigmoid without bias or groups).  Fetching the next row
+  // early, or keeping the bias in registers, costs more warps than it gains.
   DeviceAttrs dev;
   const cudaError_t de = current_device_attrs(&dev);
   if (de != cudaSuccess) return de;
   cfg.gridDim = dim3(std::min((a.tokens + kRouteWarps - 1) / kRouteWarps, dev.sms * kRouteResident));
   cfg.blockDim = dim3(32 * kRouteWarps);
-  cfg.dynamicSmemBytes = sizeof(double) * kRouteWarps * warp_doubles(a.experts) + sizeof(int) * a.experts;
+  cfg.dynamicSmemBytes = sizeof(double) * kRouteWarps * warp_doubles(a.experts) + 2 * sizeof(int) * a.experts;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
