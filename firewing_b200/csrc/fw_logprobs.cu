@@ -6,7 +6,9 @@
 //   S = sum 2^y_i,  W = sum 2^y_i y_i
 //   log p_i = (z_i - M) / temperature - ln S,  H = ln 2 (log2 S - W / S)
 // S and W are sums of f32 terms that any part of the row adds up against a
-// reference of its own; parts are joined by rescaling.  One pass over the
+// reference of its own; parts are joined by rescaling, and carry S - 1, without
+// the maximum's own term: a row that is sure of one token has a log S far
+// below the rounding of S.  One pass over the
 // row keeps S, W and the candidates for the alternatives.
 //
 // The reference is the warp's maximum so far: with one far below the row's,
@@ -189,26 +191,22 @@ struct Row<kF32> {
   __device__ static __forceinline__ float one(const void* p, long long i) { return static_cast<const float*>(p)[i]; }
 };
 
-struct Part {  // sums of a part of a row against the reference m (-inf: nothing yet)
+// Sums of a part of a row against its maximum m (-inf: nothing yet), without
+// the maximum's own term 1 in s.
+struct Part {
   float m, s, w;
 };
 __device__ __forceinline__ Part join(const Part& a, const Part& b, float c) {
-  Part r;
-  r.m = fmaxf(a.m, b.m);
-  r.s = r.w = 0.0f;
-  const Part* p[2] = {&a, &b};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (p[i]->m == -INFINITY) {  // no finite value; s is 0, or NaN where the part holds one
-      r.s = __fadd_rn(r.s, p[i]->s);
-      continue;
-    }
-    const float d = max_nan(__fmul_rn(__fsub_rn(p[i]->m, r.m), c), kLowest);
-    const float f = ex2(d);
-    r.s = __fmaf_rn(p[i]->s, f, r.s);
-    r.w = __fmaf_rn(__fmaf_rn(d, p[i]->s, p[i]->w), f, r.w);
-  }
-  return r;
+  // no finite value: s is 0, or NaN where the part holds one
+  if (a.m == -INFINITY) return {b.m, __fadd_rn(a.s, b.s), b.w};
+  if (b.m == -INFINITY) return {a.m, __fadd_rn(a.s, b.s), a.w};
+  const bool up = a.m < b.m;
+  const Part& hi = up ? b : a;
+  const Part& lo = up ? a : b;
+  const float d = max_nan(__fmul_rn(__fsub_rn(lo.m, hi.m), c), kLowest);
+  const float f = ex2(d);
+  const float all = __fadd_rn(lo.s, 1.0f);
+  return {hi.m, __fadd_rn(hi.s, __fmul_rn(all, f)), __fmaf_rn(__fmaf_rn(d, all, lo.w), f, hi.w)};
 }
 
 // W warps work on a row (or a part of one).
@@ -551,8 +549,8 @@ __global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_
     fetch(j0 + kThreads * kUnroll);
     const float high = R::highest(raw);
     cover(high);
+    seen = fmaxf(seen, high);
     if (K > 0) {
-      seen = fmaxf(seen, high);
       // The floor rises after 1, 2, 4, ... batches, so that each stretch of
       // the row leaves about K candidates; the warps take turns at sorting.
       // Only the first time do they wait for one another.
@@ -609,21 +607,56 @@ __global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_
       }
     }
   }
+  seen = fmaxf(seen, ragged);
   if (K > 0 && warp == 0) {
     if (nvec == 0) floor = -INFINITY;
     offer(ragged, ragged_e);
-    seen = fmaxf(seen, ragged);
   }
   settle();
 
   // Join the lanes, then the warps.
-  float s_even, s_odd, w_even, w_odd;
-  unpack(s2, &s_even, &s_odd);
-  unpack(w2, &w_even, &w_odd);
+  float s_lane, w_lane, s_odd, w_odd;
+  unpack(s2, &s_lane, &s_odd);
+  unpack(w2, &w_lane, &w_odd);
+  s_lane = __fadd_rn(s_lane, s_odd);
+  w_lane = __fadd_rn(w_lane, w_odd);
   Part acc;
   acc.m = m;
-  acc.s = warp_sum(__fadd_rn(s_even, s_odd));
-  acc.w = warp_sum(__fadd_rn(w_even, w_odd));
+  acc.s = warp_sum(s_lane);
+  if (m > -INFINITY) {
+    acc.s = __fsub_rn(acc.s, 1.0f);
+    // One value outweighs the others: log S is about their sum, which the 1
+    // in the sum of its lane has rounded off.  The warp adds up that lane's
+    // values again without the maximum, 1 / 32 of what it has read.
+    if (acc.s < 1.0f) {
+      const int owner = __ffs(__ballot_sync(kAll, seen == m)) - 1;
+      float s = 0.0f, w = 0.0f;
+      int more = 0;
+      auto add_rest = [&](float x) {
+        const float y = max_nan(__fmul_rn(__fsub_rn(x, m), c), kLowest);
+        const float e = x == m ? 0.0f : ex2(y);
+        more += x == m ? 1 : 0;
+        s = __fadd_rn(s, e);
+        w = __fmaf_rn(e, y, w);
+      };
+#pragma unroll 1
+      for (int j = warp * 32 + owner + lane * kThreads; j < nvec; j += 32 * kThreads) {
+        float x[R::N];
+        R::unpack(vec[j], x);
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) add_rest(x[i]);
+      }
+      if (lane == owner && ragged > -INFINITY) add_rest(ragged);
+      more = static_cast<int>(__reduce_add_sync(kAll, static_cast<unsigned>(more)));
+      if (lane != owner) {
+        s = __fadd_rn(s, s_lane);
+        w = __fadd_rn(w, w_lane);
+      }
+      acc.s = __fadd_rn(warp_sum(s), static_cast<float>(more - 1));
+      w_lane = w;
+    }
+  }
+  acc.w = warp_sum(w_lane);
   if (lane == 0) sm.part[warp] = acc;
   if (K > 0 && LogprobSmem<W>::kSplit && a.splits > 1) {
     const uint32_t top = __reduce_max_sync(kAll, ordered(seen));
@@ -720,9 +753,8 @@ __global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_
 
   const Part whole = sm.whole;
   const bool bad = !(fabsf(whole.s) <= 3.4e38f);  // a NaN or +inf in the row
-  const bool empty = whole.s == 0.0f;             // every logit is -inf
-  const float log_s = log2f(whole.s);
-  const float ln_s = __fmul_rn(log_s, kLn2);
+  const bool empty = whole.m == -INFINITY;        // every logit is -inf
+  const float ln_s = log1pf(whole.s);
   const float nan = __uint_as_float(0x7fc00000u);
   auto logprob = [&](float x) {
     if (bad) return nan;
@@ -739,7 +771,7 @@ __global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_
     a.logprobs[o] = target < 0 ? 0.0f : target >= a.vocab ? nan : logprob(target_x);
   }
   if (a.entropy != nullptr && tid == kThreads - 1)
-    a.entropy[t] = bad ? nan : empty ? 0.0f : __fmul_rn(__fsub_rn(log_s, __fdiv_rn(whole.w, whole.s)), kLn2);
+    a.entropy[t] = bad ? nan : empty ? 0.0f : __fmaf_rn(-kLn2, __fdiv_rn(whole.w, __fadd_rn(whole.s, 1.0f)), ln_s);
   if (tid < K) {
     const long long o = static_cast<long long>(t) * K + tid;
     const bool there = tid < sm.found && !bad;

@@ -224,3 +224,41 @@ def test_repeatable_on_streams_and_in_graphs():
     for i in range(4):
         assert np.array_equal(outs[0][i].cpu().numpy(), want[i])
         assert np.array_equal(outs[1][i].cpu().numpy(), flipped[i])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("vocab", [2, 9, 54, 601, 5003, 50021])
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+def test_small_log_probabilities_keep_their_digits(dtype, vocab, temperature):
+    """Where one token is nearly sure, log p and the entropy are small numbers:
+    their relative errors are those of the other tokens' terms, a sum over
+    vocab and a gap of up to 64 nats with four roundings."""
+    tokens = 40
+    z = normal(vocab, tokens, vocab, std=1.0, dtype=dtype).clamp_(-4, 4)
+    at = (torch.arange(tokens, device="cuda") * 37 + (torch.arange(tokens, device="cuda") % 3 == 1) * (vocab - 1)) % vocab
+    z[torch.arange(tokens, device="cuda"), at] = 16.0
+    targets = at.to(torch.int32)[:, None].contiguous()
+    for rows in (1, tokens):  # split rows and whole ones
+        for top_k in (0, 2):
+            lp, h, ti, tl = run(z[:rows], targets[:rows], top_k, temperature=temperature)
+            y = z[:rows].double().cpu().numpy() / temperature
+            p = np.exp(y - y.max(1, keepdims=True))
+            ids = at[:rows].cpu().numpy()
+            rest = np.where(np.arange(vocab)[None] == ids[:, None], 0.0, p).sum(1)
+            tol = sum_tol(vocab) + 4 * EPS * 64
+            np.testing.assert_allclose(lp[:, 0], -np.log1p(rest), rtol=tol)
+            want = (y - y.max(1, keepdims=True)) - np.log1p(rest)[:, None]
+            np.testing.assert_allclose(h, -(p / (1 + rest)[:, None] * want).sum(1), rtol=3 * tol)
+            if top_k:
+                assert (ti[:, 0] == ids).all() and (tl[:, 0] == lp[:, 0]).all()
+
+
+def test_one_token_allowed():
+    """Log p of the only token that a mask leaves is 0, and so is the entropy."""
+    for vocab in (1, 7, 300, 40000):
+        z = torch.full((5, vocab), -float("inf"), device="cuda", dtype=torch.bfloat16)
+        at = torch.tensor([0, vocab - 1, vocab // 2, vocab // 3, vocab // 5], device="cuda")
+        z[torch.arange(5, device="cuda"), at] = torch.tensor([3.3, -700.0, 0.1, 20000.0, -0.7], device="cuda").bfloat16()
+        lp, h, ti, tl = run(z, at.to(torch.int32)[:, None].contiguous(), 1, temperature=0.7)
+        assert (lp == 0).all() and (h == 0).all() and (tl == 0).all()
+        assert (ti[:, 0] == at.cpu().numpy()).all()
