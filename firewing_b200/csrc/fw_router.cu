@@ -15,6 +15,11 @@
 // than the bound allows is decided again in 64 bits by the same warp.
 //
 // One warp per token; lane l holds the experts l, l + 32, ...
+//
+// Measured on B200, device time in a stream of calls: 8192 x 512 f32 sigmoid
+// 8.7 us, with a bias 15.4, with eight groups too 24 (the bytes: 2.7); one
+// token 6 to 8.  Bound by instructions, 1765 warp instructions a row in the
+// last form at 65 % of the issue slots; DRAM is at 8 %.
 #include <algorithm>
 #include <cstdint>
 
