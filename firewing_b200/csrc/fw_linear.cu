@@ -262,7 +262,8 @@ __device__ __forceinline__ F2 gelu2(F2 v) {
                            0.402343214f, -1.63778341f, 2.14749932f,  -1.18612599f, 0.246519342f};
   float x, y;
   unpack(v, &x, &y);
-  const F2 size = pack(fabsf(x), fabsf(y));
+  // (an infinite size would meet erfc = 0 in a product)
+  const F2 size = pack(fminf(fabsf(x), 1e30f), fminf(fabsf(y), 1e30f));
   float t0, t1;
   unpack(fma2(size, pack(0.35355339059327376f), pack(1.0f)), &t0, &t1);
   const F2 t = pack(rcp(t0), rcp(t1));
@@ -308,6 +309,14 @@ __device__ __forceinline__ F2 gate2(F2 x, F2 z) {
   unpack(add2(pack(ex2(z0), ex2(z1)), pack(1.0f)), &z0, &z1);
   return mul2(x, pack(rcp(z0), rcp(z1)));
 }
+// -inf as the lowest finite value, which a gate of 0 makes 0, the limit.
+__device__ __forceinline__ F2 finite_below(F2 v) {
+  float x, y;
+  unpack(v, &x, &y);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-3.402823466e38f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-3.402823466e38f));
+  return pack(x, y);
+}
 // The activations in f32, on N packed pairs.  gelu_tanh is 0.5 x (1 + tanh u)
 // = x / (1 + exp(-2u)) with u = sqrt(2/pi) (x + 0.044715 x^3): like SiLU and
 // the sigmoid a quotient without cancellation, whose relative error stays near
@@ -319,10 +328,10 @@ __device__ __forceinline__ void activate_pairs(int act, F2 (&v)[N]) {
     // exp(-2u) = 2^(x (c1 + c3 x^2))
     const F2 c1 = pack(-1.5957691216057308f * kLog2e), c3 = pack(-1.5957691216057308f * 0.044715f * kLog2e);
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = gate2(v[j], mul2(v[j], fma2(mul2(v[j], v[j]), c3, c1)));
+    for (int j = 0; j < N; ++j) v[j] = gate2(finite_below(v[j]), mul2(v[j], fma2(mul2(v[j], v[j]), c3, c1)));
   } else if (act == kActSilu) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = gate2(v[j], mul2(v[j], pack(-kLog2e)));
+    for (int j = 0; j < N; ++j) v[j] = gate2(finite_below(v[j]), mul2(v[j], pack(-kLog2e)));
   } else if (act == kActSigmoid) {
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = gate2(pack(1.0f), mul2(v[j], pack(-kLog2e)));

@@ -465,7 +465,8 @@ int fw_token_logprobs(const fw_logprob_config* config, const void* logits, int32
  * 1 <= rows, cols <= 2^24, 0 <= tokens <= 2^24, rows * tokens <= 2^38.
  * Device pointers of the current device.  FW_EINVAL otherwise.
  *   FW_ACT_GELU is x/2 (1 + erf(x / sqrt 2)), FW_ACT_GELU_TANH its tanh form,
- *   FW_ACT_SILU x / (1 + exp(-x)). */
+ *   FW_ACT_SILU x / (1 + exp(-x)); at infinities all have their limits, and
+ *   NaN stays NaN. */
 #define FW_ACT_NONE 0
 #define FW_ACT_RELU 1
 #define FW_ACT_GELU 2

@@ -244,3 +244,32 @@ def test_a_run_from_hidden_states_to_log_probabilities():
     torch.testing.assert_close(lp.double(), q.gather(1, targets.long()), rtol=0, atol=2.0 ** -15)
     torch.testing.assert_close(ent.double(), -(q.exp() * q).sum(1), rtol=0, atol=2.0 ** -12)
     torch.testing.assert_close(tl.double(), q.sort(1, descending=True).values[:, :4], rtol=0, atol=2.0 ** -15)
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 200, 600])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_activations_at_infinities_and_large_values(tokens, out):
+    """Sums (here the bias alone) at the ends of the range: the limits of each
+    activation, and NaN."""
+    inf, nan = math.inf, math.nan
+    at = [inf, -inf, nan, 3e38, -3e38, 1e25, -1e25, 200.0, -200.0, 0.0]
+    limits = {
+        "none": at,
+        "relu": [inf, 0, nan, 3e38, 0, 1e25, 0, 200.0, 0, 0],
+        "gelu": [inf, 0, nan, 3e38, 0, 1e25, 0, 200.0, 0, 0],
+        "gelu_tanh": [inf, 0, nan, 3e38, 0, 1e25, 0, 200.0, 0, 0],
+        "silu": [inf, 0, nan, 3e38, 0, 1e25, 0, 200.0, 0, 0],
+        "sigmoid": [1, 0, nan, 1, 0, 1, 0, 1, 0, 0.5],
+    }
+    rows = 320
+    x = torch.ones(tokens, 64, device="cuda", dtype=torch.bfloat16)
+    w = torch.zeros(rows, 64, device="cuda", dtype=torch.bfloat16)
+    bias = torch.tensor(at * (rows // len(at)), device="cuda")
+    for act, want in limits.items():
+        y = torch.empty(tokens, rows, device="cuda", dtype=DTYPES[out])
+        fw.linear_epilogue(w, x, y, bias=bias, activation=act)
+        expected = torch.tensor(want * (rows // len(at)), device="cuda").expand(tokens, rows)
+        if act != "sigmoid":
+            expected = expected.to(y.dtype)  # one rounding; 200 and 0 are exact
+        # (a sigmoid's quotient in f32: 2^-22)
+        torch.testing.assert_close(y.float(), expected.float(), rtol=2.0 ** -22, atol=1e-30, equal_nan=True)
