@@ -14,7 +14,7 @@
 //     warps 2-9   epilogue, two sets of four (set s takes the 32-column
 //                 groups s, s + 2, ...)
 //     Where TMA cannot read an operand (a row stride or base that is no
-//     multiple of 16 bytes) warps 2-5 are the epilogue and warps 6-19
+//     multiple of 16 bytes) warps 2-5 are the epilogue and warps 6-21
 //     loaders, which bring the rows into shared memory by cp.async, realign
 //     them in registers and write the same layout
 //   Few tokens: w is the M side and the K range is split over the CTAs of a
@@ -32,8 +32,9 @@
 //     in two waves of 74 pairs
 //   64 x 8192 x 2048 bf16, bias, SiLU             12.2 us  (5.4): the first
 //     loads' way, 32 blocks of a CTA, the epilogue, one after the other
-//   333 x 1001 x 1999 f16, bias, GELU, residual   20.4 us  (1.0): the loaders
-//     (26 bytes per ns and SM)
+//   333 x 1001 x 1999 f16, bias, GELU, residual   15.7 us  (1.0): the loaders
+//     (29 to 32 bytes per ns and SM), the joint, code that runs once
+//   8000 x 8001 x 2001 f16                         886 us  (154): the loaders
 //   1 x 512 x 2048 bf16                            3.0 us  (0.3): a launch and
 //     two trips to memory
 //
@@ -59,18 +60,25 @@ constexpr int kBK = 64;                   // columns per stage (one 128-byte swi
 constexpr int kABytes = kBM * kBK * 2;    // 16 KB
 constexpr int kMaxStages = 8;
 constexpr int kEpiWarps = 8;
-constexpr int kLoadWarps = 14;
+constexpr int kLoadWarps = 16;
 // The loaders are two groups that take turns at stages: what a warp waits for
 // in a stage (its words, the slot, the fence) would otherwise bound it.
 constexpr int kLoadGroups = 2;
 constexpr int kGroupWarps = kLoadWarps / kLoadGroups;
-constexpr int kWarpRows = 28;              // rows of a stage that a loader warp fills
-constexpr int kLoadBn = 64;                // N tiles are this wide at most
-static_assert(kGroupWarps * kWarpRows >= kBM + kLoadBn, "every row of a stage has a loader");
-constexpr int kAhead = 1;                             // stages of its own that a group fetches ahead
-constexpr int kRawBytes = kWarpRows * 144;            // a warp's words of a stage
-constexpr int kLoadStages = 3;                        // operand stages beside them
+constexpr int kWarpRows = 32;              // rows of a stage that a loader warp fills, at most
+constexpr int kLoadBn = 128;               // N tiles are this wide at most
+constexpr int kAhead = 1;                  // stages of its own that a group fetches ahead
+constexpr int kRawBytes = kWarpRows * 144; // a warp's words of a stage
+constexpr int kLoadStages = 2;             // operand stages beside them
 constexpr int kRawTotal = kLoadWarps * (kAhead + 1) * kRawBytes;
+// Warps of a group for the P rows, so that both sides' warps have about as
+// many rows; the others serve the Q rows.
+__host__ __device__ constexpr int p_warps(int bn) { return (kGroupWarps * kBM + (kBM + bn) / 2) / (kBM + bn); }
+constexpr bool loaders_hold(int bn) {
+  return bn > kLoadBn || (p_warps(bn) < kGroupWarps && p_warps(bn) * kWarpRows >= kBM &&
+                          (kGroupWarps - p_warps(bn)) * kWarpRows >= bn && loaders_hold(bn + 16));
+}
+static_assert(loaders_hold(16), "every row of a stage has a loader");
 constexpr int kMmaThreads = 32 * (2 + kEpiWarps);
 // With loaders half the epilogue warps: N tiles are narrow then.
 constexpr int kLoaderEpiWarps = 4;
@@ -169,7 +177,7 @@ __device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// 32 consecutive f32 columns of this thread's TMEM lane.
+// 32 (16) consecutive f32 columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
   asm volatile(
@@ -184,6 +192,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 __device__ __forceinline__ void cluster_sync_all() {
@@ -577,23 +598,22 @@ __device__ __forceinline__ void finish_block(const LinearArgs& a, int p0, int q0
 
 // ---- operands that TMA cannot read ----------------------------------------------------
 
-// Eight 16-bit elements that start `off` bytes (even, under 16) into the
-// aligned words a, b.
-__device__ __forceinline__ uint4 realign(uint4 a, uint4 b, uint32_t off) {
-  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// Moves w down by `off` bytes (even, under 16): w[0..N - 4) are then whole.
+template <int N>
+__device__ __forceinline__ void realign(uint32_t (&w)[N], uint32_t off) {
   if (off & 8) {
 #pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    for (int i = 0; i < N - 2; ++i) w[i] = w[i + 2];
   }
   if (off & 4) {
 #pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    for (int i = 0; i < N - 3; ++i) w[i] = w[i + 1];
   }
   const uint32_t sh = (off & 2) * 8;
-  return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh), __funnelshift_r(w[2], w[3], sh),
-                    __funnelshift_r(w[3], w[4], sh));
+#pragma unroll
+  for (int i = 0; i < N - 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], sh);
 }
-// The first n (below 8) of eight elements, the others 0.
+// The first n of eight elements, the others 0.
 __device__ __forceinline__ uint4 first_of(uint4 v, int n) {
   uint32_t o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -613,7 +633,9 @@ __device__ __forceinline__ uint4 load_chunk(const uint16_t* p, int n) {
   const uint4 a = __ldg(s);
   uint4 b = make_uint4(0, 0, 0, 0);
   if (off + 2 * n > 16) b = __ldg(s + 1);
-  const uint4 v = realign(a, b, off);
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  realign<8>(w, off);
+  const uint4 v = make_uint4(w[0], w[1], w[2], w[3]);
   return n < 8 ? first_of(v, n) : v;
 }
 
@@ -844,7 +866,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
         if (lane == 0) mbar_arrive(&tail->acc_empty[buf]);
         ++ai;
       } else {
-        constexpr int kGroups = LOADERS ? kLoadBn / 32 : 2;  // 32-column groups of this warp
+        constexpr int kGroups = 2;  // 32-column groups of this warp
         float acc[kGroups][32];
 #pragma unroll
         for (int g = 0; g < kGroups; ++g)
@@ -864,10 +886,13 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
           for (int g = 0; g < kGroups; ++g) {
             const int c0 = 32 * (set + kSets * g);
             if (c0 < a.bn) {
-              float v[32];
-              tmem_ld32(lane_base + buf * acc_cols + c0, v);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) acc[g][j] = __fadd_rn(acc[g][j], v[j]);
+              for (int h = 0; h < 32; h += 16) {
+                float v[16];
+                tmem_ld16(lane_base + buf * acc_cols + c0 + h, v);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[g][h + j] = __fadd_rn(acc[g][h + j], v[j]);
+              }
             }
           }
           tc_fence_before();
@@ -884,14 +909,31 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     }
   } else if (LOADERS) {
     // ---------------- loaders ----------------
-    // Each warp serves kWarpRows of a stage's rows.  A row's 64 columns lie in nine
-    // aligned 16-byte words at most; these come into the warp's own buffers
-    // by cp.async, kAhead stages ahead, and are then cut into the operand's
-    // 16-byte chunks.  A stage moves every row on by 128 bytes, so a row's
-    // offset in its words stays the same over a tile.  Words without an
-    // element of the operand are not read (size 0: zeros).
+    // Each warp serves up to kWarpRows consecutive rows of one side.  A row's
+    // 64 columns lie in nine aligned 16-byte words at most; these come into the
+    // warp's own buffers by cp.async (27 lanes, three rows a step), kAhead stages
+    // ahead, and are then cut into the operand's 16-byte chunks (sixteen rows a
+    // step).  A stage moves every row on by 128 bytes, so a row's offset in its
+    // words stays the same over a tile.  Words without an element of the
+    // operand are not read (size 0: zeros); rows beyond the operand are left
+    // as they are, as nobody reads their products.
     const int group = (warp - (2 + kEpi)) / kGroupWarps, lw = (warp - (2 + kEpi)) % kGroupWarps;
     unsigned char* mine = ring + stages * slot + (warp - (2 + kEpi)) * (kAhead + 1) * kRawBytes;
+    const int np = p_warps(a.bn);
+    const bool side_p = lw < np;
+    const int side_rows = side_p ? kBM : a.bn, side_warps = side_p ? np : kGroupWarps - np;
+    const int each = (side_rows + side_warps - 1) / side_warps;
+    const int r0 = (side_p ? lw : lw - np) * each;  // of the side's rows in a tile
+    const int most = max(0, min(each, side_rows - r0));
+    const int limit = side_p ? a.p_rows : a.q_rows;
+    const long long pitch = (side_p ? a.p_stride : a.q_stride) * 2;
+    // The rows that exist, and the first one's address.
+    const auto rows_of = [&](int u, int* count) {
+      const Tile w = tile_of(a, u);
+      const int at = (side_p ? w.p0 : w.q0) + r0;
+      *count = max(0, min(most, limit - at));
+      return reinterpret_cast<uintptr_t>(side_p ? a.p : a.q) + (*count > 0 ? at * pitch : 0);
+    };
     // The stage after the next one of the other group.
     const auto advance = [&](int* u, int* kb, int by) {
       for (int i = 0; i < by; ++i)
@@ -900,79 +942,48 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
           *u += step;
         }
     };
-    const auto row_at = [&](const Tile& w, int r, bool* there) {
-      const bool side_p = r < kBM;
-      const int grow = side_p ? w.p0 + r : w.q0 + r - kBM;
-      *there = r < kBM + a.bn && grow < (side_p ? a.p_rows : a.q_rows);
-      return reinterpret_cast<uintptr_t>((side_p ? a.p : a.q) +
-                                         (*there ? grow * (side_p ? a.p_stride : a.q_stride) : 0));
-    };
-    // What is being fetched: tile iu, block ik; the lane's word in each step.
-    constexpr int kFetch = (kWarpRows * 9 + 31) / 32, kCut = (kWarpRows * 8 + 31) / 32;
+    constexpr int kFetch = (kWarpRows + 2) / 3, kCut = kWarpRows / 16;
+    const int half = lane & 1, row2 = lane >> 1;
+    const int row3 = lane / 9, word = lane - 9 * row3;  // lanes 27 to 31 fetch nothing
     int iu = u0, ik = kb0, issued = 0, aimed = -1;
     advance(&iu, &ik, group);
-    uintptr_t word[kFetch];
-    uint32_t word_off = 0u, word_there = 0u;  // 4 bits, 1 bit a step
-    uint32_t word_full = 0u;                  // words that hold elements of a whole block
-    const auto aim = [&]() {
-      const Tile w = tile_of(a, iu);
-      word_off = word_there = word_full = 0u;
-#pragma unroll
-      for (int j = 0; j < kFetch; ++j) {
-        const int g = lane + 32 * j;
-        bool there;
-        const uintptr_t at = row_at(w, lw * kWarpRows + g / 9, &there);
-        there = there && g < kWarpRows * 9;
-        word[j] = (at & ~uintptr_t(15)) + 16 * (g % 9);
-        word_off |= static_cast<uint32_t>(at & 15u) << (4 * j);
-        word_there |= static_cast<uint32_t>(there) << j;
-        word_full |= static_cast<uint32_t>(there && (g % 9 < 8 || (at & 15u) != 0)) << j;
-      }
-    };
+    uintptr_t fetch_at = 0;
+    int fetch_rows = 0;
     const auto issue = [&]() {
       if (iu < total) {
-        if (iu != aimed) aim();
-        aimed = iu;
-        uint32_t read = word_full;
-        if (a.cols - ik * kBK < kBK) {  // the last block: words that start before a row's end
-          const int bytes = 2 * (a.cols - ik * kBK);
-          read = 0u;
-#pragma unroll
-          for (int j = 0; j < kFetch; ++j) {
-            const int end = static_cast<int>((word_off >> (4 * j)) & 15u) + bytes;
-            read |= static_cast<uint32_t>(16 * ((lane + 32 * j) % 9) < end) << j;
-          }
-          read &= word_there;
+        if (iu != aimed) {
+          fetch_at = rows_of(iu, &fetch_rows) + row3 * pitch;
+          if (row3 == 3) fetch_rows = 0;
+          aimed = iu;
         }
-        const uint32_t to = smem_u32(mine) + issued % (kAhead + 1) * kRawBytes + 16 * lane;
-        const uintptr_t on = static_cast<uintptr_t>(ik) * (2 * kBK);
+        const int bytes = 2 * min(kBK, a.cols - ik * kBK);
+        const uintptr_t on = static_cast<uintptr_t>(ik) * (2 * kBK) + 16 * word;
+        uint32_t to = smem_u32(mine) + issued % (kAhead + 1) * kRawBytes + row3 * 144 + 16 * word;
+        uintptr_t at = fetch_at;
 #pragma unroll
         for (int j = 0; j < kFetch; ++j) {
-          const uint32_t size = ((read >> j) & 1u) * 16u;
-          if (lane + 32 * j < kWarpRows * 9)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 512 * j), "l"(word[j] + on),
-                         "r"(size)
+          if (row3 + 3 * j < fetch_rows) {
+            const int off = static_cast<int>(at & 15u);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 432 * j), "l"(at - off + on),
+                         "r"(16 * word < off + bytes ? 16 : 0)
                          : "memory");
+          }
+          at += 3 * pitch;
         }
         ++issued;
         advance(&iu, &ik, kLoadGroups);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    int u = u0, kb = kb0, st = group, done = 0, cut = -1;
-    uint32_t phase = 1u, cut_off = 0u;
+    int u = u0, kb = kb0, st = group, done = 0, cut = -1, cut_rows = 0;
+    uint32_t phase = 1u, cut_at = 0u;  // cut_at: low bits of the address of the lane's first row
+    const uint32_t pitch16 = 16u * static_cast<uint32_t>(pitch);
     advance(&u, &kb, group);
     for (int i = 0; i < kAhead; ++i) issue();
     while (u < total) {
       if (u != cut) {
-        const Tile w = tile_of(a, u);
+        cut_at = static_cast<uint32_t>(rows_of(u, &cut_rows)) + static_cast<uint32_t>(row2) * static_cast<uint32_t>(pitch);
         cut = u;
-        cut_off = 0u;
-#pragma unroll
-        for (int j = 0; j < kCut; ++j) {
-          bool there;
-          cut_off |= static_cast<uint32_t>(row_at(w, lw * kWarpRows + (lane >> 3) + 4 * j, &there) & 15u) << (4 * j);
-        }
       }
       issue();
       asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
@@ -981,20 +992,30 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
         give_up(tail);
         break;
       }
-      // The lane's chunk c of rows r, r + 4, ...: row r of P at slot, row
-      // r - 128 of Q at slot + 16 KB, r * 128 either way, its chunks swapped
-      // by the row's low three bits.
-      const int c = lane & 7, r = lw * kWarpRows + (lane >> 3);
-      const unsigned char* from = mine + done % (kAhead + 1) * kRawBytes + (lane >> 3) * 144 + c * 16;
-      unsigned char* to = ring + st * slot + r * 128;
-      const int count = a.cols - kb * kBK;
+      // The lane's half of rows r, r + 16: row r of P at slot, of Q at slot +
+      // 16 KB, r * 128 either way, its chunks swapped by the row's low three
+      // bits.  (Both sides are free of bank conflicts: four rows' halves per
+      // 128 bytes.)
+      const unsigned char* from = mine + done % (kAhead + 1) * kRawBytes + row2 * 144 + half * 64;
+      unsigned char* to = ring + st * slot + (side_p ? 0 : kABytes) + (r0 + row2) * 128;
+      const int count = a.cols - kb * kBK - 32 * half;
 #pragma unroll
       for (int j = 0; j < kCut; ++j) {
-        const uint4* v = reinterpret_cast<const uint4*>(from + 4 * 144 * j);
-        uint4 o = realign(v[0], v[1], (cut_off >> (4 * j)) & 15u);
-        if (count < kBK) o = first_of(o, count - 8 * c);
-        if ((lane >> 3) + 4 * j < kWarpRows && r + 4 * j < kBM + a.bn)
-          *reinterpret_cast<uint4*>(to + 512 * j + ((c ^ ((r + 4 * j) & 7)) << 4)) = o;
+        uint32_t w[20];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          const uint4 v = reinterpret_cast<const uint4*>(from + 16 * 144 * j)[i];
+          w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+        realign<20>(w, (cut_at + j * pitch16) & 15u);
+        if (row2 + 16 * j < cut_rows) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 o = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            if (count < 32) o = first_of(o, count - 8 * i);
+            *reinterpret_cast<uint4*>(to + 2048 * j + (((4 * half + i) ^ ((r0 + row2) & 7)) << 4)) = o;
+          }
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();  // (and the buffer has been read before it is filled again)
@@ -1443,7 +1464,7 @@ struct Plan {
 
 // The plan with the shortest estimate, over the tile widths, sides and splits
 // that exist, and the pair kernel.  A CTA brings 130 bytes per ns into its shared memory (measured;
-// loaders 26), a stage of the pair is bound by its MMAs (270 ns at bn = 256);
+// loaders 29), a stage of the pair is bound by its MMAs (270 ns at bn = 256);
 // partial tiles cost 1.2 us and more with their width, the last tile's
 // epilogue in a CTA 0.6 us and 5 ns per column.  The ring is 96 KB, so
 // that the next launch's CTAs can move in beside this one's; 200 KB was no
@@ -1452,7 +1473,7 @@ struct Plan {
 // 128 x 2048 x 2048 8.1 / 8.1, 512 x 2048 x 2048 11.0 / 11.0.
 Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const ClusterRoom& room) {
   const int kblocks = (a.cols + kBK - 1) / kBK;
-  const double rate = tma ? 130.0 : 26.0;
+  const double rate = tma ? 130.0 : 29.0;
   Plan best;
   const auto consider = [&](bool swap, int bn, long long tiles, int splits) {
     const double waves = static_cast<double>((tiles * splits + sms - 1) / sms);
@@ -1470,10 +1491,10 @@ Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const Clust
     }
   };
   const long long rows128 = (a.rows + kBM - 1) / kBM, tokens128 = (a.tokens + kBM - 1) / kBM;
-  const int widest = !tma ? kLoadBn : chunked ? 128 : 256;
+  const int widest = !tma ? (chunked ? 64 : kLoadBn) : chunked ? 128 : 256;
   const int tokens16 = (a.tokens + 15) & ~15, rows16 = (a.rows + 15) & ~15;
   if (a.tokens <= 1024) {
-    for (int bn : {16, 32, 64, 96, 128, 192, 256}) {
+    for (int bn : {16, 32, 64, 96, 112, 128, 192, 256}) {
       const int n = std::min(bn, tokens16);
       if (n > widest) break;
       const long long tiles = rows128 * ((a.tokens + n - 1) / n);
