@@ -273,3 +273,23 @@ def test_activations_at_infinities_and_large_values(tokens, out):
             expected = expected.to(y.dtype)  # one rounding; 200 and 0 are exact
         # (a sigmoid's quotient in f32: 2^-22)
         torch.testing.assert_close(y.float(), expected.float(), rtol=2.0 ** -22, atol=1e-30, equal_nan=True)
+
+
+@pytest.mark.parametrize("size", [(5, 40, 9), (64, 129, 63), (100, 300, 1030), (112, 700, 517), (130, 2049, 333),
+                                  (333, 1001, 1999), (1100, 1030, 2049), (2000, 3001, 257), (7000, 2060, 70)])
+@pytest.mark.parametrize("out", ["f16", "f32"])
+@pytest.mark.parametrize("shift", [(1, 3), (0, 2), (7, 0)])
+def test_rows_at_odd_addresses_amid_nan(size, out, shift):
+    """Operands whose rows start anywhere, with NaN between and around them."""
+    T, N, K = size
+
+    def amid(seed, rows, cols, at, pad, std=1.0):
+        whole = torch.full((rows + 2, cols + pad), math.nan, device="cuda", dtype=torch.float16)
+        whole[1:-1, at:at + cols] = normal(seed, rows, cols, std=std, dtype="f16")
+        return whole[1:-1, at:at + cols]
+
+    w = amid(1, N, K, shift[0], 11, std=1 / math.sqrt(K))
+    x = amid(2, T, K, shift[1], 8)
+    y = torch.full((T, N), math.nan, device="cuda", dtype=DTYPES[out])
+    check(w, x, y, normal(3, N, dtype="f32"), "silu", normal(4, T, N, dtype="f16"))
+    check(w, x, y)
