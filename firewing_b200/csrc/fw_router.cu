@@ -17,7 +17,7 @@
 // One warp per token; lane l holds the experts l, l + 32, ...
 //
 // Measured on B200, device time in a stream of calls: 8192 x 512 f32 sigmoid
-// 8.7 us, with a bias 15.4, with eight groups too 24 (the bytes: 2.7); one
+// 8.8 us, with a bias 14.5, with eight groups too 21 (the bytes: 2.7); one
 // token 6 to 8.  Bound by instructions, 1765 warp instructions a row in the
 // last form at 65 % of the issue slots; DRAM is at 8 %.
 #include <algorithm>
@@ -145,6 +145,15 @@ __device__ __forceinline__ unsigned choose_groups(const F* keys, const RouteScor
   return rank_groups<F>(g < a.groups && l == 0 ? score : none, a, lanes, lane, gap, high);
 }
 
+// Shared memory of one warp: f32 or f64 keys of a row (group g shifted by
+// g * lanes <= 32), or the candidates being ranked (keys and ids), which may
+// stand behind f32 keys.
+constexpr int kRanked = 64;
+__host__ __device__ inline int warp_doubles(int experts) {
+  const int behind = (experts + 33) / 2 + kRanked + kRanked / 2;
+  return experts + 32 > behind ? experts + 32 : behind;
+}
+
 // Score (and bias) of a logit in 64 bits; top and sum are the softmax's.  One
 // exp and one quotient for both kinds: this code runs rarely, and fetching it
 // is most of what it costs.
@@ -167,19 +176,65 @@ __device__ __noinline__ double softmax_sum_in_64_bits(const void* logits, int dt
   return warp_sum(sum);
 }
 // The groups chosen by 64-bit scores, for a row whose f32 scores leave the
-// border open; the row's keys stay in `keys`.
+// border open; the row's f32 keys (or logits, whose order is the scores') are
+// in `keys` (see choose_groups).  Only the experts that may be among their
+// group's two best are looked at, one or two a lane: one such row in thousands
+// would otherwise end well after all others (all experts in 64 bits: 6 us).
 __device__ __noinline__ unsigned groups_in_64_bits(const RouteScoreArgs& a, long long row, double top, double sum,
-                                                   int lanes, double* keys, int lane) {
-  __syncwarp();
-  for (int e = lane; e < a.experts; e += 32) {
-    const int g = (e * a.group_inv) >> 20;
-    keys[e + g * lanes] = key_in_64_bits(a, load_logit(a.logits, row + e, a.dtype), e, top, sum);
+                                                   int lanes, float error, const float* keys, int lane) {
+  const int g = lane / lanes, l = lane - g * lanes;
+  const float* mine = keys + g * (a.group_size + lanes);
+  const int size = g < a.groups ? a.group_size : 0;
+  float m1 = -INFINITY, m2 = -INFINITY;
+  for (int j = l; j < size; j += lanes) {
+    const float v = mine[j];
+    m2 = fmaxf(m2, fminf(m1, v));
+    m1 = fmaxf(m1, v);
+  }
+  for (int o = 1; o < lanes; o <<= 1) {
+    const float o1 = __shfl_xor_sync(kAll, m1, o), o2 = __shfl_xor_sync(kAll, m2, o);
+    m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+    m1 = fmaxf(m1, o1);
+  }
+  float from = a.group_top == 2 && m2 > -INFINITY ? m2 : m1;
+  from = fmaxf(__fsub_rn(from, 2.5f * (error + kAddError * fabsf(from))), kLowest);
+  uint64_t* spare = reinterpret_cast<uint64_t*>(const_cast<float*>(keys)) + (a.experts + 33) / 2;
+  double* exact = reinterpret_cast<double*>(spare);
+  int* id = reinterpret_cast<int*>(spare + kRanked);
+  int n = 0;
+  for (int j = l; j - l < a.group_size; j += lanes) {
+    const bool in = j < size && mine[j] >= from;
+    const unsigned who = __ballot_sync(kAll, in);
+    const int at = n + __popc(who & ((1u << lane) - 1u));
+    if (in && at < kRanked) id[at] = g * a.group_size + j;
+    n += __popc(who);
   }
   __syncwarp();
-  double gap, high;
-  const unsigned chosen = choose_groups<double>(keys, a, lanes, lane, &gap, &high);
+  double gap, high, d1 = -INFINITY, d2 = -INFINITY;
+  if (n > kRanked) {  // rows of many equal keys
+    double* all = reinterpret_cast<double*>(const_cast<float*>(keys));
+    for (int e = lane; e < a.experts; e += 32)
+      all[e + ((e * a.group_inv) >> 20) * lanes] = key_in_64_bits(a, load_logit(a.logits, row + e, a.dtype), e, top, sum);
+    __syncwarp();
+    return choose_groups<double>(all, a, lanes, lane, &gap, &high);
+  }
+#pragma unroll 1
+  for (int i = lane; i < n; i += 32)
+    exact[i] = key_in_64_bits(a, load_logit(a.logits, row + id[i], a.dtype), id[i], top, sum);
   __syncwarp();
-  return chosen;
+  for (int i = l; i < n; i += lanes) {
+    if (((id[i] * a.group_inv) >> 20) != g) continue;
+    const double v = exact[i];
+    d2 = fmax(d2, fmin(d1, v));
+    d1 = fmax(d1, v);
+  }
+  for (int o = 1; o < lanes; o <<= 1) {
+    const double o1 = __shfl_xor_sync(kAll, d1, o), o2 = __shfl_xor_sync(kAll, d2, o);
+    d2 = fmax(fmin(d1, o1), fmax(d2, o2));
+    d1 = fmax(d1, o1);
+  }
+  const double score = a.group_top == 2 && d2 > -INFINITY ? d1 + d2 : d1;
+  return rank_groups<double>(g < a.groups && l == 0 ? score : -INFINITY, a, lanes, lane, &gap, &high);
 }
 // Repeated maxima of 64-bit keys, for a row with more near ties than are
 // ranked: lane k returns the k-th selected expert, -1 where there is none.
@@ -292,14 +347,6 @@ __device__ __noinline__ void select_by_rounds(const float* keys, int rounds, int
     last = m;
     last_e = e;
   }
-}
-
-// Shared memory of one warp: f32 or f64 keys of a row (group g shifted by
-// g * lanes <= 32), or the candidates being ranked.
-constexpr int kRanked = 64;
-constexpr int kRankedDoubles = kRanked + kRanked / 2;  // keys and ids
-__host__ __device__ inline int warp_doubles(int experts) {
-  return experts + 32 > kRankedDoubles ? experts + 32 : kRankedDoubles;
 }
 
 // NE experts per lane (E <= 32 * NE), logits of type DT.  A warp takes the
@@ -429,7 +476,13 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? kRouteResident : 
         }
         if (!(gap > 2.0f * (a.group_top * error + 3.0f * kAddError * high))) {
           if (softmax) sum64 = softmax_sum_in_64_bits(a.logits, DT, row, E, top64, lane);
-          chosen = groups_in_64_bits(a, row, top64, sum64, lanes, keys64, lane);
+          if (EVEN) {
+#pragma unroll
+            for (int i = 0; i < NE; ++i) keys[i * 32 + lane + (i >> shift) * lanes] = key[i];
+          }
+          __syncwarp();
+          chosen = groups_in_64_bits(a, row, top64, sum64, lanes, error, keys, lane);
+          __syncwarp();
           spread = lanes;
         }
 #pragma unroll
@@ -514,31 +567,39 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? kRouteResident : 
         float copy[NE];
 #pragma unroll
         for (int i = 0; i < NE; ++i) copy[i] = key[i];
-        select_by_rounds<NE>(copy, min(K + 1, 32), lane, &my_key, &mine);
+        select_by_rounds<NE>(copy, 32, lane, &my_key, &mine);
         after = __shfl_down_sync(kAll, my_key, 1);
         after_e = __shfl_down_sync(kAll, mine, 1);
-        if (lane == 31) {  // K = 32: the key behind has no lane and counts as near
-          after = K == 32 ? my_key : -INFINITY;
+        if (lane == 31) {  // the key behind has no lane and counts as near
+          after = my_key;
           after_e = -1;
         }
       }
       if (biased) {
+        // Neighbours in the order have to be further apart than their errors,
+        // unless they are the same logit and bias: the first K and the one
+        // behind them, and where those at the border are the same, all
+        // that follow as near.
+        const auto is_close = [&](float behind) {
+          return behind > -INFINITY &&
+                 !(__fsub_rn(my_key, behind) > 2.0f * (error + kAddError * fmaxf(fabsf(my_key), fabsf(behind))));
+        };
+        const bool close = is_close(after);
+        bool other = close;
+        if (close && my_key == after && after_e >= 0)
+          other = logit_of<DT>(a.logits, row + mine) != logit_of<DT>(a.logits, row + after_e) ||
+                  a.bias[mine] != a.bias[after_e];
+        const unsigned apart = ~(__ballot_sync(kAll, close) >> (K - 1));
+        const int end = K - 1 + (apart != 0u ? __ffs(apart) - 1 : 32);  // the last of them
+        bool near = other && lane < max(end, K);
+        if (end > 31) near = true;  // (they pass the lanes)
         // The best key that is no candidate stands behind the last one.
-        if (n <= K) {
+        if (n <= K || end == n - 1) {
           float below = -INFINITY;
 #pragma unroll
           for (int i = 0; i < NE; ++i) below = fmaxf(below, key[i] < floor ? key[i] : -INFINITY);
           below = warp_max(below);
-          if (lane == n - 1) after = below;
-        }
-        // Neighbours in the order have to be further apart than their errors,
-        // unless they are the same logit and bias.
-        bool near = false;
-        if (lane < K && after > -INFINITY) {
-          near = !(__fsub_rn(my_key, after) > 2.0f * (error + kAddError * fmaxf(fabsf(my_key), fabsf(after))));
-          if (near && my_key == after && after_e >= 0)
-            near = logit_of<DT>(a.logits, row + mine) != logit_of<DT>(a.logits, row + after_e) ||
-                   a.bias[mine] != a.bias[after_e];
+          if (lane == n - 1) near |= is_close(below);
         }
         if (__any_sync(kAll, near)) {
           if (softmax && sum64 == 0.0) sum64 = softmax_sum_in_64_bits(a.logits, DT, row, E, top64, lane);

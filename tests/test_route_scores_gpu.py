@@ -254,3 +254,46 @@ def test_the_reference_route_is_the_plain_case():
     fw.route_bf16(z, 50, 512, 10, ri, rs)
     assert np.array_equal(idx, ri.cpu().numpy())
     np.testing.assert_allclose(w, rs.float().cpu().numpy(), rtol=2.0 ** -8 + SOFTMAX_SUM_TOL)
+
+
+@pytest.mark.parametrize("shape", [(512, 8), (1024, 32), (128, 4), (160, 8), (256, 16), (96, 3), (40, 5), (8, 2), (1000, 2)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("group_top", [1, 2])
+def test_groups_that_nearly_tie(shape, scoring, biased, group_top):
+    """Groups with the same logits in other orders, but for a step of f32 in
+    one of the two best of some: scores that f32 cannot tell apart."""
+    E, G = shape
+    size = E // G
+    r = np.random.default_rng(E + group_top)
+    rows, b = [], None
+    for t in range(24):
+        base = r.normal(size=size).astype(np.float32) * 1.5 + 2.0
+        z = np.stack([base.copy() for _ in range(G)])
+        for g in range(G):
+            steps, at = int(r.integers(-2, 3)), int(np.argsort(-base)[min(int(r.integers(0, 2)), size - 1)])
+            for _ in range(abs(steps)):
+                z[g, at] = np.nextafter(z[g, at], np.float32(np.inf if steps > 0 else -np.inf))
+            if not biased:
+                z[g] = z[g][r.permutation(size)]
+        rows.append(z.reshape(-1))
+    if biased:  # the same for every group, so that the sums stay near
+        b = torch.tensor(np.tile(r.normal(size=size).astype(np.float32) * 0.1, G), device="cuda")
+    z = torch.tensor(np.stack(rows), device="cuda")
+    top_groups = max(1, G // 2)
+    check(z, min(6, top_groups * size), scoring=scoring, bias=b, groups=G, top_groups=top_groups, group_top=group_top)
+
+
+@pytest.mark.parametrize("shape", [(512, 8), (160, 8), (1024, 4)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_groups_of_equal_experts(shape, biased):
+    """More experts at a group's best score than are looked at singly."""
+    E, G = shape
+    z = torch.ones(5, E, device="cuda")
+    z[1] = 0.5
+    z[2, ::2] = 2.0
+    z[3, E // 2:] = 1.0 + 2.0 ** -23
+    z[4, -1] = 3.0
+    b = torch.full((E,), 0.25, device="cuda") if biased else None
+    for group_top in (1, 2):
+        check(z, 5, scoring="sigmoid", bias=b, groups=G, top_groups=2, group_top=group_top)
