@@ -28,6 +28,8 @@
 // bytes at 6.5 TB/s, or the products at 1.66 PFLOP/s):
 //   8192 x 8192 x 2048 bf16, bias, GELU (tanh)  176-184 us  (165): the MMAs
 //   8192 x 8192 x 8192 bf16                        682 us  (661)
+//   8192 x 8192 x 2048 bf16, f32 out               242 us  (165): the f32
+//     outputs' way out of registers, which the next tile hides in part
 //   4096 x 2048 x 8192 bf16, residual          107-124 us   (83): 128 tiles
 //     in two waves of 74 pairs
 //   64 x 8192 x 2048 bf16, bias, SiLU             12.2 us  (5.4): the first
@@ -447,13 +449,14 @@ __device__ __forceinline__ void finish_run(const LinearArgs& a, int t, int r, co
   if (a.residual != nullptr) add_vec<16>(a.residual, static_cast<long long>(t) * a.res_stride + r, a.res_dtype, p);
   store_pairs<16>(a.y, static_cast<long long>(t) * a.y_stride + r, a.out_dtype, p);
 }
-// finish_run for a whole warp's 32 tokens t0 + lane, 16-bit outputs.  A
-// lane's 64 bytes lie a row's stride from its neighbour's, so they change
-// hands in shared memory (`stage`, 2 KB; 16-byte chunks swapped by the row so
-// that both sides are free of bank conflicts): a store then covers eight
-// tokens' 64 bytes each instead of 16 bytes of 32 tokens, and a 16-bit
-// residual comes in the same way.
+// finish_run for a whole warp's 32 tokens t0 + lane.  A lane's bytes lie a
+// row's stride from its neighbour's, so they change hands in shared memory
+// (`stage`, 2 KB; 16-byte chunks swapped by the row so that both sides are
+// free of bank conflicts): a store then covers eight tokens' 64 bytes each
+// instead of 16 bytes of 32 tokens, and a 16-bit residual comes in the same
+// way.
 constexpr int kRowBytes = 64;
+template <bool F32>
 __device__ __forceinline__ void finish_warp(const LinearArgs& a, int t0, int t_end, int r, const float (&v)[32],
                                             const float* bias, unsigned char* stage, int lane) {
   const auto chunk = [&](int row, int c) {
@@ -491,6 +494,24 @@ __device__ __forceinline__ void finish_warp(const LinearArgs& a, int t0, int t_e
     }
   } else if (a.residual != nullptr && t0 + lane < t_end) {
     add_vec<16>(a.residual, static_cast<long long>(t0 + lane) * a.res_stride + r, a.res_dtype, p);
+  }
+  if (F32) {  // 16 columns at a time
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h > 0) __syncwarp();
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<ulonglong2*>(chunk(lane, c)) = make_ulonglong2(p[8 * h + 2 * c].v, p[8 * h + 2 * c + 1].v);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + 8 * i + row8;
+        if (t < t_end)
+          *reinterpret_cast<uint4*>(static_cast<float*>(a.y) + static_cast<long long>(t) * a.y_stride + r + 16 * h +
+                                    4 * c4) = *chunk(8 * i + row8, c4);
+      }
+    }
+    return;
   }
   uint32_t w[16];
   if (a.out_dtype == kBf16) {
@@ -1082,7 +1103,12 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
 // cycles of MMA, where a CTA alone with 128 x 256 loads 48 KB: the traffic from
 // L2 was what bound that one.  The even CTA issues the MMAs of both; full and
 // acc_empty barriers are its own, commits arrive at empty and acc_full of both.
+// CHUNKED: f32 outputs; a warp carries its 32 rows by 96 columns in registers
+// (128 did not fit: 8192 x 8192 x 2048 271 us, with 96 242 us, on CTAs alone
+// 329 us).
+constexpr int kPairBn = 256, kPairChunkedBn = 192;
 
+template <bool CHUNKED>
 __global__ void __launch_bounds__(kMmaThreads, 1)
     k_linear_pair(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ LinearArgs a) {
@@ -1165,7 +1191,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       bool ok = true;
       const uint32_t idesc = idesc_f16(2 * kBM, a.bn, a.dtype == kBf16);
       const uint64_t desc0 = sw128_desc(smem_u32(ring));
-      for (int u = u0; ok && u < total; u += step, ++ai) {
+      const int chunk = CHUNKED ? a.chunk : a.kblocks;
+      for (int at = 0, u = u0; ok && u < total; ++ai) {
         const int buf = ai & 1;
         if (!__all_sync(kAll, !gave_up(tail) &&
                                   mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u, kWaitNs))) {
@@ -1174,7 +1201,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         }
         tc_fence_after();
         const uint32_t d = tmem + buf * a.bn;
-        for (int kb = 0; kb < a.kblocks; ++kb) {
+        const int end = min(a.kblocks, at + chunk);
+        for (int kb = at; kb < end; ++kb) {
           if (!__all_sync(kAll, mbar_wait_bounded(&tail->full[st], phase, kWaitNs))) {
             give_up(tail);
             ok = false;
@@ -1185,7 +1213,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           if (elect_one()) {
 #pragma unroll
             for (int i = 0; i < kBK / 16; ++i)
-              umma_f16_pair(d, da + 2 * i, db + 2 * i, idesc, (kb > 0 || i > 0) ? 1u : 0u);
+              umma_f16_pair(d, da + 2 * i, db + 2 * i, idesc, (kb > at || i > 0) ? 1u : 0u);
             umma_commit_pair(&tail->empty[st]);
           }
           __syncwarp();
@@ -1196,6 +1224,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         }
         if (ok && elect_one()) umma_commit_pair(&tail->acc_full[buf]);
         __syncwarp();
+        at = end;
+        if (at == a.kblocks) {
+          at = 0;
+          u += step;
+        }
       }
       if (elect_one()) umma_commit_pair(&tail->drained);
       __syncwarp();
@@ -1209,29 +1242,77 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     unsigned char* stage = reinterpret_cast<unsigned char*>(tail + 1) + (warp - 2) * kPairStageBytes;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
     int ai = 0;
-    for (int u = u0; u < total; u += step, ++ai) {
+    bool ok = true;
+    for (int u = u0; ok && u < total; u += step) {
       const Tile w = tile_of(a, u, 2 * kBM);
       const int t0 = w.p0 + static_cast<int>(rank) * kBM + 32 * q;  // this warp's tokens
       const int valid = min(a.bn, a.q_rows - w.q0);
-      const int buf = ai & 1;
       const float* bias = fetch_bias(a, tail->bias[warp - 2], w.q0, set, 2, lane);
-      const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, kWaitNs);
-      if (!__all_sync(kAll, got)) {
-        if (lane == 0) give_up(tail);
-        break;
-      }
-      tc_fence_after();
-      for (int c0 = 32 * set; c0 < a.bn; c0 += 64) {
-        float v[32];
-        tmem_ld32(lane_base + buf * a.bn + c0, v);
+      const auto finish = [&](int c0, const float(&v)[32]) {
         if (a.vec && c0 + 32 <= valid)
-          finish_warp(a, t0, a.p_rows, w.q0 + c0, v, bias != nullptr ? bias + c0 / 64 * 32 : nullptr, stage, lane);
+          finish_warp<CHUNKED>(a, t0, a.p_rows, w.q0 + c0, v, bias != nullptr ? bias + c0 / 64 * 32 : nullptr, stage,
+                               lane);
         else
           finish_block(a, t0, w.q0 + c0, a.p_rows, w.q0 + valid, v, reinterpret_cast<float*>(stage), lane);
+      };
+      const auto await = [&](int buf) {
+        const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, kWaitNs);
+        if (!__all_sync(kAll, got)) {
+          if (lane == 0) give_up(tail);
+          return false;
+        }
+        tc_fence_after();
+        return true;
+      };
+      const auto release = [&](int buf) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_at(at_rank(&tail->acc_empty[buf], 0));
+      };
+      if (!CHUNKED) {
+        const int buf = ai & 1;
+        if (!await(buf)) break;
+        for (int c0 = 32 * set; c0 < a.bn; c0 += 64) {
+          float v[32];
+          tmem_ld32(lane_base + buf * a.bn + c0, v);
+          finish(c0, v);
+        }
+        release(buf);
+        ++ai;
+      } else {
+        constexpr int kGroups = kPairChunkedBn / 64;  // 32-column groups of this warp
+        float acc[kGroups][32];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[g][j] = 0.0f;
+        for (int k = 0; k < a.kblocks; k += a.chunk, ++ai) {
+          const int buf = ai & 1;
+          if (!await(buf)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+              float v[16];
+              tmem_ld16(lane_base + buf * a.bn + 32 * set + 64 * g + h, v);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) acc[g][h + j] = __fadd_rn(acc[g][h + j], v[j]);
+            }
+          }
+          release(buf);
+        }
+        if (!ok) break;
+#pragma unroll 1
+        for (int g = 0; g < kGroups; ++g) {
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = g == 0 ? acc[0][j] : g == 1 ? acc[1][j] : acc[2][j];
+          if (32 * set + 64 * g < valid) finish(32 * set + 64 * g, v);
+        }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_at(at_rank(&tail->acc_empty[buf], 0));
     }
   }
   __syncwarp();
@@ -1468,7 +1549,9 @@ struct Plan {
 // partial tiles cost 1.2 us and more with their width, the last tile's
 // epilogue in a CTA 0.6 us and 5 ns per column.  The ring is 96 KB, so
 // that the next launch's CTAs can move in beside this one's; 200 KB was no
-// faster but for the pair and for CTAs that run through many tiles.
+// faster but for the pair and for CTAs that run through many tiles.  f32
+// outputs, which leave from registers, cost CTAs with several tiles 24 ns per
+// column and tile more, and the pair 6 us per tile.
 // Measured against the best of a sweep (us): 64 x 8192 x 2048 10.5 / 10.5,
 // 128 x 2048 x 2048 8.1 / 8.1, 512 x 2048 x 2048 11.0 / 11.0.
 Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const ClusterRoom& room) {
@@ -1479,6 +1562,7 @@ Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const Clust
     const double waves = static_cast<double>((tiles * splits + sms - 1) / sms);
     const double stage = (kABytes + 128.0 * bn) / rate;
     double t = waves * ((kblocks + splits - 1) / splits) * stage + waves * 5.0 * bn + 600.0;
+    if (chunked && splits == 1 && waves > 1) t += waves * 24.0 * bn;
     if (splits > 1) t += 1200.0 + 10.0 * bn;
     else if (swap) t += waves * 10.0 * bn;  // narrow stores
     if (t < best.ns) {
@@ -1512,15 +1596,16 @@ Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const Clust
     consider(false, n, tokens128 * ((a.rows + n - 1) / n), 1);
     if (n < bn) break;
   }
-  if (tma && !chunked && a.tokens > 128 && a.rows > 128) {
-    const long long tiles = static_cast<long long>((a.tokens + 255) / 256) * ((a.rows + 255) / 256);
+  if (tma && a.tokens > 128 && a.rows > 128) {
+    const int bn = chunked ? kPairChunkedBn : kPairBn;
+    const long long tiles = static_cast<long long>((a.tokens + 255) / 256) * ((a.rows + bn - 1) / bn);
     const double waves = static_cast<double>((tiles + sms / 2 - 1) / (sms / 2));
-    const double t = waves * kblocks * 270.0 + 600.0 + 5.0 * 256 * 2;
+    const double t = waves * (kblocks * 270.0 * bn / kPairBn + (chunked ? 6000.0 : 0.0)) + 600.0 + 5.0 * bn * 2;
     if (t < best.ns) {
       best.ns = t;
       best.pair = true;
       best.swap = false;
-      best.bn = 256;
+      best.bn = bn;
       best.splits = 1;
       best.ring = 200 * 1024;
     }
@@ -1614,7 +1699,8 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
   }
   if (plan.pair) {
     const int grid = 2 * static_cast<int>(std::min<long long>(tiles, dev.sms / 2));
-    return launch<k_linear_pair>(grid, kMmaThreads, smem, 2, st, mp, mq, a);
+    return chunked ? launch<k_linear_pair<true>>(grid, kMmaThreads, smem, 2, st, mp, mq, a)
+                   : launch<k_linear_pair<false>>(grid, kMmaThreads, smem, 2, st, mp, mq, a);
   }
   const int grid = a.splits > 1 ? static_cast<int>(tiles) * a.splits
                                 : static_cast<int>(std::min<long long>(tiles, dev.sms));

@@ -293,3 +293,15 @@ def test_rows_at_odd_addresses_amid_nan(size, out, shift):
     y = torch.full((T, N), math.nan, device="cuda", dtype=DTYPES[out])
     check(w, x, y, normal(3, N, dtype="f32"), "silu", normal(4, T, N, dtype="f16"))
     check(w, x, y)
+
+
+@pytest.mark.parametrize("size", [(2600, 2312, 200), (4097, 4090, 136), (3000, 3000, 1032), (8192, 1600, 520), (2100, 8000, 64)])
+def test_f32_outputs_of_many_tiles(size):
+    case(*size, out="f32")
+    case(*size, out="f32", bias="bf16", activation="gelu", residual="bf16")
+    case(*size, dtype="f16", out="f32", activation="silu", residual="f32")
+    T, N, K = size  # outputs and residual at odd addresses
+    w, x = normal(1, N, K, std=1 / math.sqrt(K)), normal(2, T, K)
+    y = torch.full((T + 1, N + 5), 7.0, device="cuda")
+    check(w, x, y[:T, 3:3 + N], normal(3, N), "none", normal(4, T, N + 1)[:, 1:])
+    assert bool((y[T:] == 7).all()) and bool((y[:, :3] == 7).all()) and bool((y[:, 3 + N:] == 7).all())
