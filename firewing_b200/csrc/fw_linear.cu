@@ -556,9 +556,19 @@ __device__ __forceinline__ void finish_four(const LinearArgs& a, int t, int r, f
   unpack(p[1], &o[2], &o[3]);
   if (a.residual != nullptr) {
     const long long at = static_cast<long long>(t) * a.res_stride + r;
+    if (a.res_dtype == kF32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) o[i] = __fadd_rn(o[i], load_f32(a.residual, at + i, a.res_dtype));
+      for (int i = 0; i < 4; ++i)
+        if (i < n) o[i] = __fadd_rn(o[i], static_cast<const float*>(a.residual)[at + i]);
+    } else {
+      uint16_t raw[4] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < n) raw[i] = static_cast<const uint16_t*>(a.residual)[at + i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        o[i] = __fadd_rn(o[i], a.res_dtype == kBf16 ? bf16_to_f32(raw[i]) : __half2float(__ushort_as_half(raw[i])));
+    }
   }
   const long long at = static_cast<long long>(t) * a.y_stride + r;
   if (a.vec && a.out_dtype != kF32 && n >= 4) {
@@ -605,15 +615,38 @@ __device__ __forceinline__ void finish_block(const LinearArgs& a, int p0, int q0
 #pragma unroll
     for (int i = 0; i < 4; ++i) unpack(p[i], &o[2 * i], &o[2 * i + 1]);
     if (a.residual != nullptr) {
+      // The type is asked for once, so that the eight loads are under way
+      // together.
+      const long long from = static_cast<long long>(t) * a.res_stride + r, apart_by = a.res_stride * step;
+      float v8[8] = {};
+      if (a.res_dtype == kF32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (t + i * step < t_end) v8[i] = static_cast<const float*>(a.residual)[from + i * apart_by];
+      } else {
+        uint16_t raw[8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (t + i * step < t_end) raw[i] = static_cast<const uint16_t*>(a.residual)[from + i * apart_by];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v8[i] = a.res_dtype == kBf16 ? bf16_to_f32(raw[i]) : __half2float(__ushort_as_half(raw[i]));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = __fadd_rn(o[i], v8[i]);
+    }
+    const long long first = static_cast<long long>(t) * a.y_stride + r, on = a.y_stride * step;
+    if (a.out_dtype == kF32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (t + i * step < t_end) static_cast<float*>(a.y)[first + i * on] = o[i];
+    } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (t + i * step < t_end)
-          o[i] = __fadd_rn(o[i], load_f32(a.residual, static_cast<long long>(t + i * step) * a.res_stride + r, a.res_dtype));
+          static_cast<uint16_t*>(a.y)[first + i * on] =
+              a.out_dtype == kBf16 ? f32_to_bf16(o[i]) : __half_as_ushort(__float2half_rn(o[i]));
     }
-    const long long first = static_cast<long long>(t) * a.y_stride + r, on = a.y_stride * step;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (t + i * step < t_end) store_f32(a.y, first + i * on, a.out_dtype, o[i]);
   }
 }
 
