@@ -450,11 +450,14 @@ __global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_
   if (tid == 0) sm.short_count = sm.merged_count = 0;
   // The warp's reference M, its maximum so far.  With mc =
   // fl(M c) the terms are y = fma(z, c, -mc), which is (z - M) c + off for
-  // one small `off` common to the warp: taken out again at the end.  Values
+  // one `off` common to the warp, the rounding of M c: taken out again at the
+  // end.  It is half a step of mc at most, so mc is held below 2^24: |off| <=
+  // 1/2, and neither 2^off nor a term that counts leaves f32's range.  Values
   // are raised to `least`, far enough below M for 2^y to be 0, so that a
   // masked -inf adds 0 * y = 0.  Where the type has no such number (M near
-  // its lowest value, or a high temperature), or M c overflows, `plain` terms
-  // are computed as max((z - M) c, kLowest).
+  // its lowest value, or a high temperature), or M c is larger (rows of far
+  // logits, a low temperature, a warp that has seen nothing but a mask of
+  // -1e9), `plain` terms are computed as max((z - M) c, kLowest).
   float m = -INFINITY, mc = 0.0f, least = 0.0f;
   bool plain = false;
   F2 s2 = pack(0.0f, 0.0f), w2 = pack(0.0f, 0.0f);  // the lane's sums, even and odd elements
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_
     m = to;
     mc = __fmul_rn(m, c);
     least = R::at_least(__fsub_rn(m, a.depth));
-    plain = !(fabsf(mc) < 1e30f && __fmul_rn(__fsub_rn(least, m), c) < -1000.0f);
+    plain = !(fabsf(mc) < 0x1p24f && __fmul_rn(__fsub_rn(least, m), c) < -1000.0f);
     if (!plain) {  // the sums go on against the rounded reference
       const float off = __fmaf_rn(m, c, -mc);
       const F2 f = pack(ex2(off), ex2(off));

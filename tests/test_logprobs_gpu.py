@@ -262,3 +262,47 @@ def test_one_token_allowed():
         lp, h, ti, tl = run(z, at.to(torch.int32)[:, None].contiguous(), 1, temperature=0.7)
         assert (lp == 0).all() and (h == 0).all() and (tl == 0).all()
         assert (ti[:, 0] == at.cpu().numpy()).all()
+
+
+def far_rows(seed, tokens, vocab, mask, dtype="f32"):
+    """Rows filtered with a finite mask: in places, all but the last three, a
+    first half, everything (a uniform row), all but one, a second half."""
+    z = normal(seed, tokens, vocab, dtype=dtype)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    gone = torch.rand(tokens, vocab, generator=g, device="cuda") < 0.5
+    at = torch.arange(vocab, device="cuda")
+    for t in range(tokens):
+        kind = t % 6
+        if kind:
+            gone[t] = (at < vocab - 3, at < vocab // 2, at >= 0, at != vocab // 3, at >= vocab // 2)[kind - 1]
+    return z.masked_fill_(gone, mask)
+
+
+@pytest.mark.parametrize("mask", [-1e8, -1e9, -1e10, -1.3e10, -1e11, -1e12, -1e20, -1e30])
+@pytest.mark.parametrize("temperature", [1.0, 0.3, 0.1])
+def test_rows_filtered_with_a_finite_mask(mask, temperature):
+    for tokens, vocab in ((6, 50), (12, 5003), (6, 9001), (6, 131072)):
+        check(far_rows(20, tokens, vocab, mask), 8, temperature=temperature)
+    check(far_rows(21, 6, 5000, mask, "bf16"), 8, temperature=temperature)
+    store = torch.full((6, 9100), mask, device="cuda")  # heads and tails that are no whole vectors
+    store[:, 3:9004] = far_rows(22, 6, 9001, mask)
+    check(store[:, 3:9004], 8, temperature=temperature)
+
+
+def test_many_rows_filtered_with_a_finite_mask():
+    check(far_rows(23, 450, 9001, -1e10), 8)
+    check(far_rows(24, 450, 4096, -3e9), 8, temperature=0.3)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("size,temperature", [(6500.0, 1e-6), (30000.0, 1e-5), (1e4, 1e-4), (3.0, 1e-6), (50.0, 1e6),
+                                              (1e10, 1.0), (1e11, 1.0), (1e9, 0.01), (1e12, 1e6)])
+def test_far_logits_and_temperatures(dtype, size, temperature):
+    if dtype == "f16" and size > 6e4:
+        size = 6e4
+    for tokens, vocab in ((3, 7), (5, 3001), (450, 9001), (4, 60000)):
+        z = normal(25, tokens, vocab, std=1.0, dtype="f32").clamp_(-4, 4)
+        z[0] = z[0].abs() * 0.2 * size + 0.1 * size  # every value far off on one side
+        z[1] = -size - z[1].abs() * 2.0 ** -22 * size  # a few steps of f32 apart
+        z[2:] *= size / 5
+        check(z.to(DTYPES[dtype]), min(5, vocab), temperature=temperature)
