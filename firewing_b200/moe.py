@@ -458,6 +458,8 @@ def route_bf16(logits, tokens: int, experts: int, top_k: int, indices, scores, s
 
 
 # ---- primitives over torch tensors: shapes, types and strides are the tensors' own ----
+# `stream`: a torch.cuda.Stream or a cudaStream_t handle, by default PyTorch's
+# current stream on the tensors' device (0 is the legacy default stream).
 
 _torch = None  # imported with the first call
 _dtype_codes: dict = {}
@@ -524,6 +526,14 @@ def _columns(t, name: str) -> int:
         raise ValueError(f"{name} must be a 2-D tensor") from None
 
 
+def _stream_of(stream, device: int) -> int:
+    """Handle of `stream`, by default PyTorch's current one on `device`: the
+    stream on which the tensors' other operations are."""
+    if stream is None:
+        return _torch._C._cuda_getCurrentRawStream(device)
+    return _stream(stream)
+
+
 def _call(device: int, function, *args) -> None:
     """The C entry point on `device`, which stays current only for the call."""
     if _torch.cuda.current_device() == device:
@@ -570,12 +580,14 @@ def linear_epilogue(w, x, y, bias=None, activation: str = "none", residual=None,
         return
     c = _LinearConfig(N, K, code, out, bcode, rcode, act, ws, xs, rs, ys)
     _call(dev, library().fw_linear_epilogue, ctypes.byref(c), w.data_ptr(), x.data_ptr(), T, pb, pr, y.data_ptr(),
-          _stream(stream))
+          _stream_of(stream, dev))
 
 
 def primitive_status(stream=None) -> None:
-    """Wait for `stream` and raise FwError if a linear_epilogue kernel on the
-    current device gave up a bounded wait."""
+    """Wait for `stream` (by default PyTorch's current one) and raise FwError if
+    a linear_epilogue kernel on the current device gave up a bounded wait."""
+    if _torch is not None:  # (else none of them has run)
+        stream = _stream_of(stream, _torch.cuda.current_device())
     _check(library().fw_primitive_status(_stream(stream)))
 
 
@@ -605,7 +617,8 @@ def route_scores(logits, indices, weights, scoring: str = "softmax", bias=None, 
     if T == 0 and counts is None:
         return
     c = _RouteConfig(E, K, code, score, groups, top_groups, group_top, 1 if renormalize else 0, scale, stride)
-    _call(dev, library().fw_route_scores, ctypes.byref(c), logits.data_ptr(), T, pb, pi, pw, pc, _stream(stream))
+    _call(dev, library().fw_route_scores, ctypes.byref(c), logits.data_ptr(), T, pb, pi, pw, pc,
+          _stream_of(stream, dev))
 
 
 def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_idx=None, top_logprobs=None,
@@ -638,7 +651,7 @@ def token_logprobs(logits, targets=None, logprobs=None, entropy=None, top_idx=No
         return
     c = _LogprobConfig(V, code, C, K, temperature, stride)
     _call(dev, library().fw_token_logprobs, ctypes.byref(c), logits.data_ptr(), T, pt, pl, pe, pi, pq,
-          _stream(stream))
+          _stream_of(stream, dev))
 
 
 def topk_bf16(values: np.ndarray, k: int):

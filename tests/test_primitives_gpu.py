@@ -112,3 +112,44 @@ def test_two_threads():
     assert not failed, failed
     with pytest.raises(fw.FwError):
         fw.token_logprobs(z, entropy=want[0], temperature=0.0)
+
+
+def three_calls(x, w, z, **kw):
+    y = torch.zeros(48, 700, device="cuda")
+    r, v = torch.zeros(48, 8, device="cuda", dtype=torch.int32), torch.zeros(48, 8, device="cuda")
+    h = torch.zeros(40, device="cuda")
+    fw.linear_epilogue(w, x, y, **kw)
+    fw.route_scores(y, r, v, **kw)
+    fw.token_logprobs(z, entropy=h, **kw)
+    return y, r, v, h
+
+
+def test_the_current_stream_is_the_default():
+    w = torch.randn(700, 1024, device="cuda").bfloat16()
+    x, z = torch.randn(48, 1024, device="cuda").bfloat16(), torch.randn(40, 30001, device="cuda")
+    want = three_calls(x, w, z)
+    torch.cuda.synchronize()
+    # operands that the current stream writes late
+    late_x, late_z = torch.zeros_like(x), torch.zeros_like(z)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(40_000_000)
+        late_x.copy_(x)
+        late_z.copy_(z)
+        got = three_calls(late_x, w, late_z)
+        fw.primitive_status()
+        assert s.query()  # the stream that it waits for
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # a stream that is given goes first
+    with torch.cuda.stream(s):
+        got = three_calls(x, w, z, stream=s.cuda_stream)
+        s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # and so inside a capture
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = three_calls(x, w, z)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
