@@ -386,6 +386,25 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? kRouteResident : 
     }
     nan_bias = __syncthreads_or(nan_bias);
   }
+  // A group's score may be small and its two keys large, with their error: of
+  // opposite signs they take away from each other no more than the positive
+  // one, at most the largest bias + 1, or the other one, at most the size of
+  // the lowest bias that is a number.
+  __shared__ float bias_most[kRouteWarps], bias_least[kRouteWarps];
+  if (biased && grouped && a.group_top == 2) {
+    float most = -INFINITY, least = INFINITY;
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+      most = fmaxf(most, biases[e]);
+      if (biases[e] > -INFINITY) least = fminf(least, biases[e]);
+    }
+    most = warp_max(most);
+    least = -warp_max(-least);
+    if (lane == 0) {
+      bias_most[warp] = most;
+      bias_least[warp] = least;
+    }
+    __syncthreads();
+  }
 
   for (int t = first; t < a.tokens; t += step) {
     const long long row = t * a.stride;
@@ -473,6 +492,15 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? kRouteResident : 
           spread = 1;  // (widened where the 64-bit functions need it)
         } else {
           chosen = choose_groups<float>(keys, a, lanes, lane, &gap, &high);
+        }
+        if (biased && a.group_top == 2) {
+          float most = bias_most[0], least = bias_least[0];
+#pragma unroll
+          for (int i = 1; i < kRouteWarps; ++i) {
+            most = fmaxf(most, bias_most[i]);
+            least = fminf(least, bias_least[i]);
+          }
+          high = __fmaf_rn(2.0f, fmaxf(fminf(__fadd_rn(most, 1.0f), -least), 0.0f), high);
         }
         if (!(gap > 2.0f * (a.group_top * error + 3.0f * kAddError * high))) {
           if (softmax) sum64 = softmax_sum_in_64_bits(a.logits, DT, row, E, top64, lane);

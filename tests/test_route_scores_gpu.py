@@ -297,3 +297,21 @@ def test_groups_of_equal_experts(shape, biased):
     b = torch.full((E,), 0.25, device="cuda") if biased else None
     for group_top in (1, 2):
         check(z, 5, scoring="sigmoid", bias=b, groups=G, top_groups=2, group_top=group_top)
+
+
+@pytest.mark.parametrize("shape", [(64, 32), (128, 4), (256, 8), (160, 8), (512, 8), (40, 5)])
+@pytest.mark.parametrize("scoring,largest,noise", [("softmax", 4.0, 1e-4), ("softmax", 128.0, 1e-4),
+                                                   ("sigmoid", 16.0, 1e-5), ("sigmoid", 128.0, 1e-5)])
+def test_groups_whose_two_best_keys_cancel(shape, scoring, largest, noise):
+    """A group's two best keys are b + s and -b + s': their sum is small, its
+    error in f32 that of b."""
+    E, G = shape
+    size = E // G
+    r = np.random.default_rng(E)
+    for _ in range(4):
+        z = (0.3 + noise * r.normal(size=(40, E))).astype(np.float32)
+        b = np.full((G, size), -1000.0, np.float32)
+        b[:, 0] = r.uniform(largest / 2, largest, size=G)
+        b[:, 1] = -b[:, 0]
+        check(torch.tensor(z, device="cuda"), min(4, size), scoring=scoring, groups=G, top_groups=max(1, G // 2),
+              group_top=2, bias=torch.tensor(b.reshape(-1), device="cuda"))
