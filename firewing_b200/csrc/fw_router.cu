@@ -93,7 +93,8 @@ __device__ __forceinline__ T warp_sum(T v) {
 }
 
 // The groups to choose from, as a mask with bit g * lanes set, from the
-// groups' scores (group g's in lane g * lanes).  *gap: the lowest chosen
+// groups' scores (group g's in lane g * lanes; -inf: a group of dead experts,
+// so that an f32 sum below kLowest is passed as kLowest).  *gap: the lowest chosen
 // group's score minus the highest other one's (+inf when there is none),
 // *high the largest magnitude of the scores compared.
 template <typename F>
@@ -141,7 +142,8 @@ __device__ __forceinline__ unsigned choose_groups(const F* keys, const RouteScor
     m2 = fmax(fmin(m1, o1), fmax(m2, o2));
     m1 = fmax(m1, o1);
   }
-  const F score = (a.group_top == 2 && m2 > none) ? m1 + m2 : m1;
+  F score = m1;
+  if (a.group_top == 2 && m2 > none) score = sizeof(F) == 4 ? fmaxf(m1 + m2, kLowest) : m1 + m2;
   return rank_groups<F>(g < a.groups && l == 0 ? score : none, a, lanes, lane, gap, high);
 }
 
@@ -461,7 +463,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NE <= 16 ? kRouteResident : 
               if (a.group_top == 2) {
                 const unsigned who = __ballot_sync(kAll, m1 == best);
                 const float second = warp_max(lane == __ffs(who) - 1 ? m2 : m1);
-                if (second > -INFINITY) value = __fadd_rn(best, second);
+                if (second > -INFINITY) value = fmaxf(__fadd_rn(best, second), kLowest);
               }
               if (lane == i >> shift) score = value;
               m1 = m2 = -INFINITY;

@@ -315,3 +315,32 @@ def test_groups_whose_two_best_keys_cancel(shape, scoring, largest, noise):
         b[:, 1] = -b[:, 0]
         check(torch.tensor(z, device="cuda"), min(4, size), scoring=scoring, groups=G, top_groups=max(1, G // 2),
               group_top=2, bias=torch.tensor(b.reshape(-1), device="cuda"))
+
+
+@pytest.mark.parametrize("shape", [(64, 8), (128, 4), (40, 5)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_groups_masked_by_the_lowest_value(shape, scoring):
+    """Two keys near f32's lowest value add up to less than it; they are still
+    ahead of a group without experts, and have an order."""
+    E, G = shape
+    size = E // G
+    low = torch.finfo(torch.float32).min
+    z = normal(30, 6, E)
+    z[:, :size] = -math.inf  # the first group: nobody
+    z[5, size:2 * size] = -math.inf
+    for masks in ((low, low, 0.0), (low, 0.75 * low, 0.0), (0.75 * low, low, 0.6 * low), (low, low, low)):
+        b = torch.zeros(G, size, device="cuda")
+        b[1:] = masks[2]
+        for g, m in enumerate(masks):
+            b[1 + g] = m
+        for top_groups in range(1, G + 1):
+            for group_top in (1, 2):
+                check(z, min(6, size), scoring=scoring, bias=b.reshape(-1).contiguous(), groups=G, top_groups=top_groups,
+                      group_top=group_top)
+    high = torch.finfo(torch.float32).max
+    b = torch.zeros(G, size, device="cuda")
+    b[1:] = high
+    b[2] = 0.75 * high
+    for top_groups in range(1, G + 1):
+        check(z, min(6, size), scoring=scoring, bias=b.reshape(-1).contiguous(), groups=G, top_groups=top_groups,
+              group_top=2)
