@@ -32,6 +32,7 @@ from .moe import (  # noqa: F401
     library_path,
     linear_bf16,
     linear_epilogue,
+    primitive_set_wait_limit,
     primitive_status,
     route_bf16,
     route_scores,

@@ -1378,6 +1378,13 @@ int fw_linear_epilogue(const fw_linear_config* c, const void* w, const void* x, 
   return FW_OK;
 }
 
+int fw_primitive_set_wait_limit(uint64_t nanoseconds) {
+  if (nanoseconds < 1000000ull || nanoseconds > 60000000000ull)
+    return fail(FW_EINVAL, "the wait limit must be between 1 ms and 60 s");
+  fw::set_linear_wait_limit(nanoseconds);
+  return FW_OK;
+}
+
 int fw_primitive_status(void* stream) {
   int code = 0;
   const cudaError_t e = fw::take_linear_status(&code, static_cast<cudaStream_t>(stream));

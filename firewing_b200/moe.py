@@ -150,6 +150,7 @@ def library() -> ctypes.CDLL:
     L.fw_route_scores.argtypes = [ctypes.POINTER(_RouteConfig), vp, ctypes.c_int32, vp, vp, vp, vp, vp]
     L.fw_linear_epilogue.argtypes = [ctypes.POINTER(_LinearConfig), vp, vp, ctypes.c_int32, vp, vp, vp, vp]
     L.fw_primitive_status.argtypes = [vp]
+    L.fw_primitive_set_wait_limit.argtypes = [ctypes.c_uint64]
     L.fw_token_logprobs.argtypes = [ctypes.POINTER(_LogprobConfig), vp, ctypes.c_int32, vp, vp, vp, vp, vp, vp]
     L.fw_moe_forward_noalloc.argtypes = [ctypes.POINTER(_Config), ctypes.POINTER(_Weights), vp,
                                          ctypes.c_int32, vp, vp, vp, vp]
@@ -165,6 +166,7 @@ def library() -> ctypes.CDLL:
                  "fw_moe_load_expert_container", "fw_codec_container_check",
                  "fw_linear_bf16", "fw_swiglu_bf16", "fw_add_bf16", "fw_route_bf16", "fw_moe_forward_noalloc",
                  "fw_route_scores", "fw_token_logprobs", "fw_linear_epilogue", "fw_primitive_status",
+                 "fw_primitive_set_wait_limit",
                  "fw_moe_ep_set_transport", "fw_moe_set_wait_limit", "fw_moe_test_stall"):
         getattr(L, name).restype = ctypes.c_int
     _lib = L
@@ -589,6 +591,12 @@ def primitive_status(stream=None) -> None:
     if _torch is not None:  # (else none of them has run)
         stream = _stream_of(stream, _torch.cuda.current_device())
     _check(library().fw_primitive_status(_stream(stream)))
+
+
+def primitive_set_wait_limit(seconds: float) -> None:
+    """Bound of each device-side wait of linear_epilogue's kernels launched from
+    now on, 1 ms to 60 s (2 s until set)."""
+    _check(library().fw_primitive_set_wait_limit(int(seconds * 1e9)))
 
 
 def route_scores(logits, indices, weights, scoring: str = "softmax", bias=None, groups: int = 1,

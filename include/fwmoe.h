@@ -487,6 +487,13 @@ int fw_linear_epilogue(const fw_linear_config* config, const void* w, const void
  * kernels gave up a bounded wait (its y is then incomplete). */
 int fw_primitive_status(void* stream);
 
+/* Bound of each wait of fw_linear_epilogue's kernels, 1 ms to 60 s (2 s until
+ * set), for the launches of this process from now on (a captured launch keeps
+ * its own).  A wait is for one step of a product, not for all of it, so that
+ * the limit says nothing about how long a product may take.  FW_EINVAL outside
+ * the range. */
+int fw_primitive_set_wait_limit(uint64_t nanoseconds);
+
 /* Drop-in for the reference's only C ABI on the path,
  * `bool firewing_torch_topk_bf16(const uint16_t*, size_t, size_t, size_t*)`
  * (native/topk_shim.cpp:18-44, bound at src/decoder_layer.rs:19-39): HOST

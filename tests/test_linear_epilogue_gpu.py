@@ -305,3 +305,26 @@ def test_f32_outputs_of_many_tiles(size):
     y = torch.full((T + 1, N + 5), 7.0, device="cuda")
     check(w, x, y[:T, 3:3 + N], normal(3, N), "none", normal(4, T, N + 1)[:, 1:])
     assert bool((y[T:] == 7).all()) and bool((y[:, :3] == 7).all()) and bool((y[:, 3 + N:] == 7).all())
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_the_wait_limit_bounds_steps_and_not_the_product(out):
+    """A product that takes several times the limit of its waits (14 ms at the
+    least for 2.3e13 operations; pairs of CTAs)."""
+    T, N, K = 16384, 22528, 32768
+    w, x = normal(1, N, K, std=1 / math.sqrt(K)), normal(2, T, K)
+    want, y = (torch.full((T, N), math.nan, device="cuda", dtype=DTYPES[out]) for _ in range(2))
+    fw.linear_epilogue(w, x, want)
+    torch.cuda.synchronize()
+    fw.primitive_set_wait_limit(0.003)
+    try:
+        fw.linear_epilogue(w, x, y)
+        torch.cuda.synchronize()
+        fw.primitive_status()
+    finally:
+        fw.primitive_set_wait_limit(2.0)
+    assert torch.equal(y, want)
+    rows = torch.arange(0, T, T // 64, device="cuda")
+    part, err = reference(w, x[rows], None, "none", None)
+    half_step = torch.finfo(y.dtype).eps / 2
+    assert bool(((y[rows].double() - part).abs() <= err * (1 + half_step) + half_step * part.abs()).all())

@@ -113,3 +113,11 @@ def test_the_linear_binding_takes_tensors_of_one_gpu():
         fw.linear_epilogue(w, x, y)
     with pytest.raises(ValueError, match="activation"):
         fw.linear_epilogue(w, x, y, activation="tanh")
+
+
+@pytest.mark.parametrize("seconds", [0.0, 1e-6, 61.0])
+def test_the_products_wait_limit_has_bounds(seconds):
+    with pytest.raises(fw.FwError) as e:
+        fw.primitive_set_wait_limit(seconds)
+    assert e.value.code == fw.FW_EINVAL
+    fw.primitive_set_wait_limit(2.0)
