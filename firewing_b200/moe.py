@@ -468,6 +468,7 @@ _dtype_codes: dict = {}
 _16_BITS = (DTYPE_BF16, DTYPE_F16)
 _FLOATS = (DTYPE_BF16, DTYPE_F16, DTYPE_F32)
 _INT32 = -1
+_MOST = 2 ** 31 - 1  # of a size or a count: the C interface's int32, which ctypes would cut off without a word
 
 
 def _import_torch() -> None:
@@ -496,6 +497,8 @@ def _rows(t, name: str, codes: tuple, device: int = -1):
         raise ValueError(f"{name} is on another device")
     if s1 != 1 and c > 1:
         raise ValueError(f"{name} must have consecutive columns")
+    if r > _MOST or c > _MOST:
+        raise ValueError(f"{name}: a size is above 2^31 - 1")
     if r <= 1:
         s0 = c
     elif s0 < c:
@@ -523,9 +526,12 @@ def _dense(t, name: str, code: int, shape: tuple, device: int) -> Optional[int]:
 
 def _columns(t, name: str) -> int:
     try:
-        return t.shape[1] if t.dim() == 2 else -1
+        c = t.shape[1] if t.dim() == 2 else -1
     except (AttributeError, IndexError):
         raise ValueError(f"{name} must be a 2-D tensor") from None
+    if c > _MOST:
+        raise ValueError(f"{name}: a size is above 2^31 - 1")
+    return c
 
 
 def _stream_of(stream, device: int) -> int:
@@ -622,6 +628,8 @@ def route_scores(logits, indices, weights, scoring: str = "softmax", bias=None, 
     pi = _dense(indices, "indices", _INT32, (T, K), dev)
     pw = _dense(weights, "weights", DTYPE_F32, (T, K), dev)
     pc = _dense(counts, "counts", _INT32, (E,), dev)
+    if max(groups, top_groups, group_top) > _MOST or min(groups, top_groups, group_top) < -_MOST:
+        raise ValueError("groups, top_groups and group_top: a number is beyond 2^31 - 1")
     if T == 0 and counts is None:
         return
     c = _RouteConfig(E, K, code, score, groups, top_groups, group_top, 1 if renormalize else 0, scale, stride)

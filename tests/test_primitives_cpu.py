@@ -121,3 +121,67 @@ def test_the_products_wait_limit_has_bounds(seconds):
         fw.primitive_set_wait_limit(seconds)
     assert e.value.code == fw.FW_EINVAL
     fw.primitive_set_wait_limit(2.0)
+
+
+class Sized:
+    """What the bindings look at before a call, of a tensor on the current GPU."""
+
+    def __init__(self, *shape, dtype):
+        import torch
+
+        self.shape, self.dtype, self.strides = torch.Size(shape), getattr(torch, dtype), [1]
+        for n in shape[:0:-1]:
+            self.strides.insert(0, self.strides[0] * n)
+
+    def stride(self):
+        return tuple(self.strides)
+
+    def dim(self):
+        return len(self.shape)
+
+    def get_device(self):
+        return 0
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return FAKE
+
+
+BIG = (1 << 32) + 1  # one, to an int32
+
+
+@pytest.fixture
+def no_call(monkeypatch):
+    pytest.importorskip("torch")
+    monkeypatch.setattr(moe, "_call", lambda *a: pytest.fail("reached the library"))
+    monkeypatch.setattr(moe, "_stream_of", lambda stream, device: 0, raising=False)
+
+
+@pytest.mark.parametrize("T,N,K", [(BIG, 1, 1), (1, BIG, 1), (1, 1, BIG)])
+def test_linear_sizes_beyond_the_interface_are_refused(no_call, T, N, K):
+    w, x, y = Sized(N, K, dtype="bfloat16"), Sized(T, K, dtype="bfloat16"), Sized(T, N, dtype="bfloat16")
+    with pytest.raises(ValueError, match="2\\^31"):
+        fw.linear_epilogue(w, x, y)
+
+
+@pytest.mark.parametrize("T,E,K", [(BIG, 4, 1), (1, BIG, 1), (1, 4, BIG)])
+def test_route_sizes_beyond_the_interface_are_refused(no_call, T, E, K):
+    with pytest.raises(ValueError, match="2\\^31"):
+        fw.route_scores(Sized(T, E, dtype="float32"), Sized(T, K, dtype="int32"), Sized(T, K, dtype="float32"))
+
+
+@pytest.mark.parametrize("name", ["groups", "top_groups", "group_top"])
+@pytest.mark.parametrize("value", [BIG, 1 - (1 << 32)])
+def test_route_numbers_beyond_the_interface_are_refused(no_call, name, value):
+    with pytest.raises(ValueError, match="2\\^31"):
+        fw.route_scores(Sized(2, 4, dtype="float32"), Sized(2, 1, dtype="int32"), Sized(2, 1, dtype="float32"),
+                        **{name: value})
+
+
+@pytest.mark.parametrize("T,V,C,K", [(BIG, 2, 1, 1), (1, BIG, 1, 1), (1, 2, BIG, 1), (1, 2, 1, BIG)])
+def test_logprob_sizes_beyond_the_interface_are_refused(no_call, T, V, C, K):
+    with pytest.raises(ValueError, match="2\\^31"):
+        fw.token_logprobs(Sized(T, V, dtype="float32"), Sized(T, C, dtype="int32"), Sized(T, C, dtype="float32"),
+                          top_idx=Sized(T, K, dtype="int32"), top_logprobs=Sized(T, K, dtype="float32"))
