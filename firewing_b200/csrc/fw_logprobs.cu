@@ -769,8 +769,12 @@ __global__ void __launch_bounds__(32 * W, 24 / W) k_token_logprobs(const __grid_
   auto logprob = [&](float x) {
     if (bad) return nan;
     if (empty || x == -INFINITY) return -INFINITY;
-    // in nats throughout: a representable result does not pass through a larger number
-    return __fsub_rn(__fmul_rn(__fsub_rn(x, whole.m), a.inv_temperature), ln_s);
+    // in nats throughout: a representable result does not pass through a
+    // larger number (the difference may: it is halved then)
+    float y = __fmul_rn(__fsub_rn(x, whole.m), a.inv_temperature);
+    if (y == -INFINITY)
+      y = __fmul_rn(__fsub_rn(__fmul_rn(x, 0.5f), __fmul_rn(whole.m, 0.5f)), __fmul_rn(a.inv_temperature, 2.0f));
+    return __fsub_rn(y, ln_s);
   };
   for (int i = tid; i < a.targets_per_row; i += kThreads) {
     const long long o = static_cast<long long>(t) * a.targets_per_row + i;

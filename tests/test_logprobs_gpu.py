@@ -306,3 +306,20 @@ def test_far_logits_and_temperatures(dtype, size, temperature):
         z[1] = -size - z[1].abs() * 2.0 ** -22 * size  # a few steps of f32 apart
         z[2:] *= size / 5
         check(z.to(DTYPES[dtype]), min(5, vocab), temperature=temperature)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("temperature", [3.0, 1e3, 1e6])
+def test_differences_that_pass_the_largest_value(dtype, temperature):
+    """Logits further apart than f32 holds, whose difference over the
+    temperature is a number again."""
+    high = torch.finfo(DTYPES[dtype]).max
+    for vocab in (3, 5000, 40000):
+        z = normal(26, 3, vocab, dtype=dtype)
+        z[0, 0], z[0, 1] = high, -high
+        z[1] = -high
+        z[1, vocab // 2] = high
+        z[2, 2] = 0.75 * high
+        z[2, :2] = -0.5 * high
+        targets = torch.tensor([[0, 1, vocab // 2, vocab - 1]] * 3, device="cuda", dtype=torch.int32)
+        check(z, min(3, vocab), targets, temperature=temperature)
