@@ -539,7 +539,15 @@ def _stream_of(stream, device: int) -> int:
     stream on which the tensors' other operations are."""
     if stream is None:
         return _torch._C._cuda_getCurrentRawStream(device)
-    return _stream(stream)
+    if isinstance(stream, int):
+        return stream
+    handle = getattr(stream, "cuda_stream", None)
+    if handle is None:
+        raise ValueError("stream must be a torch.cuda.Stream or a cudaStream_t handle")
+    # Every device's default stream has the handle 0: it would be another one there.
+    if getattr(stream, "device_index", device) != device:
+        raise ValueError("stream is on another device")
+    return handle
 
 
 def _call(device: int, function, *args) -> None:

@@ -185,3 +185,37 @@ def test_logprob_sizes_beyond_the_interface_are_refused(no_call, T, V, C, K):
     with pytest.raises(ValueError, match="2\\^31"):
         fw.token_logprobs(Sized(T, V, dtype="float32"), Sized(T, C, dtype="int32"), Sized(T, C, dtype="float32"),
                           top_idx=Sized(T, K, dtype="int32"), top_logprobs=Sized(T, K, dtype="float32"))
+
+
+class Queue:
+    """A torch.cuda.Stream, as far as the bindings look."""
+
+    def __init__(self, device, handle=0):
+        self.device_index, self.cuda_stream = device, handle
+
+
+def three_operators(stream):
+    h, f, i = "bfloat16", "float32", "int32"
+    yield lambda: fw.linear_epilogue(Sized(4, 8, dtype=h), Sized(2, 8, dtype=h), Sized(2, 4, dtype=h), stream=stream)
+    yield lambda: fw.route_scores(Sized(2, 4, dtype=f), Sized(2, 1, dtype=i), Sized(2, 1, dtype=f), stream=stream)
+    yield lambda: fw.token_logprobs(Sized(2, 4, dtype=f), entropy=Sized(2, dtype=f), stream=stream)
+
+
+@pytest.mark.parametrize("stream", [Queue(1), Queue(1, 77), "a name", object()])
+def test_streams_of_another_device_and_other_objects_are_refused(monkeypatch, stream):
+    # (a default stream's handle is 0 on every device)
+    pytest.importorskip("torch")
+    monkeypatch.setattr(moe, "_call", lambda *a: pytest.fail("reached the library"))
+    for call in three_operators(stream):
+        with pytest.raises(ValueError, match="stream"):
+            call()
+
+
+@pytest.mark.parametrize("stream,handle", [(Queue(0), 0), (Queue(0, 77), 77), (78, 78), (0, 0)])
+def test_streams_that_are_given_are_passed_on(monkeypatch, stream, handle):
+    pytest.importorskip("torch")
+    seen = []
+    monkeypatch.setattr(moe, "_call", lambda device, function, *args: seen.append((device, args[-1])))
+    for call in three_operators(stream):
+        call()
+    assert seen == [(0, handle)] * 3
