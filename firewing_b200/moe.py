@@ -480,6 +480,14 @@ def _import_torch() -> None:
     _torch = torch
 
 
+def _without_gradient(name: str) -> None:
+    """For a tensor that requires a gradient.  The operators have no backward
+    pass and write past autograd, like PyTorch's out= forms, which refuse the
+    same."""
+    if _torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which the operator has not: call it under torch.no_grad()")
+
+
 def _rows(t, name: str, codes: tuple, device: int = -1):
     """(dtype code, rows, columns, row stride, device) of a 2-D CUDA tensor
     with consecutive columns, after checking it (on `device`, if given)."""
@@ -499,6 +507,8 @@ def _rows(t, name: str, codes: tuple, device: int = -1):
         raise ValueError(f"{name} must have consecutive columns")
     if r > _MOST or c > _MOST:
         raise ValueError(f"{name}: a size is above 2^31 - 1")
+    if t.requires_grad:
+        _without_gradient(name)
     if r <= 1:
         s0 = c
     elif s0 < c:
@@ -521,6 +531,8 @@ def _dense(t, name: str, code: int, shape: tuple, device: int) -> Optional[int]:
         raise ValueError(f"{name} must be contiguous with shape {shape}")
     if found != code:
         raise ValueError(f"{name}: unsupported element type {t.dtype}")
+    if t.requires_grad:
+        _without_gradient(name)
     return t.data_ptr()
 
 

@@ -126,6 +126,8 @@ def test_the_products_wait_limit_has_bounds(seconds):
 class Sized:
     """What the bindings look at before a call, of a tensor on the current GPU."""
 
+    requires_grad = False
+
     def __init__(self, *shape, dtype):
         import torch
 
@@ -219,3 +221,35 @@ def test_streams_that_are_given_are_passed_on(monkeypatch, stream, handle):
     for call in three_operators(stream):
         call()
     assert seen == [(0, handle)] * 3
+
+
+def test_tensors_that_require_a_gradient_are_refused(monkeypatch):
+    """The outputs are written without autograd: a gradient would be lost."""
+    torch = pytest.importorskip("torch")
+    calls = []
+    monkeypatch.setattr(moe, "_call", lambda *a: calls.append(a))
+    h, f, i = "bfloat16", "float32", "int32"
+    w, x, y, bias, residual = (Sized(4, 8, dtype=h), Sized(2, 8, dtype=h), Sized(2, 4, dtype=h), Sized(4, dtype=f),
+                               Sized(2, 4, dtype=h))
+    z, b, weights = Sized(2, 4, dtype=f), Sized(4, dtype=f), Sized(2, 1, dtype=f)
+    logprobs, entropy = Sized(2, 1, dtype=f), Sized(2, dtype=f)
+
+    def linear():
+        fw.linear_epilogue(w, x, y, bias=bias, residual=residual, stream=0)
+
+    def route():
+        fw.route_scores(z, Sized(2, 1, dtype=i), weights, bias=b, stream=0)
+
+    def logprob():
+        fw.token_logprobs(z, Sized(2, 1, dtype=i), logprobs, entropy=entropy, stream=0)
+
+    for call, tensors in ((linear, (w, x, y, bias, residual)), (route, (z, b, weights)), (logprob, (z, logprobs, entropy))):
+        call()
+        for t in tensors:
+            t.requires_grad = True
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+            with torch.no_grad():
+                call()
+            t.requires_grad = False
+    assert len(calls) == 3 + 11
