@@ -1381,7 +1381,7 @@ int fw_linear_epilogue(const fw_linear_config* c, const void* w, const void* x, 
 int fw_primitive_set_wait_limit(uint64_t nanoseconds) {
   if (nanoseconds < 1000000ull || nanoseconds > 60000000000ull)
     return fail(FW_EINVAL, "the wait limit must be between 1 ms and 60 s");
-  fw::set_linear_wait_limit(nanoseconds);
+  fw::set_linear_wait_limit(static_cast<uint32_t>(nanoseconds / 1000));
   return FW_OK;
 }
 

@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
       for (int u = u0; ok && u < total; u += step) {
         const Tile w = tile_of(a, u);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, a.wait_ns) && !gave_up(tail))) {
+          if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, 1000ull * a.wait_us) && !gave_up(tail))) {
             give_up(tail);
             ok = false;
             break;
@@ -827,7 +827,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
       }
       // Copies already issued land before the CTA can exit.
       for (int j = it > stages ? it - stages : 0; j < it; ++j)
-        if (!mbar_wait_bounded(&tail->full[j % stages], (j / stages) & 1, a.wait_ns)) give_up(tail);
+        if (!mbar_wait_bounded(&tail->full[j % stages], (j / stages) & 1, 1000ull * a.wait_us)) give_up(tail);
     }
   } else if (warp == 1) {
     // ---------------- MMA ----------------
@@ -839,8 +839,8 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     for (int u = u0; ok && u < total; u += step) {
       for (int k = kb0; ok && k < kb1; k += chunk, ++ai) {
         const int buf = ai & 1;
-        if (!__all_sync(kAll, !gave_up(tail) &&
-                                  mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u, a.wait_ns))) {
+        if (!__all_sync(kAll, !gave_up(tail) && mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u,
+                                                                  1000ull * a.wait_us))) {
           give_up(tail);
           ok = false;
           break;
@@ -849,7 +849,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
         const uint32_t d = tmem + buf * acc_cols;
         const int end = min(kb1, k + chunk);
         for (int kb = k; kb < end; ++kb) {
-          if (!__all_sync(kAll, mbar_wait_bounded(&tail->full[st], phase, a.wait_ns))) {
+          if (!__all_sync(kAll, mbar_wait_bounded(&tail->full[st], phase, 1000ull * a.wait_us))) {
             give_up(tail);
             ok = false;
             break;
@@ -875,7 +875,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
     // Every MMA issued has completed once `drained` flips.
     if (elect_one()) umma_commit(&tail->drained);
     __syncwarp();
-    if (!mbar_wait_bounded(&tail->drained, 0, a.wait_ns)) give_up(tail);
+    if (!mbar_wait_bounded(&tail->drained, 0, 1000ull * a.wait_us)) give_up(tail);
   } else if (warp < 2 + kEpi) {
     // ---------------- epilogue ----------------
     const int set = (warp - 2) >> 2;
@@ -904,7 +904,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
       if (!a.swap) bias = fetch_bias(a, tail->bias[warp - 2], w.q0, set, kSets, lane);
       if (!CHUNKED) {
         const int buf = ai & 1;
-        const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, a.wait_ns);
+        const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, 1000ull * a.wait_us);
         if (!__all_sync(kAll, got)) {
           if (lane == 0) give_up(tail);
           break;
@@ -929,7 +929,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
         bool ok = true;
         for (int k = kb0; k < kb1; k += chunk, ++ai) {
           const int buf = ai & 1;
-          const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, a.wait_ns);
+          const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, 1000ull * a.wait_us);
           if (!__all_sync(kAll, got)) {
             if (lane == 0) give_up(tail);
             ok = false;
@@ -1042,7 +1042,7 @@ __global__ void __launch_bounds__(LOADERS ? kLoaderThreads : kMmaThreads, 1)
       issue();
       asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
       __syncwarp();
-      if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, a.wait_ns) && !gave_up(tail))) {
+      if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, 1000ull * a.wait_us) && !gave_up(tail))) {
         give_up(tail);
         break;
       }
@@ -1193,7 +1193,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const Tile w = tile_of(a, u, 2 * kBM);
       const int p0 = w.p0 + static_cast<int>(rank) * kBM, q0 = w.q0 + static_cast<int>(rank) * (a.bn / 2);
       for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
-        if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, a.wait_ns) && !gave_up(tail))) {
+        if (!__all_sync(kAll, mbar_wait_bounded(&tail->empty[st], phase, 1000ull * a.wait_us) && !gave_up(tail))) {
           give_up(tail);
           ok = false;
           break;
@@ -1215,7 +1215,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     // flipped.
     if (rank == 0)
       for (int j = it > stages ? it - stages : 0; j < it; ++j)
-        if (!mbar_wait_bounded(&tail->full[j % stages], (j / stages) & 1, a.wait_ns)) give_up(tail);
+        if (!mbar_wait_bounded(&tail->full[j % stages], (j / stages) & 1, 1000ull * a.wait_us)) give_up(tail);
   } else if (warp == 1) {
     if (rank == 0) {
       // ---------------- MMA, for both CTAs ----------------
@@ -1227,8 +1227,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const int chunk = CHUNKED ? a.chunk : a.kblocks;
       for (int at = 0, u = u0; ok && u < total; ++ai) {
         const int buf = ai & 1;
-        if (!__all_sync(kAll, !gave_up(tail) &&
-                                  mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u, a.wait_ns))) {
+        if (!__all_sync(kAll, !gave_up(tail) && mbar_wait_bounded(&tail->acc_empty[buf], ((ai >> 1) & 1) ^ 1u,
+                                                                  1000ull * a.wait_us))) {
           give_up(tail);
           break;
         }
@@ -1236,7 +1236,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         const uint32_t d = tmem + buf * a.bn;
         const int end = min(a.kblocks, at + chunk);
         for (int kb = at; kb < end; ++kb) {
-          if (!__all_sync(kAll, mbar_wait_bounded(&tail->full[st], phase, a.wait_ns))) {
+          if (!__all_sync(kAll, mbar_wait_bounded(&tail->full[st], phase, 1000ull * a.wait_us))) {
             give_up(tail);
             ok = false;
             break;
@@ -1287,7 +1287,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           finish_block(a, t0, w.q0 + c0, a.p_rows, w.q0 + valid, v, reinterpret_cast<float*>(stage), lane);
       };
       const auto await = [&](int buf) {
-        const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, a.wait_ns);
+        const bool got = mbar_wait_bounded(&tail->acc_full[buf], (ai >> 1) & 1, 1000ull * a.wait_us);
         if (!__all_sync(kAll, got)) {
           if (lane == 0) give_up(tail);
           return false;
@@ -1350,7 +1350,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   // which issues none, waits for it when its own tiles are done: a wait from
   // the start on would bound the whole product.
   __syncthreads();
-  if (warp == 1 && !mbar_wait_bounded(&tail->drained, 0, a.wait_ns)) give_up(tail);
+  if (warp == 1 && !mbar_wait_bounded(&tail->drained, 0, 1000ull * a.wait_us)) give_up(tail);
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();  // neither CTA leaves while the other's MMAs, copies or arrivals may reach it
@@ -1651,15 +1651,15 @@ Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const Clust
 
 }  // namespace
 
-static std::atomic<uint64_t> linear_wait_ns{2000000000ull};
-void set_linear_wait_limit(uint64_t ns) { linear_wait_ns.store(ns, std::memory_order_relaxed); }
+static std::atomic<uint32_t> linear_wait_us{2000000u};
+void set_linear_wait_limit(uint32_t us) { linear_wait_us.store(us, std::memory_order_relaxed); }
 
 cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_stride, const uint16_t* x,
                                    long long x_stride, cudaStream_t st) {
   DeviceAttrs dev;
   cudaError_t e = current_device_attrs(&dev);
   if (e != cudaSuccess) return e;
-  a.wait_ns = linear_wait_ns.load(std::memory_order_relaxed);
+  a.wait_us = linear_wait_us.load(std::memory_order_relaxed);
   const auto aligned = [](const void* p, long long stride, int dtype) {
     const long long size = dtype == kF32 ? 4 : 2;
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0);

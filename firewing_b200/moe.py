@@ -551,13 +551,14 @@ def _stream_of(stream, device: int) -> int:
     stream on which the tensors' other operations are."""
     if stream is None:
         return _torch._C._cuda_getCurrentRawStream(device)
-    if isinstance(stream, int):
-        return stream
-    handle = getattr(stream, "cuda_stream", None)
-    if handle is None:
-        raise ValueError("stream must be a torch.cuda.Stream or a cudaStream_t handle")
+    try:
+        handle, on = stream.cuda_stream, stream.device_index
+    except AttributeError:
+        if isinstance(stream, int):
+            return stream
+        raise ValueError("stream must be a torch.cuda.Stream or a cudaStream_t handle") from None
     # Every device's default stream has the handle 0: it would be another one there.
-    if getattr(stream, "device_index", device) != device:
+    if on != device:
         raise ValueError("stream is on another device")
     return handle
 
