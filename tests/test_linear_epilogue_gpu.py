@@ -328,3 +328,73 @@ def test_the_wait_limit_bounds_steps_and_not_the_product(out):
     part, err = reference(w, x[rows], None, "none", None)
     half_step = torch.finfo(y.dtype).eps / 2
     assert bool(((y[rows].double() - part).abs() <= err * (1 + half_step) + half_step * part.abs()).all())
+
+
+@pytest.mark.parametrize("activation", ["gelu", "gelu_tanh", "silu", "sigmoid"])
+@pytest.mark.parametrize("tokens", [1, 5, 200, 600])
+def test_activations_keep_their_digits(activation, tokens):
+    """f32 outputs of a sum v (the bias alone).  Each is a product with 2^e, e
+    an f32 of size |e|: k roundings on its way cost ln 2 k 2^-24 |e|, and the
+    rest is an exponential (2^-22), a reciprocal (2^-23), an addition and a
+    product (2^-24 each): 2^-21.  k is 2 for SiLU and the sigmoid (log2 e and the
+    product), 8 for the tanh form (the constants' five, v^2, a sum and a
+    product), 3 for the erf form (v^2, its constant, a sum), whose polynomial
+    adds nine roundings of sums up to 2 and its fit: 2^-20.  What is below f32's
+    normal numbers times v's size (at most 88) may be 0."""
+    k, fixed = {"silu": (2, 2.0 ** -21), "sigmoid": (2, 2.0 ** -21), "gelu_tanh": (8, 2.0 ** -21),
+                "gelu": (3, 2.0 ** -21 + 2.0 ** -20)}[activation]
+    rows = 4096
+    v = torch.logspace(-6, 2, rows // 2, dtype=torch.float64, device="cuda").float()
+    v = torch.cat((v, -v))
+    x = torch.ones(tokens, 64, device="cuda", dtype=torch.bfloat16)
+    w = torch.zeros(rows, 64, device="cuda", dtype=torch.bfloat16)
+    y = torch.empty(tokens, rows, device="cuda")
+    fw.linear_epilogue(w, x, y, bias=v, activation=activation)
+    a = v.double()
+    cubic = math.sqrt(2 / math.pi) * (a + 0.044715 * a ** 3)
+    want, e = {"silu": (a / (1 + torch.exp(-a)), a), "sigmoid": (1 / (1 + torch.exp(-a)), a),
+               "gelu_tanh": (a / (1 + torch.exp(-2 * cubic)), 2 * cubic),
+               "gelu": (0.5 * a * torch.special.erfc(-a * math.sqrt(0.5)), 0.5 * a * a)}[activation]
+    bound = (fixed + math.log(2.0) * k * 2.0 ** -24 * e.abs() / math.log(2.0)) * want.abs() * (1 + 2.0 ** -10)
+    bound = bound.clamp(max=1e300) + 88 * 2.0 ** -126
+    off = (y.double() - want).abs()
+    assert bool((off <= bound).all()), (float((off / bound).max()), float(v[(off / bound).max(0).values.argmax()]))
+
+
+def rms_error(T, N, K, x_shift=0, dtype="bf16"):
+    w = normal(1, N, K + 1, std=1 / math.sqrt(K), dtype=dtype)[:, x_shift:K + x_shift]
+    x = normal(2, T, K + 8, dtype=dtype)[:, :K]
+    if not x_shift:
+        w, x = w.contiguous(), x.contiguous()
+    y = torch.full((T, N), math.nan, device="cuda")
+    fw.linear_epilogue(w, x, y)
+    want = x.double() @ w.double().t()
+    return float(((y.double() - want).norm() / want.norm()))
+
+
+# tiles shared by a cluster, tiles of a CTA alone (w and x on the M side), pairs of CTAs, loaders
+@pytest.mark.parametrize("size,shift", [((64, 512, 65536), 0), ((24, 20000, 8192), 0), ((400, 20000, 8192), 0),
+                                        ((1100, 640, 16384), 0), ((2304, 2304, 8192), 0), ((4096, 4096, 16384), 0),
+                                        ((50, 20000, 8191), 1), ((700, 3001, 8191), 1)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_f32_outputs_of_long_sums(size, shift, dtype):
+    """The tensor cores cut sums off, which one accumulation over 8192 columns
+    shows: 1.4e-6 of the outputs, in pieces of 512 columns 4.4e-7 (measured).
+    The limit between them is their geometric mean."""
+    assert rms_error(*size, shift, dtype) <= 8e-7
+
+
+@pytest.mark.parametrize("size", [(1, 300, 512), (40, 300, 512), (300, 264, 512), (2304, 2304, 128)])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("shift", [1, 2, 4])
+def test_a_bias_at_any_address(size, out, shift):
+    """A slice of a fused parameter: the outputs are those of an aligned bias."""
+    T, N, K = size
+    w, x, r = normal(1, N, K, std=1 / math.sqrt(K)), normal(2, T, K), normal(3, T, N, dtype=out)
+    for dtype in ("bf16", "f32"):
+        store = normal(4, N + 8, dtype=dtype)
+        bias = store[shift:shift + N]
+        y, want = (torch.full((T, N), math.nan, device="cuda", dtype=DTYPES[out]) for _ in range(2))
+        check(w, x, y, bias, "gelu", r)
+        fw.linear_epilogue(w, x, want, bias=bias.clone(), activation="gelu", residual=r)
+        assert torch.equal(y, want)
