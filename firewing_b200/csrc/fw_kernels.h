@@ -429,7 +429,7 @@ struct LinearArgs {
   long long p_stride, q_stride;
   int p_rows, q_rows;
   int swap;                      // the M side is w
-  int vec;                       // bias, residual and y can be read and written 16 bytes at a time
+  int vec;                       // residual and y can be read and written 16 bytes at a time
   int bn, tiles_p, tiles_q, kblocks, stages, ring_bytes, tmem_cols;
   int chunk;                     // stages per accumulation (f32 outputs)
   uint32_t wait_us;              // bound of each wait (in 64 bits the launch took 0.3 us more of the host)

@@ -28,12 +28,13 @@
 // bytes at 6.5 TB/s, or the products at 1.66 PFLOP/s):
 //   8192 x 8192 x 2048 bf16, bias, GELU (tanh)  176-184 us  (165): the MMAs
 //   8192 x 8192 x 8192 bf16                        682 us  (661)
-//   8192 x 8192 x 2048 bf16, f32 out               242 us  (165): the f32
+//   8192 x 8192 x 2048 bf16, f32 out           242-257 us  (165): the f32
 //     outputs' way out of registers, which the next tile hides in part
 //   4096 x 2048 x 8192 bf16, residual          107-124 us   (83): 128 tiles
 //     in two waves of 74 pairs
 //   64 x 8192 x 2048 bf16, bias, SiLU             12.2 us  (5.4): the first
-//     loads' way, 32 blocks of a CTA, the epilogue, one after the other
+//     loads' way, 16 blocks of a CTA, the epilogue, one after the other (11.4
+//     where L2 keeps some of the weights)
 //   333 x 1001 x 1999 f16, bias, GELU, residual   15.7 us  (1.0): the loaders
 //     (29 to 32 bytes per ns and SM), the joint, code that runs once
 //   8000 x 8001 x 2001 f16                         886 us  (154): the loaders
@@ -276,10 +277,12 @@ __device__ __forceinline__ float relu(float x) {
   return r;
 }
 // x/2 (1 + erf(x / sqrt 2)) = max(x, 0) - |x|/2 erfc(|x| / sqrt 2) per half,
-// with erfc(z) = t 2^(-z^2 log2 e + g(t)), t = 1 / (1 + z / 2): t takes z >= 0
-// to (0, 1], where log2(erfc(z) exp(z^2) / t) is smooth.  g is its least
-// squares fit at the Chebyshev points, degree 9: erfc to 1.1e-7 relative for
-// every z, 2.3e-7 in f32.
+// with erfc(z) = t 2^(-z^2 log2 e + g(t)), t = 1 / (1 + z / 2), the form of
+// erfcc in Press et al., Numerical Recipes: t takes z >= 0 to (0, 1], where
+// log2(erfc(z) exp(z^2) / t) is smooth.  g is its least squares fit at the
+// Chebyshev points, degree 9, made for this file: erfc to 1.1e-7 relative for
+// every z.  In f32 the exponent's three roundings come on top, 3 2^-24 of its
+// size in nats, x^2 / 2: of a result 4e-7 near 0, 8e-6 at x = -12.
 __device__ __forceinline__ F2 gelu2(F2 v) {
   constexpr float g[10] = {-1.82574821f, 1.44272923f,  0.539700329f, 0.139632389f,  -0.268766135f,
                            0.402343214f, -1.63778341f, 2.14749932f,  -1.18612599f, 0.246519342f};
@@ -342,8 +345,11 @@ __device__ __forceinline__ F2 finite_below(F2 v) {
 }
 // The activations in f32, on N packed pairs.  gelu_tanh is 0.5 x (1 + tanh u)
 // = x / (1 + exp(-2u)) with u = sqrt(2/pi) (x + 0.044715 x^3): like SiLU and
-// the sigmoid a quotient without cancellation, whose relative error stays near
-// 2^-21 everywhere, far under the rounding of a 16-bit y.
+// the sigmoid a quotient without cancellation.  Its relative error is 2^-21 and
+// what the exponent's roundings make of its size in nats: 2 2^-24 of it for
+// SiLU and the sigmoid (2^-17 at x = -87), 8 2^-24 for the tanh form, under
+// the rounding of a 16-bit y.  The reciprocal is 0 where 1 + 2^z passes 2^126:
+// results below |x| 2^-126 are 0.
 template <int N>
 __device__ __forceinline__ void activate_pairs(int act, F2 (&v)[N]) {
   if (act == kActNone) return;
@@ -1588,8 +1594,13 @@ struct Plan {
 // faster but for the pair and for CTAs that run through many tiles.  f32
 // outputs, which leave from registers, cost CTAs with several tiles 24 ns per
 // column and tile more, and the pair 6 us per tile.
-// Measured against the best of a sweep (us): 64 x 8192 x 2048 10.5 / 10.5,
-// 128 x 2048 x 2048 8.1 / 8.1, 512 x 2048 x 2048 11.0 / 11.0.
+// The widths are what the sweeps ran.  w on the M side: tokens come in any
+// number, and 96, 112 and 192 leave less of the last tile empty than the powers
+// of two do (112 takes 333 tokens in three tiles).  x on the M side: rows are
+// mostly multiples of 128, and a narrower tile only loads x more often.
+// Measured against the best of a sweep (us, bf16 without an epilogue, the same
+// operands again and again): 64 x 8192 x 2048 10.5 / 10.5, 128 x 2048 x 2048
+// 8.1 / 8.1, 512 x 2048 x 2048 11.0 / 11.0.
 Plan make_plan(const LinearArgs& a, bool tma, bool chunked, int sms, const ClusterRoom& room) {
   const int kblocks = (a.cols + kBK - 1) / kBK;
   const double rate = tma ? 130.0 : 29.0;
@@ -1664,8 +1675,8 @@ cudaError_t launch_linear_epilogue(LinearArgs a, const uint16_t* w, long long w_
     const long long size = dtype == kF32 ? 4 : 2;
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0);
   };
-  a.vec = aligned(a.y, a.y_stride, a.out_dtype) && aligned(a.bias, 0, a.bias_dtype) &&
-          aligned(a.residual, a.res_stride, a.res_dtype);
+  // (the bias is read an element at a time)
+  a.vec = aligned(a.y, a.y_stride, a.out_dtype) && aligned(a.residual, a.res_stride, a.res_dtype);
 
   const bool tma = tma_can_read(w, a.rows, w_stride) && tma_can_read(x, a.tokens, x_stride);
   const bool chunked = a.out_dtype == kF32;
