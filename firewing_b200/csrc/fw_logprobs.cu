@@ -26,11 +26,13 @@
 // order that depends on the shape and the row's 16-byte alignment alone.
 //
 // Measured on B200, device time in a stream of calls (floor: the logits at 6.5
-// TB/s): 2048 x 131072 bf16 93 us without alternatives, 109 with five (82);
-// 4096 x 32000 with five 71 (40); 64 x 131072 f32 with eight 15.4 (5.2); one
+// TB/s): 2048 x 131072 bf16 92 us without alternatives, 108 with five (82);
+// 4096 x 32000 with five 69 (40); 64 x 131072 f32 with eight 15.4 (5.2); one
 // row 9.5.  Many rows are bound by instructions, 9.2 per value (an exponential,
-// packed sums, raising, unpacking, maximum) at 64 % of the issue slots; few
-// rows by the chain of a row's beginning and end.
+// packed sums, raising, unpacking, maximum) at 64 % of the issue slots, and by
+// latency, with 35 % of the warps resident; few rows by the chain of a row's
+// beginning and end.  Rows nearly all of one finite mask value overflow the
+// lists: 2048 x 131072 404 us.
 #include <algorithm>
 #include <cstdint>
 
