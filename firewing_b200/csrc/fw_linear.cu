@@ -684,15 +684,21 @@ __device__ __forceinline__ uint4 first_of(uint4 v, int n) {
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
+// (volatile: stays behind the wait for the previous kernel, which may write it)
+__device__ __forceinline__ uint4 ldg_word(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 // The n (0..8) 16-bit elements at p, the others 0, from the one or two
 // aligned 16-byte words that hold them (no other word is read).
 __device__ __forceinline__ uint4 load_chunk(const uint16_t* p, int n) {
   if (n <= 0) return make_uint4(0, 0, 0, 0);
   const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
   const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) - off);
-  const uint4 a = __ldg(s);
+  const uint4 a = ldg_word(s);
   uint4 b = make_uint4(0, 0, 0, 0);
-  if (off + 2 * n > 16) b = __ldg(s + 1);
+  if (off + 2 * n > 16) b = ldg_word(s + 1);
   uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   realign<8>(w, off);
   const uint4 v = make_uint4(w[0], w[1], w[2], w[3]);

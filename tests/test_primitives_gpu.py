@@ -153,3 +153,22 @@ def test_the_current_stream_is_the_default():
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("K", [511, 1023, 999])
+def test_a_chain_of_products_whose_rows_have_tails(K):
+    """Each reads what the previous one has just written, from rows that are no
+    whole words; their kernels overlap."""
+    w = (torch.randn(K, K, device="cuda") * K ** -0.5).bfloat16()
+    x = torch.randn(2, K, device="cuda").bfloat16()
+    for T in (1, 2):
+        chain = [x[:T].clone()] + [torch.zeros(T, K, device="cuda", dtype=torch.bfloat16) for _ in range(40)]
+        single = [c.clone() for c in chain]
+        torch.cuda.synchronize()
+        for a, b in zip(single, single[1:]):
+            fw.linear_epilogue(w, a, b)
+            torch.cuda.synchronize()
+        for a, b in zip(chain, chain[1:]):
+            fw.linear_epilogue(w, a, b)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(chain, single))
