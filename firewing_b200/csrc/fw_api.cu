@@ -22,13 +22,19 @@ namespace {
 // error never allocates).
 thread_local char g_last_error[512] = "";
 
+// The runtime keeps a refused call's error until it is asked for: a later call
+// would take it for that of its own launch.
+int reported(int code) {
+  if (code == FW_ECUDA || code == FW_ENOMEM) cudaGetLastError();
+  return code;
+}
 int fail(int code, const char* msg) {
   std::snprintf(g_last_error, sizeof g_last_error, "%s", msg);
-  return code;
+  return reported(code);
 }
 int fail(int code, const char* what, const char* detail) {
   std::snprintf(g_last_error, sizeof g_last_error, "%s: %s", what, detail);
-  return code;
+  return reported(code);
 }
 int fail(int code, const std::string& msg) { return fail(code, msg.c_str()); }
 

@@ -172,3 +172,22 @@ def test_a_chain_of_products_whose_rows_have_tails(K):
             fw.linear_epilogue(w, a, b)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(chain, single))
+
+
+def test_an_error_stays_with_its_call():
+    """A call that CUDA refuses (here a wait inside a capture) says so itself and
+    leaves nothing to the next one."""
+    a = torch.randn(64, device="cuda").bfloat16()
+    out = torch.empty_like(a)
+    fw.linear_epilogue(a.view(1, 64), a.view(1, 64), torch.empty(1, 1, device="cuda"))
+    fw.swiglu_bf16(a, a, 64, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        graph.capture_begin()
+        with pytest.raises(fw.FwError, match="captur"):
+            fw.primitive_status()
+        with pytest.raises(RuntimeError):
+            graph.capture_end()
+    fw.swiglu_bf16(a, a, 64, out)
+    fw.primitive_status()
